@@ -1,0 +1,102 @@
+/*
+ * musev_tokens.h -- C ABI of the token-transformer operators of libmusev_hip.so (gfx950): packed attention, rotary positions with
+ * several axes, the gated residual norm and the int8 projection.  Conventions of musev_hip.h: extern "C", plain device pointers and
+ * explicit strides, no hidden allocation, no global mutable state except the thread-local last-error string, every launch on the
+ * hipStream_t passed as `stream` of the CURRENT device, 0 = ok / negative = MV_ERR_* with mv_last_error().
+ * Matrices are rows x columns with unit inner stride; row strides (ld*) are in elements.  Element type: MV_F16 or MV_BF16.
+ */
+#ifndef MUSEV_TOKENS_H
+#define MUSEV_TOKENS_H
+
+#include "musev_hip.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define MV_TOKENS_ABI_VERSION 1
+int mv_tokens_abi_version(void);
+
+#define MV_F16 0
+#define MV_BF16 1
+
+/* ---- packed attention -------------------------------------------------------------------------------------------------------
+ * Sequences of different lengths packed row after row; query head h reads key / value head h / (heads / kv_heads).
+ *   out[i] = sum_j softmax_j(scale * q_i . k_j) v_j   over the keys j < kv_len of i's sequence, with `causal` only
+ *   j <= i + kv_len - q_len (the last query sees every key);  a row that sees no key is 0.
+ * A wave's rows are (query, head of the group) pairs: row r of a (sequence, key / value head) is query r / group, head r % group.
+ * `items` (device, n_items x 8 int32), made by musev_amd.token_ops.attention_plan:
+ *   {first query row, q_len, first key row, kv_len, first packed row, key begin, key end, partial slot or -1}
+ * An item with a slot writes its unnormalised sums and the rows' maxima / sums to the workspace; `joins` (device, n_joins x 8 int32:
+ *   {first query row, q_len, kv_len, first packed row, first slot, slots, 0, 0}) says which slots make up which rows.            */
+typedef struct mv_attn_packed_desc {
+    const void *q, *k, *v;
+    void* out;
+    const int32_t *items, *joins;
+    void* workspace;               /* mv_attention_packed_workspace_bytes(n_slots, kv_heads, d, tile_rows) bytes, 16-byte aligned */
+    int64_t workspace_bytes;
+    int32_t n_items, n_joins, n_slots, tile_rows;   /* tile_rows: packed rows per item: 128, or 32 (few-row items) */
+    int32_t ldq, ldk, ldv, ldo;
+    int32_t heads, kv_heads, d, dtype, causal;
+    float scale;
+} mv_attn_packed_desc;
+int64_t mv_attention_packed_workspace_bytes(int32_t n_slots, int32_t kv_heads, int32_t d, int32_t tile_rows);
+int mv_attention_packed(const mv_attn_packed_desc* d, void* stream);
+
+/* ---- rotary positions with several axes ----------------------------------------------------------------------------------------
+ * Pair p of a head (p < pairs) turns by position[token, axis[p]] * turns[p] full turns:
+ *   (a, b) -> (a cos - b sin, a sin + b cos);  elements 2 p, 2 p + 1 (halves = 0) or p, p + pairs (halves = 1) of the head;
+ * elements from 2 * pairs on pass through.  k may be null.  Outputs may be the inputs themselves.                                 */
+typedef struct mv_rotary_desc {
+    const void *q, *k;
+    void *out_q, *out_k;
+    const void* positions;         /* [tokens, axes] int32 or fp32 (positions_f32), row stride ldp */
+    const double* turns;           /* [pairs] turns per position step */
+    const int32_t* axis;           /* [pairs] */
+    int64_t tokens;
+    int32_t ldq, ldk, ldoq, ldok, ldp;
+    int32_t heads, kv_heads, d, pairs, axes, halves, positions_f32, dtype;
+} mv_rotary_desc;
+int mv_rotary_axes(const mv_rotary_desc* d, void* stream);
+
+/* ---- gated residual norm ---------------------------------------------------------------------------------------------------------
+ *   y = post ? N(f) * post_gamma + post_beta : f          N: rms (x / sqrt(mean x^2 + eps)) or layer ((x - mean) / sqrt(var + eps))
+ *   s = alpha * x + gate[g] * y                            g: group_index[row], or row / rows_per_group; gate null: 1
+ *   h = (N(s) * pre_gamma + pre_beta) * (1 + scale[g]) + shift[g]   (only with norm_out)
+ * stream_out = s, norm_out = h; every statistic and s itself in fp32, each output rounded once.  A row whose group_index lies outside
+ * [0, groups) is filled with NaN.  stream_out may be x or f, norm_out may be f or x.                                                  */
+typedef struct mv_gated_norm_desc {
+    const void *x, *f;
+    void *stream_out, *norm_out;
+    const void *post_gamma, *post_beta, *pre_gamma, *pre_beta, *gate, *scale, *shift;
+    const int32_t* group_index;
+    int64_t rows, groups, rows_per_group;
+    int32_t c, ldx, ldf, lds, ldh, ldg, ldsc, ldsh;
+    int32_t post, layer, dtype;
+    float alpha, post_eps, pre_eps;
+} mv_gated_norm_desc;
+int mv_gated_residual_norm(const mv_gated_norm_desc* d, void* stream);
+
+/* ---- int8 projection -----------------------------------------------------------------------------------------------------------------
+ * mv_quantize_rows_i8: scale[m] = max_k |x[m, k]| / 127, code = round-to-nearest-even(127 x / max|x|); columns K .. ldc - 1 of the codes
+ * become 0; a row of zeros has scale 0; a row that holds an infinity or NaN has that scale and codes 0 (its products are NaN).
+ * mv_gemm_i8: out = act(a_scale[m] * w_scale[n] * sum_k a[m, k] w[n, k] + bias[n]) + residual[m, n];  the sum is exact (int32).
+ * lda, ldw: multiples of 128, the columns from K on are 0.                                                                             */
+int mv_quantize_rows_i8(const void* x, int64_t ldx, int64_t rows, int32_t k, int32_t dtype, int8_t* codes, int64_t ldc, float* scale,
+                        void* stream);
+typedef struct mv_gemm_i8_desc {
+    const int8_t *a, *w;
+    const float *a_scale, *w_scale;
+    const void *bias, *residual;
+    void* out;
+    int64_t M;
+    int32_t N, kp;                 /* kp: K rounded up to 128 */
+    int64_t lda, ldw, ldr, ldo;
+    int32_t act, dtype;
+} mv_gemm_i8_desc;
+int mv_gemm_i8(const mv_gemm_i8_desc* d, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif

@@ -141,6 +141,59 @@ SIGNATURES = {
     "mv_probe_tr16": (_i32, [_vp, _vp, _vp]),
 }
 
+# the entry points of include/musev_tokens.h (musev_amd.token_ops)
+class AttnPackedDesc(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("out", C.c_void_p), ("items", C.c_void_p), ("joins", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+        ("n_items", C.c_int32), ("n_joins", C.c_int32), ("n_slots", C.c_int32), ("tile_rows", C.c_int32),
+        ("ldq", C.c_int32), ("ldk", C.c_int32), ("ldv", C.c_int32), ("ldo", C.c_int32),
+        ("heads", C.c_int32), ("kv_heads", C.c_int32), ("d", C.c_int32), ("dtype", C.c_int32), ("causal", C.c_int32),
+        ("scale", C.c_float),
+    ]
+
+
+class RotaryDesc(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("out_q", C.c_void_p), ("out_k", C.c_void_p), ("positions", C.c_void_p),
+        ("turns", C.c_void_p), ("axis", C.c_void_p), ("tokens", C.c_int64),
+        ("ldq", C.c_int32), ("ldk", C.c_int32), ("ldoq", C.c_int32), ("ldok", C.c_int32), ("ldp", C.c_int32),
+        ("heads", C.c_int32), ("kv_heads", C.c_int32), ("d", C.c_int32), ("pairs", C.c_int32), ("axes", C.c_int32), ("halves", C.c_int32),
+        ("positions_f32", C.c_int32), ("dtype", C.c_int32),
+    ]
+
+
+class GatedNormDesc(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("f", C.c_void_p), ("stream_out", C.c_void_p), ("norm_out", C.c_void_p),
+        ("post_gamma", C.c_void_p), ("post_beta", C.c_void_p), ("pre_gamma", C.c_void_p), ("pre_beta", C.c_void_p),
+        ("gate", C.c_void_p), ("scale", C.c_void_p), ("shift", C.c_void_p), ("group_index", C.c_void_p),
+        ("rows", C.c_int64), ("groups", C.c_int64), ("rows_per_group", C.c_int64),
+        ("c", C.c_int32), ("ldx", C.c_int32), ("ldf", C.c_int32), ("lds", C.c_int32), ("ldh", C.c_int32), ("ldg", C.c_int32), ("ldsc", C.c_int32),
+        ("ldsh", C.c_int32), ("post", C.c_int32), ("layer", C.c_int32), ("dtype", C.c_int32),
+        ("alpha", C.c_float), ("post_eps", C.c_float), ("pre_eps", C.c_float),
+    ]
+
+
+class GemmI8Desc(C.Structure):
+    _fields_ = [
+        ("a", C.c_void_p), ("w", C.c_void_p), ("a_scale", C.c_void_p), ("w_scale", C.c_void_p), ("bias", C.c_void_p), ("residual", C.c_void_p),
+        ("out", C.c_void_p), ("M", C.c_int64), ("N", C.c_int32), ("kp", C.c_int32),
+        ("lda", C.c_int64), ("ldw", C.c_int64), ("ldr", C.c_int64), ("ldo", C.c_int64), ("act", C.c_int32), ("dtype", C.c_int32),
+    ]
+
+
+MV_TOKENS_ABI_VERSION = 1
+TOKEN_SIGNATURES = {
+    "mv_tokens_abi_version": (_i32, []),
+    "mv_attention_packed_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32]),
+    "mv_attention_packed": (_i32, [C.POINTER(AttnPackedDesc), _vp]),
+    "mv_rotary_axes": (_i32, [C.POINTER(RotaryDesc), _vp]),
+    "mv_gated_residual_norm": (_i32, [C.POINTER(GatedNormDesc), _vp]),
+    "mv_quantize_rows_i8": (_i32, [_vp, _i64, _i64, _i32, _i32, _vp, _i64, _vp, _vp]),
+    "mv_gemm_i8": (_i32, [C.POINTER(GemmI8Desc), _vp]),
+}
+
 _lib = None
 
 
@@ -159,12 +212,14 @@ def load() -> C.CDLL:
     # smoke() in one process).  Tensors, streams and graphs are torch's: its runtime is the one that must be resident.
     import torch  # noqa: F401
     lib = C.CDLL(LIB_PATH)
-    for name, (res, args) in SIGNATURES.items():
+    for name, (res, args) in {**SIGNATURES, **TOKEN_SIGNATURES}.items():
         fn = getattr(lib, name)  # AttributeError if the symbol is missing: the ABI is incomplete
         fn.restype = res
         fn.argtypes = args
     if lib.mv_abi_version() != MV_ABI_VERSION:
         raise MuseVHipError(f"ABI mismatch: library {lib.mv_abi_version()} vs binding {MV_ABI_VERSION}")
+    if lib.mv_tokens_abi_version() != MV_TOKENS_ABI_VERSION:
+        raise MuseVHipError(f"token ABI mismatch: library {lib.mv_tokens_abi_version()} vs binding {MV_TOKENS_ABI_VERSION}")
     _lib = lib
     return lib
 

@@ -18,6 +18,15 @@ for f in lib gemm norm attention elementwise ffn tsa xab; do
     pids+=($!)
   fi
 done
+# the token-transformer kernels: no packed-fp32 instructions (some of their operand forms gave wrong results on the MI355X, see common.h)
+TOK="tok_attention tok_rotary tok_norm tok_linear"
+TOK_FLAGS="-Xclang -target-feature -Xclang -packed-fp32-ops"
+for f in $TOK; do
+  if [ ! -f $OBJ/$f.o ] || [ $f.hip -nt $OBJ/$f.o ] || [ common.h -nt $OBJ/$f.o ] || [ tok_common.h -nt $OBJ/$f.o ] || [ ../../include/musev_tokens.h -nt $OBJ/$f.o ] || [ ../../include/musev_hip.h -nt $OBJ/$f.o ]; then
+    $HIPCC $FLAGS $TOK_FLAGS -c $f.hip -o $OBJ/$f.o &
+    pids+=($!)
+  fi
+done
 for p in "${pids[@]:-}"; do [ -n "$p" ] && wait $p; done
-$HIPCC --offload-arch=gfx950 -shared -fPIC -o $LIB $OBJ/lib.o $OBJ/gemm.o $OBJ/norm.o $OBJ/attention.o $OBJ/elementwise.o $OBJ/ffn.o $OBJ/tsa.o $OBJ/xab.o
+$HIPCC --offload-arch=gfx950 -shared -fPIC -o $LIB $OBJ/lib.o $OBJ/gemm.o $OBJ/norm.o $OBJ/attention.o $OBJ/elementwise.o $OBJ/ffn.o $OBJ/tsa.o $OBJ/xab.o $(for f in $TOK; do echo $OBJ/$f.o; done)
 echo "built $(pwd)/$LIB"

@@ -19,11 +19,15 @@ import torch
 from . import _lib
 from ._lib import (AttnDesc, GemmDesc, MV_ACT_NONE, MV_ACT_SILU, MV_GEMM_CONV3X3, MV_GEMM_LINEAR, MV_GEMM_TCONV3,
                    check)
+from .token_ops import (AttentionPlan, Int8Rows, RotaryTable, attention_packed, attention_plan, gated_residual_norm, gemm_i8, linear_i8,
+                        pack_weight_i8, quantize_rows_i8, rotary_axes, rotary_table)
 
 __all__ = [
     "gemm", "ln_fold_applies", "fold_layernorm", "conv3x3", "tconv3", "groupnorm", "groupnorm_fold_linear", "xab_fused_applies", "pack_xab_q", "xattn_block", "layernorm", "attention", "temporal_attention", "geglu", "silu", "add", "softmax_rows_",
     "conv3x3_cin_small", "conv3x3_cin_small_gemm", "pad_cols", "conv3x3_cout_small", "conv3x3_direct", "timestep_embedding", "zero_rows", "bcthw_to_bthwc", "bthwc_to_bcthw",
     "window_gather", "window_scatter_add", "window_units_reduce", "cfg_ddim_step", "cfg_affine_step", "pack_conv_weight", "probe_tr16", "MV_ACT_NONE", "MV_ACT_SILU",
+    "AttentionPlan", "attention_plan", "attention_packed", "RotaryTable", "rotary_table", "rotary_axes", "gated_residual_norm", "Int8Rows",
+    "pack_weight_i8", "quantize_rows_i8", "gemm_i8", "linear_i8",
 ]
 
 
