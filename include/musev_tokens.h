@@ -24,23 +24,24 @@ int mv_tokens_abi_version(void);
  * Sequences of different lengths packed row after row; query head h reads key / value head h / (heads / kv_heads).
  *   out[i] = sum_j softmax_j(scale * q_i . k_j) v_j   over the keys j < kv_len of i's sequence, with `causal` only
  *   j <= i + kv_len - q_len (the last query sees every key);  a row that sees no key is 0.
- * A wave's rows are (query, head of the group) pairs: row r of a (sequence, key / value head) is query r / group, head r % group.
- * `items` (device, n_items x 8 int32), made by musev_amd.token_ops.attention_plan:
- *   {first query row, q_len, first key row, kv_len, first packed row, key begin, key end, partial slot or -1}
- * An item with a slot writes its unnormalised sums and the rows' maxima / sums to the workspace; `joins` (device, n_joins x 8 int32:
- *   {first query row, q_len, kv_len, first packed row, first slot, slots, 0, 0}) says which slots make up which rows.            */
+ * A (sequence, key / value head) has q_len * group packed rows: row r is query r / group, head r % group of the group.
+ * `items` (device, 8 int32 each), made by musev_amd.token_ops.attention_plan: n_items of 128 packed rows, then n_few of 32:
+ *   {first query row, q_len, first key row, kv_len, first packed row, key begin, key end, first workspace row or -1}
+ * An item with a workspace row writes its unnormalised sums and the rows' references / sums there; `joins` (device, 8 int32 each:
+ *   {first query row, q_len, kv_len, first packed row, first workspace row, parts, rows per part, 0}) says which parts make up which rows.
+ * Rows must be 16-byte aligned.                                                                                                        */
 typedef struct mv_attn_packed_desc {
     const void *q, *k, *v;
     void* out;
     const int32_t *items, *joins;
-    void* workspace;               /* mv_attention_packed_workspace_bytes(n_slots, kv_heads, d, tile_rows) bytes, 16-byte aligned */
-    int64_t workspace_bytes;
-    int32_t n_items, n_joins, n_slots, tile_rows;   /* tile_rows: packed rows per item: 128, or 32 (few-row items) */
+    void* workspace;               /* with joins: mv_attention_packed_workspace_bytes(ws_rows, kv_heads, d) bytes, 16-byte aligned */
+    int64_t workspace_bytes, ws_rows;
+    int32_t n_items, n_few, n_joins;
     int32_t ldq, ldk, ldv, ldo;
     int32_t heads, kv_heads, d, dtype, causal;
     float scale;
 } mv_attn_packed_desc;
-int64_t mv_attention_packed_workspace_bytes(int32_t n_slots, int32_t kv_heads, int32_t d, int32_t tile_rows);
+int64_t mv_attention_packed_workspace_bytes(int64_t ws_rows, int32_t kv_heads, int32_t d);
 int mv_attention_packed(const mv_attn_packed_desc* d, void* stream);
 
 /* ---- rotary positions with several axes ----------------------------------------------------------------------------------------

@@ -145,8 +145,8 @@ SIGNATURES = {
 class AttnPackedDesc(C.Structure):
     _fields_ = [
         ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("out", C.c_void_p), ("items", C.c_void_p), ("joins", C.c_void_p),
-        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
-        ("n_items", C.c_int32), ("n_joins", C.c_int32), ("n_slots", C.c_int32), ("tile_rows", C.c_int32),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("ws_rows", C.c_int64),
+        ("n_items", C.c_int32), ("n_few", C.c_int32), ("n_joins", C.c_int32),
         ("ldq", C.c_int32), ("ldk", C.c_int32), ("ldv", C.c_int32), ("ldo", C.c_int32),
         ("heads", C.c_int32), ("kv_heads", C.c_int32), ("d", C.c_int32), ("dtype", C.c_int32), ("causal", C.c_int32),
         ("scale", C.c_float),
@@ -186,7 +186,7 @@ class GemmI8Desc(C.Structure):
 MV_TOKENS_ABI_VERSION = 1
 TOKEN_SIGNATURES = {
     "mv_tokens_abi_version": (_i32, []),
-    "mv_attention_packed_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32]),
+    "mv_attention_packed_workspace_bytes": (_i64, [_i64, _i32, _i32]),
     "mv_attention_packed": (_i32, [C.POINTER(AttnPackedDesc), _vp]),
     "mv_rotary_axes": (_i32, [C.POINTER(RotaryDesc), _vp]),
     "mv_gated_residual_norm": (_i32, [C.POINTER(GatedNormDesc), _vp]),

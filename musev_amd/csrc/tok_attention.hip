@@ -1,48 +1,423 @@
 // tok_attention.hip -- packed attention (include/musev_tokens.h: mv_attention_packed).
+//
+// One pass over the keys with a running maximum and sum.  A (sequence, key / value head) has q_len * group packed rows, row r = query
+// r / group, head r % group of the group: the heads that share keys share the tile that holds them, and one token of a wide group is a
+// tile of its own.  Scores are formed transposed, S^T = K Q^T with v_mfma_32x32x16: lane l then owns ONE packed row (column l & 31) and 16
+// of every 32 keys (those with bit 2 = l >> 5), so maxima and sums are in-lane up to one exchange between the two half waves, and P^T
+// already lies as the second operand of O^T += V^T P^T wants it: the contraction may walk its keys in any order, so step s takes the keys
+// in the order the scores' registers hold them (16 s + 4 h + 0..3, 16 s + 8 + 4 h + 0..3 for half h) and V^T is read to match with the
+// transposing LDS read (4 keys x 16 columns per 16 lanes).
+// K and V tiles go global -> LDS directly (16 bytes per lane).  LDS rows are 128 or 256 bytes; the 16-byte slots of a row are permuted by
+// an XOR with row bits, applied to the source column each lane fetches, so that both the 16-byte reads of K (16 rows, one column) and the
+// transposing reads of V (4 rows x 64 bytes per half wave) touch every bank once.
+// Two forms of one kernel:
+//   wide (FEW = false): 4 waves x 32 packed rows share 64-key tiles, two stages, one barrier per tile; two blocks per CU
+//   few rows (FEW = true): 32 packed rows (a token of a group of heads); the 4 waves walk different 32-key tiles of their own and are joined
+//                  at the end: what counts here is the number of bytes in flight
 #include "tok_common.h"
 
 extern "C" int mv_tokens_abi_version(void) { return MV_TOKENS_ABI_VERSION; }
 
 struct PackedItem {
-    int q_row, q_len, k_row, kv_len, m0, key_begin, key_end, slot;
+    int q_row, q_len, k_row, kv_len, m0, key_begin, key_end, ws_row;
+};
+struct PackedJoin {
+    int q_row, q_len, kv_len, m0, ws_row, parts, rows, pad;
 };
 
-// one wave per packed row: 64 lanes hold the row's head dim two columns apart, the keys walk one after the other
-template <typename T>
-__global__ __launch_bounds__(256) void attention_rows_kernel(const mv_attn_packed_desc p) {
-    const PackedItem it = ((const PackedItem*)p.items)[blockIdx.x / p.kv_heads];
-    const int kvh = blockIdx.x % p.kv_heads, group = p.heads / p.kv_heads, lane = threadIdx.x & 63;
-    for (int t = threadIdx.x >> 6; t < p.tile_rows; t += 4) {
-        const int64_t r = (int64_t)it.m0 + t;
-        if (r >= (int64_t)it.q_len * group) break;
-        const int i = (int)(r / group), h = kvh * group + (int)(r % group);
-        const T* q = (const T*)p.q + (int64_t)(it.q_row + i) * p.ldq + (int64_t)h * p.d;
-        const int c0 = lane, c1 = lane + 64;
-        const float q0 = c0 < p.d ? (float)q[c0] : 0.f, q1 = c1 < p.d ? (float)q[c1] : 0.f;
-        const int64_t seen = p.causal ? (int64_t)i + it.kv_len - it.q_len + 1 : it.kv_len;
-        const int end = (int)(seen < it.key_end ? seen : it.key_end);
-        float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-        for (int j = it.key_begin; j < end; ++j) {
-            const T* k = (const T*)p.k + (int64_t)(it.k_row + j) * p.ldk + (int64_t)kvh * p.d;
-            const T* v = (const T*)p.v + (int64_t)(it.k_row + j) * p.ldv + (int64_t)kvh * p.d;
-            const float s = p.scale * wave_sum((c0 < p.d ? q0 * (float)k[c0] : 0.f) + (c1 < p.d ? q1 * (float)k[c1] : 0.f));
-            const float mn = fmaxf(m, s);
-            const float a = m == -INFINITY ? 0.f : __expf(m - mn), e = __expf(s - mn);
-            l = l * a + e;
-            if (c0 < p.d) o0 = o0 * a + e * (float)v[c0];
-            if (c1 < p.d) o1 = o1 * a + e * (float)v[c1];
-            m = mn;
+__device__ __forceinline__ float16v mfma_32x32x16(half8v a, half8v b, float16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ float16v mfma_32x32x16(bf16x8 a, bf16x8 b, float16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+
+template <typename T> struct ExpBits;   // both elements of a dword: exponent mask, and what lifts an all-ones exponent into the sign bit
+template <> struct ExpBits<half_t> { static constexpr unsigned mask = 0x7c007c00u, one = 0x04000400u; };
+template <> struct ExpBits<bf16_t> { static constexpr unsigned mask = 0x7f807f80u, one = 0x00800080u; };
+
+template <int DC, bool FEW>
+struct PackedCfg {
+    static constexpr int RS = DC <= 64 ? 64 : 128;     // elements per LDS row
+    static constexpr int SLOTS = RS / 8;               // 16-byte slots per LDS row
+    static constexpr int KT = FEW ? 32 : 64;           // keys per tile
+    static constexpr int TILE = KT * RS;               // elements of a K (or V) tile
+    static constexpr int PIECES = TILE * 2 / 1024;     // 1-KiB pieces of a tile
+    static constexpr int PPW = FEW ? PIECES : PIECES / 4;   // ... that one wave fetches, of K and of V each
+    static constexpr int RINGS = FEW ? 4 : 1;          // few rows: a ring per wave
+    static constexpr int RING = 2 * 2 * TILE;          // elements of a ring: two stages of K, V
+    static constexpr int LDS_BYTES = RINGS * RING * 2;
+    static constexpr int NS = KT / 32, NB = DC / 32;   // 32-key score blocks of a tile, 32-column blocks of the output
+};
+
+// The slot permutation of a row.  K: 16 rows x one slot must fall on 16 different slots of a 256-byte line (two rows of 128 bytes share a
+// line).  V: 4 rows x 64 bytes must fall on the 4 different quarters of a line.
+template <int RS> __device__ __forceinline__ int swz_k(int row) { return RS == 128 ? (row & 15) : ((row >> 1) & 7); }
+template <int RS> __device__ __forceinline__ int swz_v(int row) { return RS == 128 ? ((row & 3) << 2) : (((row >> 1) & 1) << 2); }
+
+template <typename T, int DC, bool FEW>
+__global__ __launch_bounds__(256, FEW ? 1 : 2) void attention_packed_kernel(const mv_attn_packed_desc p, const int item0) {
+    using C = PackedCfg<DC, FEW>;
+    typedef typename Vec8<T>::type V8;
+    typedef __attribute__((address_space(3))) T lds_t;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const PackedItem it = ((const PackedItem*)p.items)[item0 + blockIdx.x / p.kv_heads];
+    const int kvh = blockIdx.x % p.kv_heads, group = p.heads / p.kv_heads;
+    const int rows = it.q_len * group;
+    const int row0 = it.m0 + (FEW ? 0 : wave * 32);
+    const bool active = row0 < rows;                       // (wave-uniform) the last tile's waves may have no row
+    const int r = min(row0 + l31, rows - 1);               // this lane's packed row (padding lanes repeat the last one)
+    const int qi = r / group, hq = kvh * group + (r - qi * group);
+    const int seen = p.causal ? max(0, qi + it.kv_len - it.q_len + 1) : it.kv_len;
+    const int lim = min(seen, it.key_end);                 // this row walks the keys [key_begin, lim)
+    const int lim_lo = __builtin_amdgcn_readlane(lim, 0), lim_hi = __builtin_amdgcn_readlane(lim, 31);
+
+    // ---- Q (second operand of S^T): row in the lane, 8 columns per half wave and step; a negative scale turns its sign here ----
+    const float c = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-30f);   // scores in powers of two
+    V8 qf[DC / 16];
+    {
+        const T* q = (const T*)p.q + (int64_t)(it.q_row + qi) * p.ldq + (int64_t)hq * p.d;
+#pragma unroll
+        for (int s = 0; s < DC / 16; ++s) {
+            const int col = 16 * s + 8 * h;
+            u32x4 w = {0, 0, 0, 0};
+            if (col < p.d) w = *(const u32x4*)(q + col);
+            if (p.scale < 0.f) w ^= 0x80008000u;
+            qf[s] = __builtin_bit_cast(V8, w);
         }
-        T* o = (T*)p.out + (int64_t)(it.q_row + i) * p.ldo + (int64_t)h * p.d;
-        const float inv = seen > 0 ? 1.0f / l : 0.f;
-        if (c0 < p.d) o[c0] = (T)(seen > 0 ? o0 * inv : 0.f);
-        if (c1 < p.d) o[c1] = (T)(seen > 0 ? o1 * inv : 0.f);
+    }
+    float16v acc[C::NB];
+#pragma unroll
+    for (int b = 0; b < C::NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[b][e] = 0.f;
+    float m = -1.0e30f, l = 0.f;    // reference of the exponents (score units; m * c stays finite), sum of this lane's own keys
+
+    // ---- global -> LDS ----
+    lds_t* ring = (lds_t*)((__attribute__((address_space(3))) char*)smem) + (FEW ? wave * C::RING : 0);
+    unsigned ok[C::PPW], ov[C::PPW];   // byte offset of this lane's 16 bytes from the tile's first row; columns past d: out of range, read as 0
+#pragma unroll
+    for (int j = 0; j < C::PPW; ++j) {
+        const int at = ((FEW ? 0 : wave * C::PPW) + j) * 64 + lane;
+        const int row = at / C::SLOTS, slot = at % C::SLOTS;
+        const int sk = slot ^ swz_k<C::RS>(row), sv = slot ^ swz_v<C::RS>(row);
+        ok[j] = sk * 8 < p.d ? (unsigned)((row * p.ldk + sk * 8) * 2) : 0x80000000u;
+        ov[j] = sv * 8 < p.d ? (unsigned)((row * p.ldv + sv * 8) * 2) : 0x80000000u;
+    }
+    const char* kbase = (const char*)((const T*)p.k + (int64_t)it.k_row * p.ldk + (int64_t)kvh * p.d);
+    const char* vbase = (const char*)((const T*)p.v + (int64_t)it.k_row * p.ldv + (int64_t)kvh * p.d);
+    // tile at key `key` into stage `stage`: the descriptors start at the tile (64-bit address) and end with the sequence's last row, so rows
+    // behind it read as 0
+    auto issue = [&](int key, int stage) __attribute__((always_inline)) {
+        const int left = min(it.kv_len - key, C::KT);
+        const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)(kbase + (int64_t)key * p.ldk * 2), 0, (unsigned)(((left - 1) * p.ldk + p.d) * 2), 0x00020000);
+        const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)(vbase + (int64_t)key * p.ldv * 2), 0, (unsigned)(((left - 1) * p.ldv + p.d) * 2), 0x00020000);
+        lds_t* dst = ring + stage * 2 * C::TILE + (FEW ? 0 : wave * C::PPW * 512);
+#pragma unroll
+        for (int j = 0; j < C::PPW; ++j)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (__attribute__((address_space(3))) void*)(dst + j * 512), 16, (int)ok[j], 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < C::PPW; ++j)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (__attribute__((address_space(3))) void*)(dst + C::TILE + j * 512), 16, (int)ov[j], 0, 0, 0);
+    };
+
+    // ---- one tile ----
+    const int i16 = lane & 15;
+    int ka[C::SLOTS / 2];    // element offset of K fragment step s in a tile (row l31)
+#pragma unroll
+    for (int s = 0; s < DC / 16; ++s) ka[s] = l31 * C::RS + ((2 * s + h) ^ swz_k<C::RS>(l31)) * 8;
+    int va[C::NB];           // element offset of V^T fragment block b (keys 4 h + 0..3)
+#pragma unroll
+    for (int b = 0; b < C::NB; ++b) {
+        const int row = 4 * h + (i16 >> 2), slot = 4 * b + 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
+        va[b] = row * C::RS + (slot ^ swz_v<C::RS>(row)) * 8 + (i16 & 1) * 4;
+    }
+    auto compute = [&](int key, int stage) __attribute__((always_inline)) {
+        const lds_t* sk = ring + stage * 2 * C::TILE;
+        const lds_t* sv = sk + C::TILE;
+        float16v s[C::NS];
+#pragma unroll
+        for (int n = 0; n < C::NS; ++n)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[n][e] = 0.f;
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int k = 0; k < DC / 16; ++k)
+#pragma unroll
+            for (int n = 0; n < C::NS; ++n) {
+                const V8 kf = *(const __attribute__((address_space(3))) V8*)(sk + ka[k] + n * 32 * C::RS);
+                s[n] = mfma_32x32x16(kf, qf[k], s[n]);
+            }
+        __builtin_amdgcn_s_setprio(0);
+        const bool masked = key + C::KT > lim_lo;   // (wave-uniform) some row does not see all of the tile
+        if (masked) {
+            const int left = lim - key - 4 * h;
+#pragma unroll
+            for (int n = 0; n < C::NS; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (32 * n + (e & 3) + 8 * (e >> 2) >= left) s[n][e] = -INFINITY;
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int n = 0; n < C::NS; ++n)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[n][e]);
+        // the reference moves only when a score passes it by more than 2^6: P stays below 64 and the accumulators are rarely rescaled
+        if (__any((mx - m) * c > 6.0f)) {
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const float mn = fmaxf(m, mx);
+            const float a = __builtin_amdgcn_exp2f((m - mn) * c);
+            m = mn;
+            l *= a;
+#pragma unroll
+            for (int b = 0; b < C::NB; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[b][e] *= a;
+        }
+        const float mc = m * c;
+        float t0 = 0.f, t1 = 0.f;
+        V8 pf[2 * C::NS];
+#pragma unroll
+        for (int n = 0; n < C::NS; ++n)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][e], c, -mc));
+                if (e & 1) t1 += pe; else t0 += pe;
+                s[n][e] = pe;
+                pf[2 * n + (e >> 3)][e & 7] = (T)pe;   // P in the input type: half a step of it, relative, on each weight
+            }
+        l += t0 + t1;
+        if (masked) {
+            // a masked weight is 0, but 0 x infinity is not: where the tile's values are not all finite, the rows take their visible keys one
+            // by one instead
+            unsigned bad = 0;
+#pragma unroll
+            for (int j = 0; j < C::TILE / 512; ++j) {
+                const u32x4 w = *(const __attribute__((address_space(3))) u32x4*)(sv + (j * 64 + lane) * 8);
+                bad |= ((w.x & ExpBits<T>::mask) + ExpBits<T>::one) | ((w.y & ExpBits<T>::mask) + ExpBits<T>::one) |
+                       ((w.z & ExpBits<T>::mask) + ExpBits<T>::one) | ((w.w & ExpBits<T>::mask) + ExpBits<T>::one);
+            }
+            if (__any((bad & 0x80008000u) != 0)) {
+#pragma unroll 1
+                for (int j = 0; j < C::KT; ++j) {
+                    const int e = (j & 3) + 4 * ((j >> 3) & 3) + 16 * (j >> 5);
+                    float pe = 0.f;
+#pragma unroll
+                    for (int x = 0; x < 16 * C::NS; ++x) pe = x == e ? s[x >> 4][x & 15] : pe;
+                    pe = (float)(T)__shfl(pe, l31 + 32 * ((j >> 2) & 1), 64);
+                    const bool vis = key + j < lim;
+#pragma unroll
+                    for (int b = 0; b < C::NB; ++b)
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) {
+                            const int col = 32 * b + (x & 3) + 8 * (x >> 2) + 4 * h;
+                            const float v = (float)sv[j * C::RS + (((col >> 3) ^ swz_v<C::RS>(j)) << 3) + (col & 7)];
+                            if (vis) acc[b][x] = __builtin_fmaf(pe, v, acc[b][x]);
+                        }
+                }
+                return;
+            }
+        }
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int k = 0; k < 2 * C::NS; ++k)
+#pragma unroll
+            for (int b = 0; b < C::NB; ++b) {
+                const lds_t* a = sv + va[b] + 16 * k * C::RS;
+                const short4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)a);
+                const short4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(a + 8 * C::RS));
+                typedef short short8v __attribute__((ext_vector_type(8)));
+                const short8v xy = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+                acc[b] = mfma_32x32x16(__builtin_bit_cast(V8, xy), pf[k], acc[b]);
+            }
+        __builtin_amdgcn_s_setprio(0);
+    };
+
+    const int tiles = (it.key_end - it.key_begin + C::KT - 1) / C::KT;
+    if constexpr (!FEW) {
+        if (tiles > 0) issue(it.key_begin, 0);
+#pragma unroll 1
+        for (int t = 0; t < tiles; ++t) {
+            const int key = it.key_begin + t * C::KT;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // this wave's share of tile t has landed ...
+            __builtin_amdgcn_s_barrier();                        // ... and everyone's; everyone has left tile t - 1 and its stage
+            asm volatile("" ::: "memory");
+            if (t + 1 < tiles) issue(key + C::KT, (t + 1) & 1);
+            if (active && key < lim_hi) compute(key, t & 1);
+        }
+    } else {
+        // tiles wave, wave + 4, ...: this wave's own ring, no barrier
+        if (wave < tiles) issue(it.key_begin + wave * C::KT, 0);
+        if (wave + 4 < tiles) issue(it.key_begin + (wave + 4) * C::KT, 1);
+        int stage = 0;
+#pragma unroll 1
+        for (int t = wave; t < tiles; t += 4) {
+            if (t + 4 < tiles) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * C::PPW) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            compute(it.key_begin + t * C::KT, stage);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the stage's reads are done before it is filled again
+            if (t + 8 < tiles) issue(it.key_begin + (t + 8) * C::KT, stage);
+            stage ^= 1;
+        }
+    }
+    l += __shfl_xor(l, 32, 64);
+
+    if constexpr (FEW) {
+        // ---- the four waves' parts, joined through LDS: [wave][row][DC + 4] unnormalised sums, then [wave][row] references and sums ----
+        constexpr int PR = DC + 4;
+        float* part = (float*)smem;
+        float* ml = part + 4 * 32 * PR;
+        static_assert((4 * 32 * PR + 4 * 32 * 2) * 4 <= C::LDS_BYTES, "the joined parts fit the rings");
+        __syncthreads();
+#pragma unroll
+        for (int b = 0; b < C::NB; ++b)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *(float4v*)(part + (wave * 32 + l31) * PR + 32 * b + 8 * g + 4 * h) = float4v{acc[b][4 * g], acc[b][4 * g + 1], acc[b][4 * g + 2], acc[b][4 * g + 3]};
+        if (h == 0) {
+            ml[(wave * 32 + l31) * 2] = m;
+            ml[(wave * 32 + l31) * 2 + 1] = l;
+        }
+        __syncthreads();
+        const int n = min(32, rows - it.m0), quads = p.d / 4;
+        for (int x = tid; x < n * quads; x += 256) {
+            const int q = x / quads, col = (x - q * quads) * 4;
+            float mm = ml[q * 2];
+#pragma unroll
+            for (int w = 1; w < 4; ++w) mm = fmaxf(mm, ml[(w * 32 + q) * 2]);
+            float ll = 0.f;
+            float4v o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float a = __builtin_amdgcn_exp2f((ml[(w * 32 + q) * 2] - mm) * c), lw = ml[(w * 32 + q) * 2 + 1];
+                ll += a * lw;
+                // a wave that saw no key of the row has a sum of 0 and adds nothing
+                if (lw != 0.f) o += *(const float4v*)(part + (w * 32 + q) * PR + col) * a;
+            }
+            const int rr = it.m0 + q, i = rr / group, head = kvh * group + (rr - i * group);
+            if (it.ws_row >= 0) {
+                float* ws = (float*)p.workspace;
+                const int64_t at = (int64_t)kvh * p.ws_rows + it.ws_row + q;
+                *(float4v*)(ws + at * p.d + col) = o;
+                if (col == 0) {
+                    float* wml = ws + (int64_t)p.kv_heads * p.ws_rows * p.d + at * 2;
+                    wml[0] = mm * c;
+                    wml[1] = ll;
+                }
+            } else {
+                const int see = p.causal ? i + it.kv_len - it.q_len + 1 : it.kv_len;
+                const float inv = 1.0f / ll;
+                T* out = (T*)p.out + (int64_t)(it.q_row + i) * p.ldo + (int64_t)head * p.d + col;
+                T w4[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w4[e] = see > 0 ? (T)(o[e] * inv) : (T)0.f;
+                *(uint2*)out = *(const uint2*)w4;
+            }
+        }
+    } else {
+        if (row0 + l31 >= rows) return;
+        if (it.ws_row >= 0) {
+            float* ws = (float*)p.workspace;
+            const int64_t at = (int64_t)kvh * p.ws_rows + it.ws_row + wave * 32 + l31;
+#pragma unroll
+            for (int b = 0; b < C::NB; ++b)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int col = 32 * b + 8 * g + 4 * h;
+                    if (col < p.d) *(float4v*)(ws + at * p.d + col) = float4v{acc[b][4 * g], acc[b][4 * g + 1], acc[b][4 * g + 2], acc[b][4 * g + 3]};
+                }
+            if (h == 0) {
+                float* wml = ws + (int64_t)p.kv_heads * p.ws_rows * p.d + at * 2;
+                wml[0] = m * c;
+                wml[1] = l;
+            }
+            return;
+        }
+        const float inv = 1.0f / l;
+        T* out = (T*)p.out + (int64_t)(it.q_row + qi) * p.ldo + (int64_t)hq * p.d;
+#pragma unroll
+        for (int b = 0; b < C::NB; ++b)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int col = 32 * b + 8 * g + 4 * h;
+                if (col >= p.d) continue;
+                T w4[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w4[e] = seen > 0 ? (T)(acc[b][4 * g + e] * inv) : (T)0.f;
+                *(uint2*)(out + col) = *(const uint2*)w4;
+            }
     }
 }
 
-extern "C" int64_t mv_attention_packed_workspace_bytes(int32_t n_slots, int32_t kv_heads, int32_t d, int32_t tile_rows) {
-    if (n_slots < 0 || kv_heads < 1 || d < 1 || tile_rows < 1) return -1;
-    return (int64_t)n_slots * kv_heads * tile_rows * (d + 2) * 4;
+// joins the parts of rows whose keys were split over several items; one wave per packed row
+template <typename T>
+__global__ __launch_bounds__(256) void attention_join_kernel(const mv_attn_packed_desc p) {
+    const int blocks = 128 / 4;   // (a join has at most 128 rows, a block 4)
+    const PackedJoin jn = ((const PackedJoin*)p.joins)[blockIdx.x / (p.kv_heads * blocks)];
+    const int kvh = (blockIdx.x / blocks) % p.kv_heads, group = p.heads / p.kv_heads;
+    const int row = (blockIdx.x % blocks) * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int rr = jn.m0 + row;
+    if (row >= jn.rows || rr >= jn.q_len * group) return;
+    const int i = rr / group, head = kvh * group + (rr - i * group);
+    const float* ws = (const float*)p.workspace;
+    const int64_t at = (int64_t)kvh * p.ws_rows + jn.ws_row + row;
+    const float* ml = ws + (int64_t)p.kv_heads * p.ws_rows * p.d;
+    float mm = -3.0e38f;
+    for (int s = 0; s < jn.parts; ++s) mm = fmaxf(mm, ml[(at + (int64_t)s * jn.rows) * 2]);
+    float ll = 0.f, o0 = 0.f, o1 = 0.f;
+    const int col = lane * 2;
+    for (int s = 0; s < jn.parts; ++s) {
+        const int64_t r = at + (int64_t)s * jn.rows;
+        const float lw = ml[r * 2 + 1], a = __builtin_amdgcn_exp2f(ml[r * 2] - mm);
+        if (lw == 0.f) continue;   // no key of this part was seen
+        ll += a * lw;
+        if (col < p.d) {
+            const float2v w = *(const float2v*)(ws + r * p.d + col);
+            o0 = __builtin_fmaf(a, w.x, o0);
+            o1 = __builtin_fmaf(a, w.y, o1);
+        }
+    }
+    const int see = p.causal ? i + jn.kv_len - jn.q_len + 1 : jn.kv_len;
+    if (col < p.d) {
+        T w2[2] = {see > 0 ? (T)(o0 / ll) : (T)0.f, see > 0 ? (T)(o1 / ll) : (T)0.f};
+        *(unsigned*)((T*)p.out + (int64_t)(jn.q_row + i) * p.ldo + (int64_t)head * p.d + col) = *(const unsigned*)w2;
+    }
+}
+
+extern "C" int64_t mv_attention_packed_workspace_bytes(int64_t ws_rows, int32_t kv_heads, int32_t d) {
+    if (ws_rows < 0 || kv_heads < 1 || d < 1) return -1;
+    return ws_rows * kv_heads * (d + 2) * 4;
+}
+
+template <typename T, int DC, bool FEW>
+static int launch_packed(const mv_attn_packed_desc* d, int item0, int n, hipStream_t st) {
+    using C = PackedCfg<DC, FEW>;
+    const auto kernel = attention_packed_kernel<T, DC, FEW>;
+    if (C::LDS_BYTES > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS_BYTES);
+        if (e != hipSuccess) {
+            mv_set_error("mv_attention_packed: %s", hipGetErrorString(e));
+            return MV_ERR_LAUNCH;
+        }
+    }
+    kernel<<<(unsigned)(n * d->kv_heads), 256, C::LDS_BYTES, st>>>(*d, item0);
+    MV_CHECK_LAUNCH("mv_attention_packed");
+    return MV_OK;
+}
+
+template <typename T>
+static int launch_all(const mv_attn_packed_desc* d, hipStream_t st) {
+    int rc = MV_OK;
+    if (d->n_items > 0)
+        rc = d->d <= 64 ? launch_packed<T, 64, false>(d, 0, d->n_items, st)
+           : d->d <= 96 ? launch_packed<T, 96, false>(d, 0, d->n_items, st) : launch_packed<T, 128, false>(d, 0, d->n_items, st);
+    if (rc == MV_OK && d->n_few > 0)
+        rc = d->d <= 64 ? launch_packed<T, 64, true>(d, d->n_items, d->n_few, st)
+           : d->d <= 96 ? launch_packed<T, 96, true>(d, d->n_items, d->n_few, st) : launch_packed<T, 128, true>(d, d->n_items, d->n_few, st);
+    if (rc == MV_OK && d->n_joins > 0) {
+        attention_join_kernel<T><<<(unsigned)(d->n_joins * d->kv_heads * 32), 256, 0, st>>>(*d);
+        MV_CHECK_LAUNCH("mv_attention_packed (join)");
+    }
+    return rc;
 }
 
 extern "C" int mv_attention_packed(const mv_attn_packed_desc* d, void* stream) {
@@ -51,10 +426,16 @@ extern "C" int mv_attention_packed(const mv_attn_packed_desc* d, void* stream) {
     MV_REQUIRE(d->d >= 8 && d->d <= 128 && d->d % 8 == 0, "mv_attention_packed: head dim %d (a multiple of 8 up to 128)", d->d);
     MV_REQUIRE(d->kv_heads >= 1 && d->heads >= d->kv_heads && d->heads % d->kv_heads == 0, "mv_attention_packed: %d heads over %d key / value heads",
                d->heads, d->kv_heads);
-    MV_REQUIRE(d->n_items >= 0 && (int64_t)d->n_items * d->kv_heads < (1ll << 31), "mv_attention_packed: %d items", d->n_items);
-    if (d->n_items == 0) return MV_OK;
+    MV_REQUIRE(d->scale >= -1e6f && d->scale <= 1e6f, "mv_attention_packed: scale %g (at most 1e6 in size)", (double)d->scale);
+    MV_REQUIRE(d->n_items >= 0 && d->n_few >= 0 && d->n_joins >= 0 && ((int64_t)d->n_items + d->n_few) * d->kv_heads < (1ll << 31) &&
+               (int64_t)d->n_joins * d->kv_heads * 32 < (1ll << 31), "mv_attention_packed: %d + %d items, %d joins", d->n_items, d->n_few, d->n_joins);
+    if (d->n_items + d->n_few == 0) return MV_OK;
     MV_REQUIRE(d->q && d->k && d->v && d->out && d->items, "mv_attention_packed: null pointer");
-    MV_DISPATCH_TYPE(d->dtype, (attention_rows_kernel<T><<<(unsigned)(d->n_items * d->kv_heads), 256, 0, (hipStream_t)stream>>>(*d)));
-    MV_CHECK_LAUNCH("mv_attention_packed");
-    return MV_OK;
+    MV_REQUIRE((((uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v | (uintptr_t)d->out) & 15) == 0 && ((d->ldq | d->ldk | d->ldv | d->ldo) & 7) == 0,
+               "mv_attention_packed: rows must be 16-byte aligned");
+    MV_REQUIRE(d->ldk >= 0 && d->ldk <= (1 << 23) && d->ldv >= 0 && d->ldv <= (1 << 23), "mv_attention_packed: key / value row stride above 2^23");
+    MV_REQUIRE(d->n_joins == 0 || (d->joins && d->workspace && ((uintptr_t)d->workspace & 15) == 0 &&
+               d->workspace_bytes >= mv_attention_packed_workspace_bytes(d->ws_rows, d->kv_heads, d->d)),
+               "mv_attention_packed: the workspace is missing, unaligned or too small");
+    return d->dtype == MV_F16 ? launch_all<half_t>(d, (hipStream_t)stream) : launch_all<bf16_t>(d, (hipStream_t)stream);
 }

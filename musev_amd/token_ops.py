@@ -115,17 +115,17 @@ class _Held:
 class AttentionPlan(_Held):
     """the work list of :func:`attention_packed` for one set of sequence lengths (:func:`attention_plan`)"""
 
-    def __init__(self, q_lens, kv_lens, heads, kv_heads, d, causal, scale, tile_rows, items, joins, n_slots):
+    def __init__(self, q_lens, kv_lens, heads, kv_heads, d, causal, scale, n_items, n_few, items, joins, ws_rows):
         self.q_lens, self.kv_lens = tuple(q_lens), tuple(kv_lens)
         self.heads, self.kv_heads, self.d, self.causal, self.scale = heads, kv_heads, d, causal, scale
         self.total_q, self.total_kv = sum(q_lens), sum(kv_lens)
         self._hold(items, joins)
         ds = AttnPackedDesc()
         ds.items, ds.joins = items.data_ptr(), joins.data_ptr()
-        ds.n_items, ds.n_joins, ds.n_slots, ds.tile_rows = items.shape[0], joins.shape[0], n_slots, tile_rows
+        ds.n_items, ds.n_few, ds.n_joins, ds.ws_rows = n_items, n_few, joins.shape[0], ws_rows
         ds.heads, ds.kv_heads, ds.d, ds.causal, ds.scale = heads, kv_heads, d, int(causal), scale
         self._desc = ds
-        self._workspace = 0
+        self._workspace = 4 * ws_rows * kv_heads * (d + 2)   # mv_attention_packed_workspace_bytes
 
 
 def _lens(v, name: str) -> List[int]:
@@ -139,13 +139,44 @@ def _lens(v, name: str) -> List[int]:
     return v
 
 
-def _plan_items(ql: Sequence[int], kl: Sequence[int], group: int, tile_rows: int) -> Tuple[List[tuple], List[tuple], int]:
-    items, q_row, k_row = [], 0, 0
+WIDE_ROWS, FEW_ROWS = 128, 32   # packed rows per item of the two kernel forms
+# Keys of an item that is worth a split: an item's parts each write and the join reads back (d + 2) fp32 per row.
+MIN_PART_WIDE, MIN_PART_FEW = 512, 256
+BLOCKS = 512                    # two blocks on each of the 256 CUs
+
+
+def _plan_items(ql: Sequence[int], kl: Sequence[int], group: int, kv_heads: int, causal: bool):
+    """(wide items, few-row items, joins, workspace rows): see include/musev_tokens.h.  A sequence of at most FEW_ROWS packed rows makes one
+    few-row item.  An item's keys end with what its last query sees.  Where the items alone would leave CUs idle, or one item would outlast
+    the others, its keys are split into parts of about 1 / BLOCKS of all the work; the longest items come first."""
+    tiles, q_row, k_row = ([], []), 0, 0
     for q, kv in zip(ql, kl):
-        for m0 in range(0, q * group, tile_rows):
-            items.append((q_row, q, k_row, kv, m0, 0, kv, -1))
+        rows = q * group
+        few = rows <= FEW_ROWS
+        for m0 in range(0, rows, FEW_ROWS if few else WIDE_ROWS):
+            last = min(m0 + (FEW_ROWS if few else WIDE_ROWS), rows) - 1
+            end = max(0, min(kv, last // group + kv - q + 1)) if causal else kv
+            tiles[few].append((q_row, q, k_row, kv, m0, end))
         q_row, k_row = q_row + q, k_row + kv
-    return items, [], 0
+    out, joins, ws = ([], []), [], 0
+    for few in (False, True):
+        width, least = (FEW_ROWS, MIN_PART_FEW) if few else (WIDE_ROWS, MIN_PART_WIDE)
+        part = max(least, -(-sum(t[5] for t in tiles[few]) * kv_heads // BLOCKS))
+        part = -(-part // 64) * 64
+        for q_row, q, k_row, kv, m0, end in tiles[few]:
+            n = max(1, (end + part // 2) // part)
+            if n == 1:
+                out[few].append((q_row, q, k_row, kv, m0, 0, end, -1))
+                continue
+            size = -(-(-(-end // n)) // 64) * 64
+            n = -(-end // size)
+            rows = min(width, q * group - m0)
+            for s in range(n):
+                out[few].append((q_row, q, k_row, kv, m0, s * size, min(end, (s + 1) * size), ws + s * rows))
+            joins.append((q_row, q, kv, m0, ws, n, rows, 0))
+            ws += n * rows
+        out[few].sort(key=lambda i: i[5] - i[6])
+    return out[0], out[1], joins, ws
 
 
 def attention_plan(q_lens: Sequence[int], kv_lens: Optional[Sequence[int]] = None, *, heads: int, kv_heads: Optional[int] = None, d: int,
@@ -166,16 +197,16 @@ def attention_plan(q_lens: Sequence[int], kv_lens: Optional[Sequence[int]] = Non
     if max(ql) * (heads // kv_heads) > _I32_MAX:
         raise ValueError("attention_plan: more than 2^31 - 1 (query, head) rows per key / value head")
     scale = d ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError("attention_plan: scale must be finite")
+    if not abs(scale) <= 1e6:
+        raise ValueError(f"attention_plan: scale {scale} (at most 1e6 in size)")
     dev = torch.device(device)
     if dev.type == "cuda" and dev.index is None:
         dev = torch.device("cuda", torch.cuda.current_device())
-    tile_rows = 128
-    items, joins, n_slots = _plan_items(ql, kl, heads // kv_heads, tile_rows)
-    table = torch.tensor(items or [(0,) * 8], dtype=torch.int32).to(dev)[:len(items)]
-    join = torch.tensor(joins or [(0,) * 8], dtype=torch.int32).to(dev)[:len(joins)]
-    return AttentionPlan(ql, kl, heads, kv_heads, d, bool(causal), scale, tile_rows, table, join, n_slots)
+    wide, few, joins, ws_rows = _plan_items(ql, kl, heads // kv_heads, kv_heads, bool(causal))
+    # one upload for both tables
+    table = torch.tensor((wide + few + joins) or [(0,) * 8], dtype=torch.int32).to(dev)
+    n = len(wide) + len(few)
+    return AttentionPlan(ql, kl, heads, kv_heads, d, bool(causal), scale, len(wide), len(few), table[:n], table[n:n + len(joins)], ws_rows)
 
 
 def attention_packed(plan: AttentionPlan, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:

@@ -71,16 +71,17 @@ def test_entry_points_refuse_without_a_gpu():
         refused(fn(None, None), b"null descriptor")
     a = _lib.AttnPackedDesc()
     a.q = a.k = a.v = a.out = a.items = 16
-    a.n_items, a.tile_rows, a.heads, a.kv_heads, a.d, a.scale = 1, 128, 4, 2, 64, 0.125
+    a.n_items, a.heads, a.kv_heads, a.d, a.scale = 1, 4, 2, 64, 0.125
     a.ldq = a.ldo = 256
     a.ldk = a.ldv = 128
     for name, bad, text in (("d", 12, b"head dim"), ("d", 136, b"head dim"), ("kv_heads", 3, b"heads"), ("dtype", 2, b"element type"),
-                            ("n_items", -1, b"items"), ("q", 0, b"null")):
+                            ("n_items", -1, b"items"), ("q", 0, b"null"), ("k", 8, b"aligned"), ("ldv", 132, b"aligned"), ("ldk", 1 << 24, b"stride"),
+                            ("n_joins", 1, b"workspace"), ("scale", float("nan"), b"scale"), ("scale", 2e6, b"scale")):
         old = getattr(a, name)
         setattr(a, name, bad)
         refused(lib.mv_attention_packed(C.byref(a), None), text)
         setattr(a, name, old)
-    assert lib.mv_attention_packed_workspace_bytes(-1, 1, 64, 128) == -1
+    assert lib.mv_attention_packed_workspace_bytes(-1, 1, 64) == -1 and lib.mv_attention_packed_workspace_bytes(3, 2, 64) == 3 * 2 * 66 * 4
     r = _lib.RotaryDesc()
     r.q = r.out_q = r.positions = r.turns = r.axis = 16
     r.tokens, r.heads, r.kv_heads, r.d, r.pairs, r.axes = 4, 2, 2, 64, 32, 1
@@ -109,41 +110,41 @@ def test_entry_points_refuse_without_a_gpu():
     refused(lib.mv_quantize_rows_i8(16, 64, 4, 0, 0, 16, 128, 16, None), b"131072")
 
 
-def _cover(plan_items, joins, ql, kl, group, causal, tile_of):
-    """every packed row's every visible key is walked exactly once, by items whose slots are joined for exactly those rows"""
-    q_at = k_at = 0
-    starts = []
+def _cover(wide, few, joins, ws_rows, ql, kl, group, causal):
+    """every packed row's every visible key is walked by exactly one item, the parts of a row are joined for exactly that row, and no two
+    parts share workspace rows"""
+    want, q_at, k_at = set(), 0, 0
     for q, kv in zip(ql, kl):
-        starts.append((q_at, q, k_at, kv))
+        for m0 in range(0, q * group, 32 if q * group <= 32 else 128):
+            want.add((q_at, q, k_at, kv, m0))
         q_at, k_at = q_at + q, k_at + kv
-    by_tile = {}
-    for it in plan_items:
-        by_tile.setdefault((it[0], it[1], it[2], it[3], it[4]), []).append(it)
-    slot_rows = {}
-    for j in joins:
-        for s in range(j[4], j[4] + j[5]):
-            assert s not in slot_rows
-            slot_rows[s] = (j[0], j[1], j[2], j[3])
-    want = {}
-    for s in starts:
-        for m0 in range(0, s[1] * group, tile_of(s)):
-            want[(s[0], s[1], s[2], s[3], m0)] = None
-    want = {k: v for k, v in want.items() if k[1] > 0}
-    assert set(by_tile) == set(want)
-    for key, items in by_tile.items():
-        last = min((key[4] + tile_of((key[0], key[1], key[2], key[3])) - 1) // group, key[1] - 1)
-        vis = key[3] if not causal else max(0, min(key[3], last + key[3] - key[1] + 1))
-        at = 0
-        items = sorted(items, key=lambda i: i[5])
-        for it in items:
-            assert it[5] == at and it[6] >= it[5], (key, items)
-            at = it[6]
-            if len(items) > 1:
-                assert slot_rows[it[7]] == (key[0], key[1], key[3], key[4])
-            else:
-                assert it[7] == -1
-        assert vis <= at <= key[3] or (vis == 0 and at <= key[3])
-    assert sum(len(v) for v in by_tile.values() if len(v) > 1) == len(slot_rows)
+    tiles = {}
+    for it in wide + few:
+        tiles.setdefault(tuple(it[:5]), []).append(it)
+    assert set(tiles) == want
+    joined = {(j[0], j[1], j[2], j[3]): j for j in joins}
+    assert len(joined) == len(joins)
+    used = set()
+    for key, items in tiles.items():
+        q_row, q, k_row, kv, m0 = key
+        small = q * group <= 32
+        assert all((it in few) == small for it in items)
+        rows = min(32 if small else 128, q * group - m0)
+        last = (m0 + rows - 1) // group
+        vis = kv if not causal else max(0, min(kv, last + kv - q + 1))
+        items.sort(key=lambda i: i[5])
+        assert items[0][5] == 0 and items[-1][6] == vis and all(a[6] == b[5] for a, b in zip(items, items[1:]))
+        if len(items) == 1:
+            assert items[0][7] == -1 and (q_row, q, kv, m0) not in joined
+            continue
+        j = joined.pop((q_row, q, kv, m0))
+        assert j[5] == len(items) and j[6] == rows
+        for s, it in enumerate(items):
+            assert it[7] == j[4] + s * rows and it[5] < it[6] and it[5] % 64 == 0
+            mine = set(range(it[7], it[7] + rows))
+            assert not (mine & used)
+            used |= mine
+    assert not joined and used == set(range(ws_rows))
 
 
 @pytest.mark.parametrize("seed", range(12))
@@ -155,13 +156,14 @@ def test_plan_covers_every_visible_key_once(seed):
         one = r.random() < 0.4
         ql = [1 if one else r.choice([0, 1, 2, 31, 33, 127, 128, 129, 700]) for _ in range(n)]
         kl = [r.choice([0, 1, 63, 64, 65, 500, 5000, 20000]) for _ in range(n)]
-        kvh = r.choice([1, 2, 8])
-        group = r.choice([1, 3, 4, 8])
+        kvh, group = r.choice([1, 2, 8]), r.choice([1, 3, 4, 8])
         plan = to.attention_plan(ql, kl, heads=kvh * group, kv_heads=kvh, d=64, causal=causal, device="cpu")
         items, joins = (t.tolist() for t in plan._tensors)
-        _cover(items, joins, ql, kl, group, causal, lambda s: plan._desc.tile_rows)
-        slots = {it[7] for it in items if it[7] >= 0}
-        assert slots == set(range(plan._desc.n_slots))
+        d = plan._desc
+        assert len(items) == d.n_items + d.n_few and len(joins) == d.n_joins
+        _cover(items[:d.n_items], items[d.n_items:], joins, d.ws_rows, ql, kl, group, causal)
+        from musev_amd import _lib
+        assert plan._workspace == _lib.load().mv_attention_packed_workspace_bytes(d.ws_rows, kvh, 64)
 
 
 def test_plan_refusals():
@@ -425,7 +427,8 @@ def test_what_is_not_seen_does_not_reach_the_output(bad, one):
     q, k, v = attention_inputs(ql, kl, heads, kvh, d, dt, 9)
     pad = torch.zeros(40, kvh * d, dtype=dt, device=DEV)
     k, v = torch.cat([k, pad]), torch.cat([v, pad])
-    clean = ops.attention_packed(ops.attention_plan(ql, kl, heads=heads, kv_heads=kvh, d=d), q, k, v)
+    # (the bound is attention_oracle's: the order in which a row's sum is formed is not part of the definition and may differ beside such values)
+    clean, bound = attention_oracle(q, k, v, ql, kl, heads, kvh, d, True)
     k2, v2 = k.clone(), v.clone()
     k2[sum(kl):], v2[sum(kl):] = bad, bad
     if one:
@@ -436,7 +439,7 @@ def test_what_is_not_seen_does_not_reach_the_output(bad, one):
         k2[70 + 150], v2[70 + 150] = bad, bad
     got = ops.attention_packed(ops.attention_plan(ql, kl, heads=heads, kv_heads=kvh, d=d), q, k2, v2)
     torch.cuda.synchronize()
-    assert torch.equal(got[:first_bad], clean[:first_bad])
+    within(got[:first_bad], clean[:first_bad], bound[:first_bad])
     if not one:   # V alone: a visible infinity is an infinity, a visible NaN is NaN, in its own columns only
         v3 = v.clone()
         v3[70 + 150, 5] = bad
@@ -446,7 +449,7 @@ def test_what_is_not_seen_does_not_reach_the_output(bad, one):
         assert bool((torch.isnan(seen) if math.isnan(bad) else seen == bad).all())
         rest = torch.ones_like(got, dtype=torch.bool)
         rest.view(-1, heads, d)[40 + 150:, :2, 5] = False
-        assert torch.equal(got[rest], clean[rest])
+        within(got[rest], clean[rest], bound[rest])
 
 
 @gpu
