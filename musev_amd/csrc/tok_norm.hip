@@ -1,83 +1,161 @@
 // tok_norm.hip -- the gated residual norm (include/musev_tokens.h: mv_gated_residual_norm).
 #include "tok_common.h"
 
-__device__ __forceinline__ float block_sum(float v, float* red) {
+// sums over a row held by WAVES waves
+template <int WAVES>
+__device__ __forceinline__ float row_sum(float v, float* red) {
     v = wave_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return red[0] + red[1] + red[2] + red[3];
+    if constexpr (WAVES > 1) {
+        __syncthreads();   // (the previous sum's readers are through)
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = red[0];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) v += red[w];
+    }
+    return v;
 }
 
-// one block per row, the row's fp32 values in LDS
-template <typename T>
+// A row stays in registers from its one read to its one write: NV chunks of 8 columns per lane, WAVES waves per row, 4 / WAVES rows per
+// block.  Both norms' statistics are formed in two passes over the registers (mean, then squared deviations), in fp32.  Bound by memory:
+// x and f in, s and h out.
+template <typename T, int NV, int WAVES>
 __global__ __launch_bounds__(256) void gated_norm_kernel(const mv_gated_norm_desc p) {
-    extern __shared__ __attribute__((aligned(16))) float row_s[];
     __shared__ float red[4];
-    const int64_t row = blockIdx.x;
-    const int c = p.c, tid = threadIdx.x;
-    const T* x = (const T*)p.x + row * p.ldx;
-    const T* f = (const T*)p.f + row * p.ldf;
+    constexpr int LANES = 64 * WAVES;
+    const int lane = threadIdx.x % LANES, c = p.c;
+    const int64_t row = (int64_t)blockIdx.x * (4 / WAVES) + threadIdx.x / LANES;
+    if (row >= p.rows) return;   // (a whole wave; with WAVES = 4 the grid is exact)
     T* so = (T*)p.stream_out + row * p.lds;
     T* ho = (T*)p.norm_out + row * p.ldh;
-    const int64_t g = p.group_index ? (int64_t)p.group_index[row] : p.rows_per_group > 0 ? row / p.rows_per_group : 0;
+    const int64_t g = p.group_index ? (int64_t)p.group_index[row] : p.rows_per_group > 0 ? (int64_t)((unsigned)row / (unsigned)p.rows_per_group) : 0;
     if (g < 0 || g >= p.groups) {
-        for (int i = tid; i < c; i += 256) {
+        for (int i = lane; i < c; i += LANES) {
             so[i] = (T)NAN;
             if (p.norm_out) ho[i] = (T)NAN;
         }
         return;
     }
-    const T* gate = p.gate ? (const T*)p.gate + g * p.ldg : nullptr;
-    float mean = 0.f, rstd = 1.f;
-    if (p.post) {
+    const T* x = (const T*)p.x + row * p.ldx;
+    const T* f = (const T*)p.f + row * p.ldf;
+    float s[NV][8], y[NV][8];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int col = (j * LANES + lane) * 8;
+        if (col < c) {
+            load8(f + col, c - col, y[j]);
+            load8(x + col, c - col, s[j]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[j][e] = s[j][e] = 0.f;
+        }
+    }
+    const float inv_c = 1.0f / (float)c;
+    // mean and 1 / sqrt(mean square deviation + eps) of a row in registers (columns past c hold 0)
+    auto statistics = [&](const float (&v)[NV][8], float eps, float& mean, float& rstd) __attribute__((always_inline)) {
+        mean = 0.f;
         if (p.layer) {
-            float s = 0.f;
-            for (int i = tid; i < c; i += 256) s += (float)f[i];
-            mean = block_sum(s, red) / c;
+            float t = 0.f;
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) t += v[j][e];
+            mean = row_sum<WAVES>(t, red) * inv_c;
         }
-        float s = 0.f;
-        for (int i = tid; i < c; i += 256) {
-            const float v = (float)f[i] - mean;
-            s += v * v;
+        float t = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int col = (j * LANES + lane) * 8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float d = col + e < c ? v[j][e] - mean : 0.f;
+                t = __builtin_fmaf(d, d, t);
+            }
         }
-        rstd = rsqrtf(block_sum(s, red) / c + p.post_eps);
-    }
-    float sum = 0.f;
-    for (int i = tid; i < c; i += 256) {
-        float y = (float)f[i];
+        rstd = 1.0f / sqrtf(row_sum<WAVES>(t, red) * inv_c + eps);
+    };
+    float mean, rstd;
+    if (p.post) statistics(y, p.post_eps, mean, rstd);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int col = (j * LANES + lane) * 8;
+        if (col >= c) continue;
         if (p.post) {
-            y = (y - mean) * rstd;
-            if (p.post_gamma) y *= (float)((const T*)p.post_gamma)[i];
-            if (p.post_beta) y += (float)((const T*)p.post_beta)[i];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[j][e] = (y[j][e] - mean) * rstd;
+            if (p.post_gamma) {
+                float w[8];
+                load8((const T*)p.post_gamma + col, c - col, w);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[j][e] *= w[e];
+            }
+            if (p.post_beta) {
+                float w[8];
+                load8((const T*)p.post_beta + col, c - col, w);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[j][e] += w[e];
+            }
         }
-        const float s = p.alpha * (float)x[i] + (gate ? (float)gate[i] * y : y);
-        row_s[i] = s;
-        sum += s;
-    }
-    mean = 0.f;
-    if (p.norm_out) {
-        if (p.layer) mean = block_sum(sum, red) / c;
-        float s = 0.f;
-        for (int i = tid; i < c; i += 256) {
-            const float v = row_s[i] - mean;
-            s += v * v;
+        if (p.gate) {
+            float w[8];
+            load8((const T*)p.gate + g * p.ldg + col, c - col, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[j][e] *= w[e];
         }
-        rstd = rsqrtf(block_sum(s, red) / c + p.pre_eps);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[j][e] = col + e < c ? __builtin_fmaf(p.alpha, s[j][e], y[j][e]) : 0.f;
+        store8(so + col, c - col, s[j]);
     }
-    __syncthreads();   // (stream_out may be x or f: every read of the row is done)
-    for (int i = tid; i < c; i += 256) {
-        const float s = row_s[i];
-        so[i] = (T)s;
-        if (p.norm_out) {
-            float h = (s - mean) * rstd;
-            if (p.pre_gamma) h *= (float)((const T*)p.pre_gamma)[i];
-            if (p.pre_beta) h += (float)((const T*)p.pre_beta)[i];
-            if (p.scale) h *= 1.0f + (float)((const T*)p.scale)[g * p.ldsc + i];
-            if (p.shift) h += (float)((const T*)p.shift)[g * p.ldsh + i];
-            ho[i] = (T)h;
+    if (!p.norm_out) return;
+    statistics(s, p.pre_eps, mean, rstd);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int col = (j * LANES + lane) * 8;
+        if (col >= c) continue;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[j][e] = (s[j][e] - mean) * rstd;
+        float w[8];
+        if (p.pre_gamma) {
+            load8((const T*)p.pre_gamma + col, c - col, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[j][e] *= w[e];
         }
+        if (p.pre_beta) {
+            load8((const T*)p.pre_beta + col, c - col, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[j][e] += w[e];
+        }
+        if (p.scale) {
+            load8((const T*)p.scale + g * p.ldsc + col, c - col, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[j][e] = __builtin_fmaf(s[j][e], w[e], s[j][e]);
+        }
+        if (p.shift) {
+            load8((const T*)p.shift + g * p.ldsh + col, c - col, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[j][e] += w[e];
+        }
+        store8(ho + col, c - col, s[j]);
     }
+}
+
+template <typename T, int NV, int WAVES>
+static void launch_norm(const mv_gated_norm_desc* d, hipStream_t st) {
+    constexpr int R = 4 / WAVES;
+    gated_norm_kernel<T, NV, WAVES><<<(unsigned)((d->rows + R - 1) / R), 256, 0, st>>>(*d);
+}
+
+// up to 2048 columns a wave holds a row; wider rows take the block's four waves
+template <typename T>
+static void launch_norm_width(const mv_gated_norm_desc* d, hipStream_t st) {
+    const int c = d->c;
+    if (c <= 512) launch_norm<T, 1, 1>(d, st);
+    else if (c <= 1024) launch_norm<T, 2, 1>(d, st);
+    else if (c <= 1536) launch_norm<T, 3, 1>(d, st);
+    else if (c <= 2048) launch_norm<T, 4, 1>(d, st);
+    else if (c <= 4096) launch_norm<T, 2, 4>(d, st);
+    else if (c <= 8192) launch_norm<T, 4, 4>(d, st);
+    else launch_norm<T, 8, 4>(d, st);
 }
 
 extern "C" int mv_gated_residual_norm(const mv_gated_norm_desc* d, void* stream) {
@@ -85,9 +163,10 @@ extern "C" int mv_gated_residual_norm(const mv_gated_norm_desc* d, void* stream)
     MV_REQUIRE(d->dtype == MV_F16 || d->dtype == MV_BF16, "mv_gated_residual_norm: element type %d", d->dtype);
     MV_REQUIRE(d->c >= 1 && d->c <= 16384, "mv_gated_residual_norm: %d columns (1 .. 16384)", d->c);
     MV_REQUIRE(d->rows >= 0 && d->rows < (1ll << 31) && d->groups >= 1, "mv_gated_residual_norm: %ld rows, %ld groups", (long)d->rows, (long)d->groups);
+    MV_REQUIRE(d->rows_per_group >= 0 && d->rows_per_group < (1ll << 31), "mv_gated_residual_norm: groups of %ld rows", (long)d->rows_per_group);
     if (d->rows == 0) return MV_OK;
     MV_REQUIRE(d->x && d->f && d->stream_out, "mv_gated_residual_norm: null pointer");
-    MV_DISPATCH_TYPE(d->dtype, (gated_norm_kernel<T><<<(unsigned)d->rows, 256, d->c * 4, (hipStream_t)stream>>>(*d)));
+    MV_DISPATCH_TYPE(d->dtype, launch_norm_width<T>(d, (hipStream_t)stream));
     MV_CHECK_LAUNCH("mv_gated_residual_norm");
     return MV_OK;
 }
