@@ -8,30 +8,79 @@ __device__ __forceinline__ void turn_sincos(double pos, double turns, float* s, 
     sincospif(2.0f * (float)(t - rint(t)), s, c);
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void rotary_kernel(const mv_rotary_desc p) {
-    const int all = p.heads + (p.k ? p.kv_heads : 0);
-    const int tail = p.d - 2 * p.pairs, per_head = p.pairs + tail;
-    const int64_t total = p.tokens * all * per_head;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t tok = i / (all * per_head);
-        const int r = (int)(i - tok * (all * per_head));
-        const int head = r / per_head, e = r - head * per_head;
-        const bool isk = head >= p.heads;
-        const T* in = isk ? (const T*)p.k + tok * p.ldk + (head - p.heads) * p.d : (const T*)p.q + tok * p.ldq + head * p.d;
-        T* out = isk ? (T*)p.out_k + tok * p.ldok + (head - p.heads) * p.d : (T*)p.out_q + tok * p.ldoq + head * p.d;
-        if (e >= p.pairs) {
-            out[p.pairs + e] = in[p.pairs + e];
-            continue;
-        }
-        const int64_t at = tok * p.ldp + p.axis[e];
+// n / d for n * d < 2^32 as one high product, m = ceil(2^32 / d)
+struct Div {
+    unsigned d, m;
+};
+static Div make_div(unsigned d) { return Div{d, d == 1 ? 0u : (unsigned)(((1ull << 32) + d - 1) / d)}; }
+__device__ __forceinline__ unsigned div_of(unsigned n, Div v) { return v.d == 1 ? n : __umulhi(n, v.m); }
+
+struct RotaryArgs {
+    mv_rotary_desc p;
+    Div per_token, per_head, pairs;   // work items of a token, of a head
+    int rot_items, tokens_per_block;  // items of a head that turn (the others copy what passes through)
+};
+
+// A block owns a few tokens: their sines and cosines go to LDS once, shared by all heads, then every thread takes work items of 8 elements
+// (adjacent pairs: 4 pairs; halves: 8 + 8 elements) with 16-byte accesses.  Bound by memory: q and k in and out.
+template <typename T, bool HALVES>
+__global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
+    extern __shared__ __attribute__((aligned(16))) float2 turn[];   // [token][pair] {sin, cos}
+    const mv_rotary_desc& p = a.p;
+    const int64_t tok0 = (int64_t)blockIdx.x * a.tokens_per_block;
+    const int n_tok = (int)min((int64_t)a.tokens_per_block, p.tokens - tok0);
+    for (unsigned i = threadIdx.x; i < (unsigned)(n_tok * p.pairs); i += 256) {
+        const unsigned t = div_of(i, a.pairs), pr = i - t * p.pairs;
+        const int64_t at = (tok0 + t) * p.ldp + p.axis[pr];
         const double pos = p.positions_f32 ? (double)((const float*)p.positions)[at] : (double)((const int32_t*)p.positions)[at];
         float sn, cs;
-        turn_sincos(pos, p.turns[e], &sn, &cs);
-        const int ia = p.halves ? e : 2 * e, ib = p.halves ? e + p.pairs : 2 * e + 1;
-        const float a = (float)in[ia], b = (float)in[ib];
-        out[ia] = (T)(a * cs - b * sn);
-        out[ib] = (T)(a * sn + b * cs);
+        turn_sincos(pos, p.turns[pr], &sn, &cs);
+        turn[i] = float2{sn, cs};
+    }
+    __syncthreads();
+    const unsigned total = n_tok * a.per_token.d;
+    for (unsigned i = threadIdx.x; i < total; i += 256) {
+        const unsigned t = div_of(i, a.per_token), r = i - t * a.per_token.d;
+        const unsigned head = div_of(r, a.per_head), e = r - head * a.per_head.d;
+        const int64_t tok = tok0 + t;
+        const bool isk = head >= (unsigned)p.heads;
+        const T* in = isk ? (const T*)p.k + tok * p.ldk + (int)(head - p.heads) * p.d : (const T*)p.q + tok * p.ldq + (int)head * p.d;
+        T* out = isk ? (T*)p.out_k + tok * p.ldok + (int)(head - p.heads) * p.d : (T*)p.out_q + tok * p.ldoq + (int)head * p.d;
+        if (e >= (unsigned)a.rot_items) {   // what passes through
+            const int at = 2 * p.pairs + (int)(e - a.rot_items) * 8, n = p.d - at;
+            float v[8];
+            load8(in + at, n, v);
+            store8(out + at, n, v);
+            continue;
+        }
+        const float2* tr = turn + t * p.pairs;
+        if constexpr (HALVES) {
+            const int pr = (int)e * 8, n = p.pairs - pr;
+            float u[8], w[8];
+            load8(in + pr, n, u);
+            load8(in + p.pairs + pr, n, w);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+                const float2 sc = tr[min(pr + x, p.pairs - 1)];
+                const float x0 = u[x], y0 = w[x];
+                u[x] = x0 * sc.y - y0 * sc.x;
+                w[x] = x0 * sc.x + y0 * sc.y;
+            }
+            store8(out + pr, n, u);
+            store8(out + p.pairs + pr, n, w);
+        } else {
+            const int pr = (int)e * 4, n = 2 * (p.pairs - pr);
+            float u[8];
+            load8(in + 2 * pr, n, u);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const float2 sc = tr[min(pr + x, p.pairs - 1)];
+                const float x0 = u[2 * x], y0 = u[2 * x + 1];
+                u[2 * x] = x0 * sc.y - y0 * sc.x;
+                u[2 * x + 1] = x0 * sc.x + y0 * sc.y;
+            }
+            store8(out + 2 * pr, n, u);
+        }
     }
 }
 
@@ -41,13 +90,24 @@ extern "C" int mv_rotary_axes(const mv_rotary_desc* d, void* stream) {
     MV_REQUIRE(d->tokens >= 0 && d->heads >= 1 && d->d >= 2 && d->d <= 1024 && d->pairs >= 1 && 2 * d->pairs <= d->d && d->axes >= 1,
                "mv_rotary_axes: tokens %ld, heads %d, d %d, pairs %d, axes %d", (long)d->tokens, d->heads, d->d, d->pairs, d->axes);
     MV_REQUIRE(!d->k || d->kv_heads >= 1, "mv_rotary_axes: kv_heads %d", d->kv_heads);
-    MV_REQUIRE((int64_t)(d->heads + (d->k ? d->kv_heads : 0)) * d->d <= (1 << 24), "mv_rotary_axes: more than 2^24 elements per token");
+    MV_REQUIRE((int64_t)(d->heads + (d->k ? d->kv_heads : 0)) * d->d <= (1 << 17), "mv_rotary_axes: more than 2^17 elements per token");
     if (d->tokens == 0) return MV_OK;
     MV_REQUIRE(d->q && d->out_q && d->positions && d->turns && d->axis && (!d->k || d->out_k), "mv_rotary_axes: null pointer");
-    const int64_t work = d->tokens * (d->heads + (d->k ? d->kv_heads : 0)) * (d->d - d->pairs);
-    const int64_t want = (work + 255) / 256;
-    const int grid = (int)(want < 16384 ? want : 16384);
-    MV_DISPATCH_TYPE(d->dtype, (rotary_kernel<T><<<grid, 256, 0, (hipStream_t)stream>>>(*d)));
+    RotaryArgs a;
+    a.p = *d;
+    const int heads = d->heads + (d->k ? d->kv_heads : 0), tail = d->d - 2 * d->pairs;
+    a.rot_items = d->halves ? (d->pairs + 7) / 8 : (d->pairs + 3) / 4;
+    a.per_head = make_div(a.rot_items + (tail + 7) / 8);
+    a.per_token = make_div((unsigned)heads * a.per_head.d);
+    a.pairs = make_div(d->pairs);
+    MV_REQUIRE(a.per_token.d < 32768, "mv_rotary_axes: %u work items per token (below 32768)", a.per_token.d);   // (div_of's range with 4 tokens)
+    // several tokens per block where there are enough to fill the chip with blocks, one otherwise
+    a.tokens_per_block = d->tokens >= 4096 ? 4 : 1;
+    const int64_t grid = (d->tokens + a.tokens_per_block - 1) / a.tokens_per_block;
+    MV_REQUIRE(grid < (1ll << 31), "mv_rotary_axes: %ld tokens", (long)d->tokens);
+    const size_t lds = (size_t)a.tokens_per_block * d->pairs * sizeof(float2);
+    if (d->halves) MV_DISPATCH_TYPE(d->dtype, (rotary_kernel<T, true><<<(unsigned)grid, 256, lds, (hipStream_t)stream>>>(a)));
+    else MV_DISPATCH_TYPE(d->dtype, (rotary_kernel<T, false><<<(unsigned)grid, 256, lds, (hipStream_t)stream>>>(a)));
     MV_CHECK_LAUNCH("mv_rotary_axes");
     return MV_OK;
 }
