@@ -2,38 +2,102 @@
 #include "tok_common.h"
 
 // ---- activations to int8, one scale per row ------------------------------------------------------------------------------------
-// code = rne(127 x / top) with top = max |x|: 127 x is exact in fp32 for 16-bit inputs and a correctly rounded quotient of an 18-bit and
-// an 11-bit number is never rounded ONTO a tie (a value that is no tie is at least 2^-12 away from one, the quotient's half step is
-// 2^-18), so the code is that of the exact quotient.  f (a power of two) keeps 127 x of bf16's largest and smallest values in range.
+// code = rne(127 x / top) with top = max |x|, of the exact quotient q: x = X 2^a and top = T 2^b with integers X, T < 2^11, so a q that is no
+// half-integer is at least 1 / (2 T 2^(b - a)) = q / (2 * 127 X) > q 2^-19 away from every half-integer, and fp32 (2^-23 relative for the
+// two roundings below) resolves that.  f (a power of two) keeps the factors of bf16's largest and smallest values in range.
 struct RowScale {
-    float f, den, scale;
-    bool finite;
+    float f, inv, scale;
 };
 __device__ __forceinline__ RowScale row_scale(unsigned top_bits) {
     RowScale r;
     const float top = __uint_as_float(top_bits);
-    r.finite = top_bits < 0x7f800000u;
-    r.f = top > 0x1p100f ? 0x1p-32f : top < 0x1p-80f ? 0x1p64f : 1.0f;
-    r.den = top > 0.f && r.finite ? top * r.f : 1.0f;
+    const bool finite = top_bits < 0x7f800000u;
+    r.f = !finite ? 0.0f : top > 0x1p100f ? 0x1p-32f : top < 0x1p-80f ? 0x1p64f : 1.0f;
+    r.inv = top > 0.f && finite ? 127.0f / (top * r.f) : 0.0f;
     r.scale = top / 127.0f;
     return r;
 }
-__device__ __forceinline__ int row_code(float x, const RowScale& r) { return r.finite ? (int)rintf(127.0f * (x * r.f) / r.den) : 0; }
+// a product within q 2^-21 of a half-integer is that half-integer: the tie itself.  (A row that is not finite has f = inv = 0; its NaN and infinite elements become 0 in the last step.)
+__device__ __forceinline__ int row_code(float x, const RowScale& r) {
+    const float q = (x * r.f) * r.inv, twice = q + q, near = rintf(twice);
+    const float v = rintf(fabsf(twice - near) < fabsf(twice) * 0x1p-21f ? 0.5f * near : q);
+    return r.inv > 0.f ? (int)v : 0;
+}
 
-template <typename T>
-__global__ __launch_bounds__(256) void quantize_rows_kernel(const T* x, int64_t ldx, int k, int8_t* codes, int64_t ldc, float* scale) {
+// |x| as bits: ordered like the values, NaN above infinity
+__device__ __forceinline__ unsigned abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+template <int WAVES>
+__device__ __forceinline__ unsigned row_top(unsigned v, unsigned* red) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o, 64));
+    if constexpr (WAVES > 1) {
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = max(max(red[0], red[1]), max(red[2], red[3]));
+    }
+    return v;
+}
+__device__ __forceinline__ uint2 eight_codes(const float* v, const RowScale& r) {
+    unsigned w[2] = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e >> 2] |= (unsigned)(row_code(v[e], r) & 255) << (8 * (e & 3));
+    return uint2{w[0], w[1]};
+}
+
+// A row is read once and stays in registers between its maximum and its codes: NV chunks of 8 columns per lane, WAVES waves per row.  Rows
+// wider than the registers hold (REREAD) are read a second time, from the caches.  Bound by memory: 2 bytes in, 1 out per element.
+template <typename T, int NV, int WAVES, bool REREAD>
+__global__ __launch_bounds__(256) void quantize_rows_kernel(const T* x, int64_t ldx, int64_t rows, int k, int8_t* codes, int64_t ldc, float* scale) {
     __shared__ unsigned red[4];
-    const int64_t row = blockIdx.x;
+    constexpr int LANES = 64 * WAVES;
+    const int lane = threadIdx.x % LANES;
+    const int64_t row = (int64_t)blockIdx.x * (4 / WAVES) + threadIdx.x / LANES;
+    if (row >= rows) return;
     const T* xr = x + row * ldx;
-    unsigned top = 0;   // |x| as bits: ordered like the values, NaN above infinity
-    for (int i = threadIdx.x; i < k; i += 256) top = max(top, __float_as_uint((float)xr[i]) & 0x7fffffffu);
-    for (int o = 32; o > 0; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o, 64));
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
-    __syncthreads();
-    top = max(max(red[0], red[1]), max(red[2], red[3]));
-    const RowScale r = row_scale(top);
-    if (threadIdx.x == 0) scale[row] = r.scale;
-    for (int i = threadIdx.x; i < ldc; i += 256) codes[row * ldc + i] = i < k ? (int8_t)row_code((float)xr[i], r) : (int8_t)0;
+    int8_t* cr = codes + row * ldc;
+    float v[NV][8];
+    unsigned top = 0;
+    const int step = NV * LANES * 8;
+    for (int c0 = 0; c0 < (REREAD ? k : 1); c0 += step) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int col = c0 + (j * LANES + lane) * 8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
+            if (col < k) load8(xr + col, k - col, v[j]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = max(top, abs_bits(v[j][e]));
+        }
+    }
+    const RowScale r = row_scale(row_top<WAVES>(top, red));
+    if (lane == 0) scale[row] = r.scale;
+    for (int c0 = 0; c0 < (REREAD ? (int)ldc : 1); c0 += step) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int col = c0 + (j * LANES + lane) * 8;
+            if (REREAD) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
+                if (col < k) load8(xr + col, k - col, v[j]);
+            }
+            if (col < ldc) *(uint2*)(cr + col) = eight_codes(v[j], r);   // (columns from k on: codes of 0)
+        }
+    }
+}
+
+template <typename T, int NV, int WAVES, bool REREAD>
+static void launch_quantize(const void* x, int64_t ldx, int64_t rows, int k, int8_t* codes, int64_t ldc, float* scale, hipStream_t st) {
+    constexpr int R = 4 / WAVES;
+    quantize_rows_kernel<T, NV, WAVES, REREAD><<<(unsigned)((rows + R - 1) / R), 256, 0, st>>>((const T*)x, ldx, rows, k, codes, ldc, scale);
+}
+template <typename T>
+static void launch_quantize_width(const void* x, int64_t ldx, int64_t rows, int k, int8_t* codes, int64_t ldc, float* scale, hipStream_t st) {
+    if (ldc <= 512) launch_quantize<T, 1, 1, false>(x, ldx, rows, k, codes, ldc, scale, st);
+    else if (ldc <= 1536) launch_quantize<T, 3, 1, false>(x, ldx, rows, k, codes, ldc, scale, st);
+    else if (ldc <= 2048) launch_quantize<T, 1, 4, false>(x, ldx, rows, k, codes, ldc, scale, st);
+    else if (ldc <= 6144) launch_quantize<T, 3, 4, false>(x, ldx, rows, k, codes, ldc, scale, st);
+    else if (ldc <= 16384) launch_quantize<T, 8, 4, false>(x, ldx, rows, k, codes, ldc, scale, st);
+    else launch_quantize<T, 8, 4, true>(x, ldx, rows, k, codes, ldc, scale, st);
 }
 
 extern "C" int mv_quantize_rows_i8(const void* x, int64_t ldx, int64_t rows, int32_t k, int32_t dtype, int8_t* codes, int64_t ldc, float* scale,
@@ -43,38 +107,220 @@ extern "C" int mv_quantize_rows_i8(const void* x, int64_t ldx, int64_t rows, int
     MV_REQUIRE(ldc % 128 == 0 && ldc >= k && ldc < k + 128, "mv_quantize_rows_i8: code rows of %ld for k = %d (k rounded up to 128)", (long)ldc, k);
     if (rows == 0) return MV_OK;
     MV_REQUIRE(x && codes && scale && ((uintptr_t)codes & 15) == 0, "mv_quantize_rows_i8: null or unaligned pointer");
-    MV_DISPATCH_TYPE(dtype, (quantize_rows_kernel<T><<<(unsigned)rows, 256, 0, (hipStream_t)stream>>>((const T*)x, ldx, k, codes, ldc, scale)));
+    MV_DISPATCH_TYPE(dtype, launch_quantize_width<T>(x, ldx, rows, k, codes, ldc, scale, (hipStream_t)stream));
     MV_CHECK_LAUNCH("mv_quantize_rows_i8");
     return MV_OK;
 }
 
 // ---- the product ---------------------------------------------------------------------------------------------------------------
-template <typename T>
-__device__ __forceinline__ void store_i8_result(const mv_gemm_i8_desc& p, int64_t m, int n, int acc) {
-    float v = p.a_scale[m] * p.w_scale[n] * (float)acc;
-    if (p.bias) v += (float)((const T*)p.bias)[n];
-    if (p.act == MV_ACT_SILU) v = mv_silu(v);
-    if (p.residual) v += (float)((const T*)p.residual)[m * p.ldr + n];
-    ((T*)p.out)[m * p.ldo + n] = (T)v;
+__device__ __forceinline__ float i8_result(float a_scale, float w_scale, int acc, float bias, int act) {
+    float v = __builtin_fmaf(a_scale * w_scale, (float)acc, bias);
+    return act == MV_ACT_SILU ? mv_silu(v) : v;
+}
+
+typedef int int4v __attribute__((ext_vector_type(4)));
+typedef int int16v __attribute__((ext_vector_type(16)));
+
+// Tiles through LDS: BM rows of activations x BN rows of weights, 128 bytes of K per step, two stages, every wave WM x WN of the result in
+// v_mfma_i32_32x32x32_i8 blocks (weights as the first operand: a lane holds 4 consecutive outputs of one row).  LDS rows are 128 bytes =
+// 8 slots of 16; two rows share a 256-byte line of banks, so the slots of a row are permuted by (row >> 1) & 7 and a fragment read (16
+// rows, one slot) touches every bank once.  The permutation is applied to the column each lane fetches (global -> LDS directly).
+template <int BM, int BN, int WM, int WN>
+struct GemmI8Cfg {
+    static constexpr int WAVES = (BM / WM) * (BN / WN), THREADS = 64 * WAVES;
+    static constexpr int STAGE = (BM + BN) * 128;
+    static constexpr int PA = BM / 8 / WAVES, PW = BN / 8 / WAVES;   // 1-KiB pieces (8 rows) a wave fetches of each tile
+    static constexpr int SROW = WN + 4;                              // ints per row of the result staging
+    static constexpr int LDS = 2 * STAGE > WAVES * 32 * SROW * 4 ? 2 * STAGE : WAVES * 32 * SROW * 4;
+};
+
+template <typename T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__((GemmI8Cfg<BM, BN, WM, WN>::THREADS)) void gemm_i8_kernel(const mv_gemm_i8_desc p, const int tiles_m, const int tiles_n) {
+    using C = GemmI8Cfg<BM, BN, WM, WN>;
+    typedef __attribute__((address_space(3))) char lds_c;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    lds_c* const lds = (lds_c*)smem;
+    const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int tm, tn;
+    mv_tile_order(mv_xcd_remap(blockIdx.x, gridDim.x), tiles_m, tiles_n, MV_TILE_GROUP, &tm, &tn);
+    const int64_t m0 = (int64_t)tm * BM;
+    const int n0 = tn * BN;
+    const int wm = (wave / (BN / WN)) * WM, wn = (wave % (BN / WN)) * WN;
+
+    // descriptors end with the matrices' last rows: rows behind them read as 0
+    const int ma = (int)min((int64_t)BM, p.M - m0), na = min(BN, p.N - n0);
+    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)(p.a + m0 * p.lda), 0, (unsigned)(ma * p.lda), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)(p.w + n0 * p.ldw), 0, (unsigned)(na * p.ldw), 0x00020000);
+    unsigned oa[C::PA], ow[C::PW];
+#pragma unroll
+    for (int j = 0; j < C::PA; ++j) {
+        const int row = (wave * C::PA + j) * 8 + (lane >> 3);
+        oa[j] = (unsigned)(row * p.lda + (((lane & 7) ^ ((row >> 1) & 7)) << 4));
+    }
+#pragma unroll
+    for (int j = 0; j < C::PW; ++j) {
+        const int row = (wave * C::PW + j) * 8 + (lane >> 3);
+        ow[j] = (unsigned)(row * p.ldw + (((lane & 7) ^ ((row >> 1) & 7)) << 4));
+    }
+    auto issue = [&](int k, int stage) __attribute__((always_inline)) {
+        lds_c* dst = lds + stage * C::STAGE;
+#pragma unroll
+        for (int j = 0; j < C::PA; ++j)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void*)(dst + (wave * C::PA + j) * 1024), 16, (int)oa[j], k, 0, 0);
+#pragma unroll
+        for (int j = 0; j < C::PW; ++j)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (__attribute__((address_space(3))) void*)(dst + BM * 128 + (wave * C::PW + j) * 1024), 16, (int)ow[j], k, 0, 0);
+    };
+    int16v acc[WM / 32][WN / 32];
+#pragma unroll
+    for (int i = 0; i < WM / 32; ++i)
+#pragma unroll
+        for (int j = 0; j < WN / 32; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
+    int fo[4];   // byte offset of fragment step s in a 32-row block (row l31)
+#pragma unroll
+    for (int s = 0; s < 4; ++s) fo[s] = l31 * 128 + (((2 * s + h) ^ ((l31 >> 1) & 7)) << 4);
+
+    issue(0, 0);
+    int stage = 0;
+#pragma unroll 1
+    for (int k = 0; k < p.kp; k += 128) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wave's share of the step has landed ...
+        __builtin_amdgcn_s_barrier();                      // ... and everyone's; everyone has left the other stage
+        asm volatile("" ::: "memory");
+        if (k + 128 < p.kp) issue(k + 128, stage ^ 1);
+        const lds_c* sa = lds + stage * C::STAGE + wm * 128;
+        const lds_c* sw = lds + stage * C::STAGE + BM * 128 + wn * 128;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            int4v fa[WM / 32], fw[WN / 32];
+#pragma unroll
+            for (int i = 0; i < WM / 32; ++i) fa[i] = *(const __attribute__((address_space(3))) int4v*)(sa + i * 4096 + fo[s]);
+#pragma unroll
+            for (int j = 0; j < WN / 32; ++j) fw[j] = *(const __attribute__((address_space(3))) int4v*)(sw + j * 4096 + fo[s]);
+#pragma unroll
+            for (int i = 0; i < WM / 32; ++i)
+#pragma unroll
+                for (int j = 0; j < WN / 32; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[j], fa[i], acc[i][j], 0, 0, 0);
+        }
+        stage ^= 1;
+    }
+    __syncthreads();   // the stages become the waves' result staging
+
+    // 32 rows at a time through this wave's own LDS, so that rows are read (residual) and written 16 bytes per lane
+    int* st = (int*)smem + wave * 32 * C::SROW;
+    constexpr int LPR = WN / 8, RPP = 64 / LPR;   // lanes per row, rows per pass
+    const int c8 = (lane % LPR) * 8, n = n0 + wn + c8, left = p.N - n;
+    float ws[8], bs[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        ws[e] = e < left ? p.w_scale[n + e] : 0.f;
+        bs[e] = p.bias && e < left ? (float)((const T*)p.bias)[n + e] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < WM / 32; ++i) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int j = 0; j < WN / 32; ++j)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *(int4v*)(st + l31 * C::SROW + 32 * j + 8 * g + 4 * h) = int4v{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int r0 = 0; r0 < 32; r0 += RPP) {
+            const int row = r0 + lane / LPR;
+            const int64_t m = m0 + wm + 32 * i + row;
+            if (m >= p.M || left <= 0) continue;
+            const int4v u = *(const int4v*)(st + row * C::SROW + c8), w = *(const int4v*)(st + row * C::SROW + c8 + 4);
+            const float as = p.a_scale[m];
+            float v[8], r[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = i8_result(as, ws[e], e < 4 ? u[e & 3] : w[e & 3], bs[e], p.act);
+            if (p.residual) {
+                load8((const T*)p.residual + m * p.ldr + n, left, r);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] += r[e];
+            }
+            store8((T*)p.out + m * p.ldo + n, left, v);
+        }
+    }
+}
+
+// Few rows of activations (M <= 16 MT): the weights are streamed once, straight from memory into fragments.  A block owns 16 weight rows, its
+// 8 waves take 128-byte units of K in turn; in a unit, lane group g = lane / 16 holds bytes 32 g .. 32 g + 31 of its row as the fragments of two
+// v_mfma_i32_16x16x64_i8 (weights and activations in the same order of K: the sum does not care which).  The waves' sums meet in LDS.
+template <typename T, int MT>
+__global__ __launch_bounds__(512) void gemm_i8_few_kernel(const mv_gemm_i8_desc p) {
+    __shared__ int part[8][MT * 256];
+    const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n0 = blockIdx.x * 16;
+    const int8_t* w = p.w + (int64_t)min(n0 + l15, p.N - 1) * p.ldw + 32 * g;
+    const int8_t* a[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) a[t] = p.a + min((int64_t)(16 * t + l15), p.M - 1) * p.lda + 32 * g;
+    int4v acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = int4v{0, 0, 0, 0};
+    for (int k = wave * 128; k < p.kp; k += 8 * 128) {
+        const int4v w0 = *(const int4v*)(w + k), w1 = *(const int4v*)(w + k + 16);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const int4v a0 = *(const int4v*)(a[t] + k), a1 = *(const int4v*)(a[t] + k + 16);
+            acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w0, a0, acc[t], 0, 0, 0);
+            acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w1, a1, acc[t], 0, 0, 0);
+        }
+    }
+    // lane l holds weight rows 4 g .. 4 g + 3 of activation row l15
+#pragma unroll
+    for (int t = 0; t < MT; ++t) *(int4v*)(&part[wave][t * 256 + l15 * 16 + 4 * g]) = acc[t];
+    __syncthreads();
+    for (int x = tid; x < MT * 256; x += 512) {
+        const int64_t m = x >> 4;
+        const int n = n0 + (x & 15);
+        if (m >= p.M || n >= p.N) continue;
+        int sum = 0;
+#pragma unroll
+        for (int v = 0; v < 8; ++v) sum += part[v][x];
+        float v = i8_result(p.a_scale[m], p.w_scale[n], sum, p.bias ? (float)((const T*)p.bias)[n] : 0.f, p.act);
+        if (p.residual) v += (float)((const T*)p.residual)[m * p.ldr + n];
+        ((T*)p.out)[m * p.ldo + n] = (T)v;
+    }
+}
+
+template <typename T, int BM, int BN, int WM, int WN>
+static int launch_gemm_i8(const mv_gemm_i8_desc* d, hipStream_t st) {
+    using C = GemmI8Cfg<BM, BN, WM, WN>;
+    const auto kernel = gemm_i8_kernel<T, BM, BN, WM, WN>;
+    const int64_t tm = (d->M + BM - 1) / BM, tn = (d->N + BN - 1) / BN;
+    MV_REQUIRE(tm * tn < (1ll << 31), "mv_gemm_i8: %ld x %ld tiles", (long)tm, (long)tn);
+    if (C::LDS > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
+        if (e != hipSuccess) {
+            mv_set_error("mv_gemm_i8: %s", hipGetErrorString(e));
+            return MV_ERR_LAUNCH;
+        }
+    }
+    kernel<<<(unsigned)(tm * tn), C::THREADS, C::LDS, st>>>(*d, (int)tm, (int)tn);
+    MV_CHECK_LAUNCH("mv_gemm_i8");
+    return MV_OK;
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void gemm_i8_kernel(const mv_gemm_i8_desc p) {
-    const int n = blockIdx.x * 16 + (threadIdx.x & 15);
-    for (int64_t m = (int64_t)blockIdx.y * 16 + (threadIdx.x >> 4); m < p.M; m += (int64_t)gridDim.y * 16) {
-        if (n >= p.N) continue;
-        const int4* a = (const int4*)(p.a + m * p.lda);
-        const int4* w = (const int4*)(p.w + (int64_t)n * p.ldw);
-        int acc = 0;
-        for (int i = 0; i < p.kp / 16; ++i) {
-            const int4 u = a[i], v = w[i];
-            acc = __builtin_amdgcn_sdot4(u.x, v.x, acc, false);
-            acc = __builtin_amdgcn_sdot4(u.y, v.y, acc, false);
-            acc = __builtin_amdgcn_sdot4(u.z, v.z, acc, false);
-            acc = __builtin_amdgcn_sdot4(u.w, v.w, acc, false);
-        }
-        store_i8_result<T>(p, m, n, acc);
+static int launch_gemm_i8_shape(const mv_gemm_i8_desc* d, hipStream_t st) {
+    if (d->M <= 64) {
+        const unsigned grid = (d->N + 15) / 16;
+        if (d->M <= 16) gemm_i8_few_kernel<T, 1><<<grid, 512, 0, st>>>(*d);
+        else if (d->M <= 32) gemm_i8_few_kernel<T, 2><<<grid, 512, 0, st>>>(*d);
+        else gemm_i8_few_kernel<T, 4><<<grid, 512, 0, st>>>(*d);
+        MV_CHECK_LAUNCH("mv_gemm_i8");
+        return MV_OK;
     }
+    // 128 x 128 tiles where they fill the 256 CUs, 64 x 64 otherwise
+    const int64_t big = ((d->M + 127) / 128) * ((d->N + 127) / 128);
+    return big >= 256 ? launch_gemm_i8<T, 128, 128, 64, 64>(d, st) : launch_gemm_i8<T, 64, 64, 32, 32>(d, st);
 }
 
 extern "C" int mv_gemm_i8(const mv_gemm_i8_desc* d, void* stream) {
@@ -83,14 +329,11 @@ extern "C" int mv_gemm_i8(const mv_gemm_i8_desc* d, void* stream) {
     MV_REQUIRE(d->act == MV_ACT_NONE || d->act == MV_ACT_SILU, "mv_gemm_i8: activation %d", d->act);
     MV_REQUIRE(d->M >= 0 && d->M < (1ll << 31) && d->N >= 1 && d->kp >= 128 && d->kp % 128 == 0 && d->kp <= 131072,
                "mv_gemm_i8: M %ld, N %d, kp %d (a multiple of 128 up to 131072)", (long)d->M, d->N, d->kp);
-    MV_REQUIRE(d->lda % 128 == 0 && d->ldw % 128 == 0 && d->lda >= d->kp && d->ldw >= d->kp, "mv_gemm_i8: lda %ld, ldw %ld for kp %d", (long)d->lda,
+    MV_REQUIRE(d->lda % 128 == 0 && d->ldw % 128 == 0 && d->lda >= d->kp && d->ldw >= d->kp && d->lda <= (1 << 22) && d->ldw <= (1 << 22),
+               "mv_gemm_i8: lda %ld, ldw %ld for kp %d", (long)d->lda,
                (long)d->ldw, d->kp);
     if (d->M == 0) return MV_OK;
     MV_REQUIRE(d->a && d->w && d->a_scale && d->w_scale && d->out, "mv_gemm_i8: null pointer");
     MV_REQUIRE((((uintptr_t)d->a | (uintptr_t)d->w) & 15) == 0, "mv_gemm_i8: codes must be 16-byte aligned");
-    const int64_t mt = (d->M + 15) / 16;
-    const dim3 grid((d->N + 15) / 16, (unsigned)(mt < 32768 ? mt : 32768));
-    MV_DISPATCH_TYPE(d->dtype, (gemm_i8_kernel<T><<<grid, 256, 0, (hipStream_t)stream>>>(*d)));
-    MV_CHECK_LAUNCH("mv_gemm_i8");
-    return MV_OK;
+    return d->dtype == MV_F16 ? launch_gemm_i8_shape<half_t>(d, (hipStream_t)stream) : launch_gemm_i8_shape<bf16_t>(d, (hipStream_t)stream);
 }

@@ -390,7 +390,7 @@ def gated_residual_norm(x: torch.Tensor, f: torch.Tensor, *, kind: str = "layer"
         rows_per_group = int(rows_per_group)
         if groups is None or rows_per_group < 1 or groups * rows_per_group < rows:
             raise ValueError(f"gated_residual_norm: {groups} groups of {rows_per_group} rows do not cover {rows}")
-        ds.rows_per_group = rows_per_group
+        ds.rows_per_group = min(rows_per_group, _I32_MAX)
     elif groups is not None and groups > 1:
         raise ValueError(f"gated_residual_norm: {groups} groups need rows_per_group or group_index")
     ins = (("x", x), ("f", f), ("gate", gate), ("scale", scale), ("shift", shift), ("group_index", group_index))
