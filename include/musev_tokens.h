@@ -96,6 +96,19 @@ typedef struct mv_gemm_i8_desc {
     int32_t act, dtype;
 } mv_gemm_i8_desc;
 int mv_gemm_i8(const mv_gemm_i8_desc* d, void* stream);
+/* both in one call: x [M, K] of the element type; workspace: M * kp bytes of codes and M fp32 scales, 16-byte aligned */
+typedef struct mv_linear_i8_desc {
+    const void* x;
+    const int8_t* w;
+    const float* w_scale;
+    const void *bias, *residual;
+    void *out, *workspace;
+    int64_t M;
+    int32_t N, K;
+    int64_t kp, ldx, ldw, ldr, ldo;
+    int32_t act, dtype;
+} mv_linear_i8_desc;
+int mv_linear_i8(const mv_linear_i8_desc* d, void* stream);
 
 #ifdef __cplusplus
 }

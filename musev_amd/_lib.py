@@ -183,15 +183,24 @@ class GemmI8Desc(C.Structure):
     ]
 
 
+class LinearI8Desc(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("w", C.c_void_p), ("w_scale", C.c_void_p), ("bias", C.c_void_p), ("residual", C.c_void_p), ("out", C.c_void_p),
+        ("workspace", C.c_void_p), ("M", C.c_int64), ("N", C.c_int32), ("K", C.c_int32), ("kp", C.c_int64),
+        ("ldx", C.c_int64), ("ldw", C.c_int64), ("ldr", C.c_int64), ("ldo", C.c_int64), ("act", C.c_int32), ("dtype", C.c_int32),
+    ]
+
+
 MV_TOKENS_ABI_VERSION = 1
-TOKEN_SIGNATURES = {
+TOKEN_SIGNATURES = {   # (descriptors are passed as packed bytes or by reference)
     "mv_tokens_abi_version": (_i32, []),
     "mv_attention_packed_workspace_bytes": (_i64, [_i64, _i32, _i32]),
-    "mv_attention_packed": (_i32, [C.POINTER(AttnPackedDesc), _vp]),
-    "mv_rotary_axes": (_i32, [C.POINTER(RotaryDesc), _vp]),
-    "mv_gated_residual_norm": (_i32, [C.POINTER(GatedNormDesc), _vp]),
+    "mv_attention_packed": (_i32, [_vp, _vp]),
+    "mv_rotary_axes": (_i32, [_vp, _vp]),
+    "mv_gated_residual_norm": (_i32, [_vp, _vp]),
     "mv_quantize_rows_i8": (_i32, [_vp, _i64, _i64, _i32, _i32, _vp, _i64, _vp, _vp]),
-    "mv_gemm_i8": (_i32, [C.POINTER(GemmI8Desc), _vp]),
+    "mv_gemm_i8": (_i32, [_vp, _vp]),
+    "mv_linear_i8": (_i32, [_vp, _vp]),
 }
 
 _lib = None

@@ -113,30 +113,29 @@ extern "C" int mv_quantize_rows_i8(const void* x, int64_t ldx, int64_t rows, int
 }
 
 // ---- the product ---------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ float i8_result(float a_scale, float w_scale, int acc, float bias, int act) {
-    float v = __builtin_fmaf(a_scale * w_scale, (float)acc, bias);
-    return act == MV_ACT_SILU ? mv_silu(v) : v;
-}
-
 typedef int int4v __attribute__((ext_vector_type(4)));
 typedef int int16v __attribute__((ext_vector_type(16)));
 
-// Tiles through LDS: BM rows of activations x BN rows of weights, 128 bytes of K per step, two stages, every wave WM x WN of the result in
-// v_mfma_i32_32x32x32_i8 blocks (weights as the first operand: a lane holds 4 consecutive outputs of one row).  LDS rows are 128 bytes =
-// 8 slots of 16; two rows share a 256-byte line of banks, so the slots of a row are permuted by (row >> 1) & 7 and a fragment read (16
-// rows, one slot) touches every bank once.  The permutation is applied to the column each lane fetches (global -> LDS directly).
-template <int BM, int BN, int WM, int WN>
+// Tiles through LDS: BM rows of activations x BN rows of weights, BK bytes of K per step, NST stages of which NST - 1 are in flight, every
+// wave WM x WN of the result in v_mfma_i32_32x32x32_i8 blocks (weights as the first operand: a lane holds 4 consecutive outputs of one
+// row).  LDS rows are BK bytes = SLOTS slots of 16; 256 / BK rows share a 256-byte line of banks, so the slots of a row are permuted by the
+// line's number and a fragment read (16 rows, one slot) touches every bank once.  The permutation is applied to the column each lane
+// fetches (global -> LDS directly).
+template <int BM, int BN, int WM, int WN, int BK, int NST>
 struct GemmI8Cfg {
     static constexpr int WAVES = (BM / WM) * (BN / WN), THREADS = 64 * WAVES;
-    static constexpr int STAGE = (BM + BN) * 128;
-    static constexpr int PA = BM / 8 / WAVES, PW = BN / 8 / WAVES;   // 1-KiB pieces (8 rows) a wave fetches of each tile
-    static constexpr int SROW = WN + 4;                              // ints per row of the result staging
-    static constexpr int LDS = 2 * STAGE > WAVES * 32 * SROW * 4 ? 2 * STAGE : WAVES * 32 * SROW * 4;
+    static constexpr int SLOTS = BK / 16, PROWS = 1024 / BK;            // slots of a row; rows of a 1-KiB piece
+    static constexpr int STAGE = (BM + BN) * BK;
+    static constexpr int PA = BM / PROWS / WAVES, PW = BN / PROWS / WAVES;   // pieces a wave fetches of each tile
+    static constexpr int SROW = WN + 4;                                 // ints per row of the result staging
+    static constexpr int LDS = NST * STAGE > WAVES * 32 * SROW * 4 ? NST * STAGE : WAVES * 32 * SROW * 4;
+    static_assert(BM % (PROWS * WAVES) == 0 && BN % (PROWS * WAVES) == 0, "every wave fetches whole pieces");
+    static __device__ __forceinline__ int swz(int row) { return (row / (256 / BK)) % SLOTS; }
 };
 
-template <typename T, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__((GemmI8Cfg<BM, BN, WM, WN>::THREADS)) void gemm_i8_kernel(const mv_gemm_i8_desc p, const int tiles_m, const int tiles_n) {
-    using C = GemmI8Cfg<BM, BN, WM, WN>;
+template <typename T, int BM, int BN, int WM, int WN, int BK, int NST>
+__global__ __launch_bounds__((GemmI8Cfg<BM, BN, WM, WN, BK, NST>::THREADS), 2) void gemm_i8_kernel(const mv_gemm_i8_desc p, const int tiles_m, const int tiles_n) {
+    using C = GemmI8Cfg<BM, BN, WM, WN, BK, NST>;
     typedef __attribute__((address_space(3))) char lds_c;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     lds_c* const lds = (lds_c*)smem;
@@ -153,15 +152,16 @@ __global__ __launch_bounds__((GemmI8Cfg<BM, BN, WM, WN>::THREADS)) void gemm_i8_
     const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)(p.a + m0 * p.lda), 0, (unsigned)(ma * p.lda), 0x00020000);
     const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)(p.w + n0 * p.ldw), 0, (unsigned)(na * p.ldw), 0x00020000);
     unsigned oa[C::PA], ow[C::PW];
+    const int prow = lane / C::SLOTS, pslot = lane % C::SLOTS;
 #pragma unroll
     for (int j = 0; j < C::PA; ++j) {
-        const int row = (wave * C::PA + j) * 8 + (lane >> 3);
-        oa[j] = (unsigned)(row * p.lda + (((lane & 7) ^ ((row >> 1) & 7)) << 4));
+        const int row = (wave * C::PA + j) * C::PROWS + prow;
+        oa[j] = (unsigned)(row * p.lda + ((pslot ^ C::swz(row)) << 4));
     }
 #pragma unroll
     for (int j = 0; j < C::PW; ++j) {
-        const int row = (wave * C::PW + j) * 8 + (lane >> 3);
-        ow[j] = (unsigned)(row * p.ldw + (((lane & 7) ^ ((row >> 1) & 7)) << 4));
+        const int row = (wave * C::PW + j) * C::PROWS + prow;
+        ow[j] = (unsigned)(row * p.ldw + ((pslot ^ C::swz(row)) << 4));
     }
     auto issue = [&](int k, int stage) __attribute__((always_inline)) {
         lds_c* dst = lds + stage * C::STAGE;
@@ -170,7 +170,7 @@ __global__ __launch_bounds__((GemmI8Cfg<BM, BN, WM, WN>::THREADS)) void gemm_i8_
             __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void*)(dst + (wave * C::PA + j) * 1024), 16, (int)oa[j], k, 0, 0);
 #pragma unroll
         for (int j = 0; j < C::PW; ++j)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (__attribute__((address_space(3))) void*)(dst + BM * 128 + (wave * C::PW + j) * 1024), 16, (int)ow[j], k, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (__attribute__((address_space(3))) void*)(dst + BM * BK + (wave * C::PW + j) * 1024), 16, (int)ow[j], k, 0, 0);
     };
     int16v acc[WM / 32][WN / 32];
 #pragma unroll
@@ -179,40 +179,73 @@ __global__ __launch_bounds__((GemmI8Cfg<BM, BN, WM, WN>::THREADS)) void gemm_i8_
         for (int j = 0; j < WN / 32; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
-    int fo[4];   // byte offset of fragment step s in a 32-row block (row l31)
+    int fo[BK / 32];   // byte offset of fragment step s in a 32-row block (row l31)
 #pragma unroll
-    for (int s = 0; s < 4; ++s) fo[s] = l31 * 128 + (((2 * s + h) ^ ((l31 >> 1) & 7)) << 4);
+    for (int s = 0; s < BK / 32; ++s) fo[s] = l31 * BK + (((2 * s + h) ^ C::swz(l31)) << 4);
 
-    issue(0, 0);
-    int stage = 0;
-#pragma unroll 1
-    for (int k = 0; k < p.kp; k += 128) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wave's share of the step has landed ...
-        __builtin_amdgcn_s_barrier();                      // ... and everyone's; everyone has left the other stage
-        asm volatile("" ::: "memory");
-        if (k + 128 < p.kp) issue(k + 128, stage ^ 1);
-        const lds_c* sa = lds + stage * C::STAGE + wm * 128;
-        const lds_c* sw = lds + stage * C::STAGE + BM * 128 + wn * 128;
+    // what the result needs besides the sums.  A lane holds row l31 of every 32 while it multiplies, and finishes columns n .. n + 7 of the rows
+    // lane / LPR + RPP x of every 32.
+    typedef typename Vec8<T>::type V8;
+    constexpr int LPR = WN / 8, RPP = 64 / LPR, PASSES = 32 / RPP, NRES = WM / 32 * PASSES;   // lanes per row, rows per pass
+    constexpr int FIRST = NRES > 8 ? NRES / 2 : NRES;   // residual loads the registers have room for beside the fragments; the others follow the last step
+    const int c8 = (lane % LPR) * 8, n = n0 + wn + c8, left = p.N - n, frow = lane / LPR;
+    float as[WM / 32];
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
+    for (int i = 0; i < WM / 32; ++i) as[i] = p.a_scale[min(m0 + wm + 32 * i + l31, p.M - 1)];
+    // The residual is fetched beside the last two steps: as long as the sums take, its loads are hidden (26 624 x 1280 -> 5120: one block per CU,
+    // nothing else would hide them).  Only whole 16-byte loads, so that their number is known to the wait below; rows and columns past the end
+    // fetch the last ones.  Otherwise it is read where it is added.
+    V8 res[NRES];
+    auto residual_at = [&](int x) __attribute__((always_inline)) {
+        return (const V8*)((const T*)p.residual + min(m0 + wm + 32 * (x / PASSES) + (x % PASSES) * RPP + frow, p.M - 1) * p.ldr + min(n, p.N - 8));
+    };
+    const bool early = p.residual && p.kp >= 2 * BK && ((p.N | p.ldr) & 7) == 0 && ((uintptr_t)p.residual & 15) == 0;
+
+    const int steps = p.kp / BK;   // (kp is a multiple of 128: at least two steps of 64)
+    int into = 0, from = 0;
+#pragma unroll
+    for (int s = 0; s < NST - 1; ++s)
+        if (s < steps) issue(s * BK, into++);
+#pragma unroll 1
+    for (int t = 0; t < steps; ++t) {
+        // this wave's share of step t has landed ... (younger steps may be on their way)
+        if (t + 1 == steps && early) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(FIRST) : "memory");   // (the residual's loads are the youngest)
+        else if (NST > 2 && t + NST - 2 < steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * (C::PA + C::PW)) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();                      // ... and everyone's; everyone has left the stage of step t - 1
+        asm volatile("" ::: "memory");
+        if (t + NST - 1 < steps) issue((t + NST - 1) * BK, into);
+        if (t + 2 == steps && early) {
+            asm volatile("" ::: "memory");   // (behind the last stage's loads)
+#pragma unroll
+            for (int x = 0; x < FIRST; ++x) res[x] = *residual_at(x);
+            asm volatile("" ::: "memory");
+        }
+        into = into + 1 == NST ? 0 : into + 1;
+        const lds_c* sa = lds + from * C::STAGE + wm * BK;
+        const lds_c* sw = lds + from * C::STAGE + BM * BK + wn * BK;
+        from = from + 1 == NST ? 0 : from + 1;
+#pragma unroll
+        for (int s = 0; s < BK / 32; ++s) {
             int4v fa[WM / 32], fw[WN / 32];
 #pragma unroll
-            for (int i = 0; i < WM / 32; ++i) fa[i] = *(const __attribute__((address_space(3))) int4v*)(sa + i * 4096 + fo[s]);
+            for (int i = 0; i < WM / 32; ++i) fa[i] = *(const __attribute__((address_space(3))) int4v*)(sa + i * 32 * BK + fo[s]);
 #pragma unroll
-            for (int j = 0; j < WN / 32; ++j) fw[j] = *(const __attribute__((address_space(3))) int4v*)(sw + j * 4096 + fo[s]);
+            for (int j = 0; j < WN / 32; ++j) fw[j] = *(const __attribute__((address_space(3))) int4v*)(sw + j * 32 * BK + fo[s]);
 #pragma unroll
             for (int i = 0; i < WM / 32; ++i)
 #pragma unroll
                 for (int j = 0; j < WN / 32; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[j], fa[i], acc[i][j], 0, 0, 0);
         }
-        stage ^= 1;
+    }
+    if (early) {
+#pragma unroll
+        for (int x = FIRST; x < NRES; ++x) res[x] = *residual_at(x);
     }
     __syncthreads();   // the stages become the waves' result staging
 
     // 32 rows at a time through this wave's own LDS, so that rows are read (residual) and written 16 bytes per lane
-    int* st = (int*)smem + wave * 32 * C::SROW;
-    constexpr int LPR = WN / 8, RPP = 64 / LPR;   // lanes per row, rows per pass
-    const int c8 = (lane % LPR) * 8, n = n0 + wn + c8, left = p.N - n;
+    float* st = (float*)smem + wave * 32 * C::SROW;
     float ws[8], bs[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -225,20 +258,30 @@ __global__ __launch_bounds__((GemmI8Cfg<BM, BN, WM, WN>::THREADS)) void gemm_i8_
 #pragma unroll
         for (int j = 0; j < WN / 32; ++j)
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
-                *(int4v*)(st + l31 * C::SROW + 32 * j + 8 * g + 4 * h) = int4v{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+            for (int g = 0; g < 4; ++g) {
+                float4v v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = (float)acc[i][j][4 * g + e] * as[i];
+                *(float4v*)(st + l31 * C::SROW + 32 * j + 8 * g + 4 * h) = v;
+            }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-        for (int r0 = 0; r0 < 32; r0 += RPP) {
-            const int row = r0 + lane / LPR;
+        for (int x = 0; x < PASSES; ++x) {
+            const int row = x * RPP + frow;
             const int64_t m = m0 + wm + 32 * i + row;
             if (m >= p.M || left <= 0) continue;
-            const int4v u = *(const int4v*)(st + row * C::SROW + c8), w = *(const int4v*)(st + row * C::SROW + c8 + 4);
-            const float as = p.a_scale[m];
-            float v[8], r[8];
+            const float4v u = *(const float4v*)(st + row * C::SROW + c8), w = *(const float4v*)(st + row * C::SROW + c8 + 4);
+            float v[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = i8_result(as, ws[e], e < 4 ? u[e & 3] : w[e & 3], bs[e], p.act);
-            if (p.residual) {
+            for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(e < 4 ? u[e & 3] : w[e & 3], ws[e], bs[e]);
+            if (p.act == MV_ACT_SILU)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = mv_silu(v[e]);
+            if (early) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] += (float)res[i * PASSES + x][e];
+            } else if (p.residual) {
+                float r[8];
                 load8((const T*)p.residual + m * p.ldr + n, left, r);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] += r[e];
@@ -284,16 +327,17 @@ __global__ __launch_bounds__(512) void gemm_i8_few_kernel(const mv_gemm_i8_desc 
         int sum = 0;
 #pragma unroll
         for (int v = 0; v < 8; ++v) sum += part[v][x];
-        float v = i8_result(p.a_scale[m], p.w_scale[n], sum, p.bias ? (float)((const T*)p.bias)[n] : 0.f, p.act);
+        float v = __builtin_fmaf((float)sum * p.a_scale[m], p.w_scale[n], p.bias ? (float)((const T*)p.bias)[n] : 0.f);
+        if (p.act == MV_ACT_SILU) v = mv_silu(v);
         if (p.residual) v += (float)((const T*)p.residual)[m * p.ldr + n];
         ((T*)p.out)[m * p.ldo + n] = (T)v;
     }
 }
 
-template <typename T, int BM, int BN, int WM, int WN>
+template <typename T, int BM, int BN, int WM, int WN, int BK, int NST>
 static int launch_gemm_i8(const mv_gemm_i8_desc* d, hipStream_t st) {
-    using C = GemmI8Cfg<BM, BN, WM, WN>;
-    const auto kernel = gemm_i8_kernel<T, BM, BN, WM, WN>;
+    using C = GemmI8Cfg<BM, BN, WM, WN, BK, NST>;
+    const auto kernel = gemm_i8_kernel<T, BM, BN, WM, WN, BK, NST>;
     const int64_t tm = (d->M + BM - 1) / BM, tn = (d->N + BN - 1) / BN;
     MV_REQUIRE(tm * tn < (1ll << 31), "mv_gemm_i8: %ld x %ld tiles", (long)tm, (long)tn);
     if (C::LDS > 64 * 1024) {
@@ -310,17 +354,20 @@ static int launch_gemm_i8(const mv_gemm_i8_desc* d, hipStream_t st) {
 
 template <typename T>
 static int launch_gemm_i8_shape(const mv_gemm_i8_desc* d, hipStream_t st) {
-    if (d->M <= 64) {
+    if (d->M <= 32) {
         const unsigned grid = (d->N + 15) / 16;
         if (d->M <= 16) gemm_i8_few_kernel<T, 1><<<grid, 512, 0, st>>>(*d);
-        else if (d->M <= 32) gemm_i8_few_kernel<T, 2><<<grid, 512, 0, st>>>(*d);
-        else gemm_i8_few_kernel<T, 4><<<grid, 512, 0, st>>>(*d);
+        else gemm_i8_few_kernel<T, 2><<<grid, 512, 0, st>>>(*d);
         MV_CHECK_LAUNCH("mv_gemm_i8");
         return MV_OK;
     }
-    // 128 x 128 tiles where they fill the 256 CUs, 64 x 64 otherwise
-    const int64_t big = ((d->M + 127) / 128) * ((d->N + 127) / 128);
-    return big >= 256 ? launch_gemm_i8<T, 128, 128, 64, 64>(d, st) : launch_gemm_i8<T, 64, 64, 32, 32>(d, st);
+    // The largest tile that still gives every CU a few blocks: 256 x 256 (one block per CU) from four rounds on, 128 x 64 (three per CU) from two
+    // blocks per CU, 64 x 64 below.  Measured (us, 256 x 256 / 128 x 64 / 64 x 64): 8192^3 475 / 661 / -; 26 624 x 1280 x 5120 278 / 325 / 385;
+    // 4096 x 1280 x 2560 27.6 / 25.9 / 32.3; 2048 x 1280 x 1280 23.7 / 10.3 / 10.2; 512 x 1280 x 1280 23 / 8.6 / 6.4.
+    const auto tiles = [&](int64_t bm, int64_t bn) { return ((d->M + bm - 1) / bm) * ((d->N + bn - 1) / bn); };
+    if (tiles(256, 256) >= 1024) return launch_gemm_i8<T, 256, 256, 128, 64, 128, 2>(d, st);
+    if (tiles(128, 64) >= 512) return launch_gemm_i8<T, 128, 64, 64, 32, 128, 2>(d, st);
+    return launch_gemm_i8<T, 64, 64, 32, 32, 128, 2>(d, st);
 }
 
 extern "C" int mv_gemm_i8(const mv_gemm_i8_desc* d, void* stream) {
@@ -336,4 +383,30 @@ extern "C" int mv_gemm_i8(const mv_gemm_i8_desc* d, void* stream) {
     MV_REQUIRE(d->a && d->w && d->a_scale && d->w_scale && d->out, "mv_gemm_i8: null pointer");
     MV_REQUIRE((((uintptr_t)d->a | (uintptr_t)d->w) & 15) == 0, "mv_gemm_i8: codes must be 16-byte aligned");
     return d->dtype == MV_F16 ? launch_gemm_i8_shape<half_t>(d, (hipStream_t)stream) : launch_gemm_i8_shape<bf16_t>(d, (hipStream_t)stream);
+}
+
+extern "C" int mv_linear_i8(const mv_linear_i8_desc* d, void* stream) {
+    MV_REQUIRE(d, "mv_linear_i8: null descriptor");
+    MV_REQUIRE(d->M >= 0 && d->K >= 1 && d->kp >= d->K && d->kp < d->K + 128 && d->kp % 128 == 0, "mv_linear_i8: M %ld, K %d, kp %ld", (long)d->M, d->K, (long)d->kp);
+    if (d->M == 0) return MV_OK;
+    MV_REQUIRE(d->workspace, "mv_linear_i8: null workspace");
+    mv_gemm_i8_desc g;
+    g.a = (const int8_t*)d->workspace;
+    g.a_scale = (const float*)(g.a + d->M * d->kp);
+    g.w = d->w;
+    g.w_scale = d->w_scale;
+    g.bias = d->bias;
+    g.residual = d->residual;
+    g.out = d->out;
+    g.M = d->M;
+    g.N = d->N;
+    g.kp = (int32_t)d->kp;
+    g.lda = d->kp;
+    g.ldw = d->ldw;
+    g.ldr = d->ldr;
+    g.ldo = d->ldo;
+    g.act = d->act;
+    g.dtype = d->dtype;
+    const int rc = mv_quantize_rows_i8(d->x, d->ldx, d->M, d->K, d->dtype, (int8_t*)d->workspace, d->kp, (float*)g.a_scale, stream);
+    return rc == MV_OK ? mv_gemm_i8(&g, stream) : rc;
 }

@@ -11,12 +11,13 @@ from __future__ import annotations
 
 import ctypes as C
 import math
-from typing import List, Optional, Sequence, Tuple, Union
+import struct
+from typing import Callable, List, Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import _lib
-from ._lib import MV_ACT_NONE, MV_ACT_SILU, AttnPackedDesc, GatedNormDesc, GemmI8Desc, RotaryDesc, check
+from ._lib import MV_ACT_NONE, MV_ACT_SILU, AttnPackedDesc, GatedNormDesc, GemmI8Desc, LinearI8Desc, RotaryDesc, check
 
 __all__ = ["AttentionPlan", "attention_plan", "attention_packed", "RotaryTable", "rotary_table", "rotary_axes", "gated_residual_norm",
            "Int8Rows", "pack_weight_i8", "quantize_rows_i8", "gemm_i8", "linear_i8"]
@@ -24,43 +25,61 @@ __all__ = ["AttentionPlan", "attention_plan", "attention_packed", "RotaryTable",
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 _I32_MAX = 2 ** 31 - 1
 
+# A small call's time is the host's: checks read each tensor's geometry once, a descriptor is packed in one go, the stream is asked for as a
+# raw handle.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+
+
+def _packer(desc) -> Callable[..., bytes]:
+    """packs a descriptor's fields, in their order, into the bytes of the C struct (0 for a null pointer)"""
+    code = {C.c_void_p: "P", C.c_int64: "q", C.c_int32: "i", C.c_float: "f"}
+    form = struct.Struct("@" + "".join(code[t] for _, t in desc._fields_) + "0P")
+    assert form.size == C.sizeof(desc)
+    return form.pack
+
+
+_pack_attention, _pack_rotary, _pack_norm, _pack_gemm, _pack_linear = (_packer(d) for d in (AttnPackedDesc, RotaryDesc, GatedNormDesc, GemmI8Desc,
+                                                                                           LinearI8Desc))
+
 
 def _on_gpu(t: torch.Tensor) -> bool:
     return t.is_cuda
 
 
-class _device_of:
-    """makes ``dev`` the current device for a launch (only where it is not already) and gives the raw handle of its current stream"""
-
-    def __init__(self, dev: torch.device):
-        self.idx = dev.index
-
-    def __enter__(self) -> int:
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.idx:
-            torch.cuda.set_device(self.idx)
-        return torch.cuda.current_stream(self.idx).cuda_stream
-
-    def __exit__(self, *exc) -> None:
-        if self.prev != self.idx:
-            torch.cuda.set_device(self.prev)
+def _launch(entry: str, desc: bytes, dev: int, held: Sequence["_Held"] = ()) -> None:
+    """one call of the C ABI on device ``dev``'s current stream"""
+    if _current_device() != dev:
+        with torch.cuda.device(dev):
+            return _launch(entry, desc, dev, held)
+    stream = _raw_stream(dev)
+    for h in held:
+        if stream not in h._streams:
+            h._use(stream)
+    status = getattr(_lib.load(), entry)(desc, stream)
+    if status:
+        check(status, entry)
 
 
-def _matrix(t: torch.Tensor, name: str, dtype: Optional[torch.dtype] = None, device: Optional[torch.device] = None) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor) or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"{name}: expected a 2-D tensor with unit inner stride, got "
-                         f"{(tuple(t.shape), t.stride()) if isinstance(t, torch.Tensor) else type(t).__name__}")
+def _matrix(t: torch.Tensor, name: str, dtype: Optional[torch.dtype] = None, dev: Optional[int] = None) -> Tuple[int, int, int]:
+    """(rows, columns, row stride) of a 2-D tensor with unit inner stride on the GPU; a single row has no stride of its own: its width stands in"""
+    if not isinstance(t, torch.Tensor) or t.ndim != 2:
+        raise ValueError(f"{name}: expected a 2-D tensor, got {tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__}")
+    (rows, cols), (ld, inner) = t.shape, t.stride()
+    if inner != 1 and cols > 1:
+        raise ValueError(f"{name}: expected unit inner stride, got shape {(rows, cols)} strides {(ld, inner)}")
     if not _on_gpu(t) or (t.dtype not in _DTYPES if dtype is None else t.dtype != dtype):
         raise ValueError(f"{name}: expected a CUDA {'fp16 | bf16' if dtype is None else dtype} tensor, got {t.dtype} on {t.device}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name}: on {t.device}, the other tensors are on {device}")
-    if t.shape[0] > 1 and (t.stride(0) > _I32_MAX or (t.stride(0) < t.shape[1])):
-        raise ValueError(f"{name}: row stride {t.stride(0)} for {t.shape[1]} columns")
-    return t
+    if dev is not None and t.get_device() != dev:
+        raise ValueError(f"{name}: on {t.device}, the other tensors are on device {dev}")
+    if rows <= 1:
+        return rows, cols, cols
+    if ld < cols or ld > _I32_MAX:
+        raise ValueError(f"{name}: row stride {ld} for {cols} columns")
+    return rows, cols, ld
 
 
 def _ld(t: torch.Tensor) -> int:
-    """row stride in elements (a single row has none of its own)"""
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
@@ -101,11 +120,12 @@ class _Held:
     def _hold(self, *tensors: torch.Tensor) -> None:
         self._tensors = tensors
         self.device = tensors[0].device
-        self._streams = {torch.cuda.current_stream(self.device).cuda_stream} if tensors[0].is_cuda else set()
+        self._dev = tensors[0].get_device()
+        self._streams = {_raw_stream(self._dev)} if tensors[0].is_cuda else set()
 
     def _use(self, stream: int) -> None:
-        # the allocator may not hand the memory out again while a launch on another stream still reads it
-        if stream not in self._streams and not torch.cuda.is_current_stream_capturing():
+        # (first use on a stream) the allocator may not hand the memory out again while a launch there still reads it
+        if not torch.cuda.is_current_stream_capturing():
             for t in self._tensors:
                 t.record_stream(torch.cuda.current_stream(self.device))
             self._streams.add(stream)
@@ -119,12 +139,9 @@ class AttentionPlan(_Held):
         self.q_lens, self.kv_lens = tuple(q_lens), tuple(kv_lens)
         self.heads, self.kv_heads, self.d, self.causal, self.scale = heads, kv_heads, d, causal, scale
         self.total_q, self.total_kv = sum(q_lens), sum(kv_lens)
+        self.n_items, self.n_few, self.n_joins, self.ws_rows = n_items, n_few, joins.shape[0], ws_rows
         self._hold(items, joins)
-        ds = AttnPackedDesc()
-        ds.items, ds.joins = items.data_ptr(), joins.data_ptr()
-        ds.n_items, ds.n_few, ds.n_joins, ds.ws_rows = n_items, n_few, joins.shape[0], ws_rows
-        ds.heads, ds.kv_heads, ds.d, ds.causal, ds.scale = heads, kv_heads, d, int(causal), scale
-        self._desc = ds
+        self._tables = items.data_ptr(), joins.data_ptr()
         self._workspace = 4 * ws_rows * kv_heads * (d + 2)   # mv_attention_packed_workspace_bytes
 
 
@@ -214,36 +231,34 @@ def attention_packed(plan: AttentionPlan, q: torch.Tensor, k: torch.Tensor, v: t
     stride that keeps rows 16-byte aligned (column slices of a fused projection).  Returns [total_q, heads * d], or writes the first
     total_q rows of ``out`` and leaves the rows behind them as they were.  A query that sees no key gives 0; what a query does not see --
     later tokens, other sequences, rows behind the last one -- does not reach its output, NaN and infinities included."""
-    _matrix(q, "q")
-    _matrix(k, "k", q.dtype, q.device)
-    _matrix(v, "v", q.dtype, q.device)
+    rows, cols, ldq = _matrix(q, "q")
+    dtype, dev = q.dtype, q.get_device()
     hd, kvd = plan.heads * plan.d, plan.kv_heads * plan.d
-    if q.shape[1] != hd or q.shape[0] < plan.total_q:
-        raise ValueError(f"attention_packed: q {tuple(q.shape)}, the plan has {plan.total_q} rows of {hd}")
-    for t, nm in ((k, "k"), (v, "v")):
-        if t.shape[1] != kvd or t.shape[0] < plan.total_kv:
-            raise ValueError(f"attention_packed: {nm} {tuple(t.shape)}, the plan has {plan.total_kv} rows of {kvd}")
-    for t, nm in ((q, "q"), (k, "k"), (v, "v")) + (((_matrix(out, "out", q.dtype, q.device), "out"),) if out is not None else ()):
-        if t.data_ptr() % 16 or _ld(t) % 8 or _ld(t) > 1 << 23:
-            raise ValueError(f"attention_packed: {nm}: rows must be 16-byte aligned and at most 2^23 elements apart, row stride {_ld(t)}")
-    if plan.device != q.device:
+    if cols != hd or rows < plan.total_q:
+        raise ValueError(f"attention_packed: q {(rows, cols)}, the plan has {plan.total_q} rows of {hd}")
+    rows, cols, ldk = _matrix(k, "k", dtype, dev)
+    if cols != kvd or rows < plan.total_kv:
+        raise ValueError(f"attention_packed: k {(rows, cols)}, the plan has {plan.total_kv} rows of {kvd}")
+    rows, cols, ldv = _matrix(v, "v", dtype, dev)
+    if cols != kvd or rows < plan.total_kv:
+        raise ValueError(f"attention_packed: v {(rows, cols)}, the plan has {plan.total_kv} rows of {kvd}")
+    if plan._dev != dev:
         raise ValueError(f"attention_packed: plan on {plan.device}, tensors on {q.device}")
     if out is None:
-        out = torch.empty((plan.total_q, hd), dtype=q.dtype, device=q.device)
+        out, ldo = q.new_empty((plan.total_q, hd)), hd
     else:
-        if out.shape[1] != hd or out.shape[0] < plan.total_q:
-            raise ValueError(f"attention_packed: out {tuple(out.shape)}, the plan has {plan.total_q} rows of {hd}")
+        rows, cols, ldo = _matrix(out, "out", dtype, dev)
+        if cols != hd or rows < plan.total_q:
+            raise ValueError(f"attention_packed: out {(rows, cols)}, the plan has {plan.total_q} rows of {hd}")
         _no_overlap(out[:plan.total_q], "attention_packed: out", (("q", q), ("k", k), ("v", v)))
-    ds = AttnPackedDesc.from_buffer_copy(plan._desc)
-    ds.q, ds.k, ds.v, ds.out = q.data_ptr(), k.data_ptr() or q.data_ptr(), v.data_ptr() or q.data_ptr(), out.data_ptr()   # (no key at all: not read)
-    ds.ldq, ds.ldk, ds.ldv, ds.ldo, ds.dtype = _ld(q), _ld(k), _ld(v), _ld(out), _DTYPES[q.dtype]
-    with _device_of(q.device) as stream:
-        plan._use(stream)
-        ws = None
-        if plan._workspace:
-            ws = torch.empty(plan._workspace, dtype=torch.uint8, device=q.device)
-            ds.workspace, ds.workspace_bytes = ws.data_ptr(), plan._workspace
-        check(_lib.load().mv_attention_packed(C.byref(ds), stream), "mv_attention_packed")
+    pq, pk, pv, po = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    if (pq | pk | pv | po) & 15 or (ldq | ldk | ldv | ldo) & 7 or max(ldk, ldv) > 1 << 23:
+        raise ValueError(f"attention_packed: rows must be 16-byte aligned and k / v rows at most 2^23 elements apart, row strides {(ldq, ldk, ldv, ldo)}")
+    ws = torch.empty(plan._workspace, dtype=torch.uint8, device=q.device) if plan._workspace else None
+    items, joins = plan._tables
+    _launch("mv_attention_packed", _pack_attention(pq, pk or pq, pv or pq, po, items, joins, ws.data_ptr() if ws is not None else 0,   # (no key: not read)
+                                                   plan._workspace, plan.ws_rows, plan.n_items, plan.n_few, plan.n_joins, ldq, ldk, ldv, ldo,
+                                                   plan.heads, plan.kv_heads, plan.d, _DTYPES[dtype], plan.causal, plan.scale), dev, (plan,))
     return out
 
 
@@ -253,8 +268,8 @@ class RotaryTable(_Held):
 
     def __init__(self, turns: torch.Tensor, axis: torch.Tensor, axes: int):
         self.pairs, self.axes = turns.numel(), axes
-        self.turns, self.axis = turns, axis
         self._hold(turns, axis)
+        self._turns, self._axis = turns.data_ptr(), axis.data_ptr()
 
 
 def rotary_table(sections: Sequence[int], theta: float = 10000.0, *, shared: bool = False, device: Union[str, torch.device] = "cuda") -> RotaryTable:
@@ -282,67 +297,66 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
     """Turns ``q`` [tokens, heads * d] and ``k`` [tokens, kv_heads * d] (or ``None``) by their tokens' ``positions`` [tokens, axes] (int32 or
     fp32) in one launch; ``pairing``: "adjacent" turns elements 2 p and 2 p + 1 of a head, "halves" p and p + pairs.  A head's elements
     behind the rotary part pass through.  ``out_q`` / ``out_k`` may be ``q`` / ``k`` themselves.  Returns (q, k) turned (k ``None`` if not given)."""
-    q = _matrix(q, "q")
-    heads, d = int(heads), int(d)
-    kv_heads = heads if kv_heads is None else int(kv_heads)
+    n, cols, ldq = _matrix(q, "q")
+    dtype, dev = q.dtype, q.get_device()
+    kv_heads = heads if kv_heads is None else kv_heads
     if pairing not in ("adjacent", "halves"):
         raise ValueError(f"rotary_axes: pairing {pairing!r} (adjacent, halves)")
-    n = q.shape[0]
-    if heads < 1 or kv_heads < 1 or d < 1 or q.shape[1] != heads * d:
-        raise ValueError(f"rotary_axes: q {tuple(q.shape)} for {heads} heads of {d}")
+    if heads < 1 or kv_heads < 1 or d < 1 or cols != heads * d:
+        raise ValueError(f"rotary_axes: q {(n, cols)} for {heads} heads of {d}")
     if 2 * table.pairs > d:
         raise ValueError(f"rotary_axes: the table turns {2 * table.pairs} elements, a head has {d}")
+    pk = pok = ldk = ldok = 0
     if k is not None:
-        _matrix(k, "k", q.dtype, q.device)
-        if k.shape != (n, kv_heads * d):
-            raise ValueError(f"rotary_axes: k {tuple(k.shape)} for {n} tokens, {kv_heads} heads of {d}")
+        rows, cols, ldk = _matrix(k, "k", dtype, dev)
+        if rows != n or cols != kv_heads * d:
+            raise ValueError(f"rotary_axes: k {(rows, cols)} for {n} tokens, {kv_heads} heads of {d}")
+        pk = k.data_ptr()
     elif out_k is not None:
         raise ValueError("rotary_axes: out_k without k")
     if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.float32):
         raise ValueError("rotary_axes: positions must be an int32 or fp32 tensor")
-    _matrix(positions, "positions", positions.dtype, q.device)
-    if positions.shape != (n, table.axes):
-        raise ValueError(f"rotary_axes: positions {tuple(positions.shape)} for {n} tokens of {table.axes} axes")
-    if table.device != q.device:
+    rows, cols, ldp = _matrix(positions, "positions", positions.dtype, dev)
+    if rows != n or cols != table.axes:
+        raise ValueError(f"rotary_axes: positions {(rows, cols)} for {n} tokens of {table.axes} axes")
+    if table._dev != dev:
         raise ValueError(f"rotary_axes: table on {table.device}, tensors on {q.device}")
-    outs = []
-    for nm, t, o in (("q", q, out_q), ("k", k, out_k)):
-        if t is None:
-            outs.append(None)
-            continue
-        if o is None:
-            o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        else:
-            _matrix(o, f"out_{nm}", q.dtype, q.device)
-            if o.shape != t.shape:
-                raise ValueError(f"rotary_axes: out_{nm} {tuple(o.shape)}, {nm} {tuple(t.shape)}")
-            _no_overlap(o, f"rotary_axes: out_{nm}", (("q", q), ("k", k), ("positions", positions)), (nm,))
-        outs.append(o)
-    oq, ok = outs
-    if ok is not None and out_q is not None and out_k is not None:
-        _no_overlap(oq, "rotary_axes: out_q", (("out_k", ok),))
-    ds = RotaryDesc()
-    ds.q, ds.out_q, ds.ldq, ds.ldoq = q.data_ptr(), oq.data_ptr(), _ld(q), _ld(oq)
+    if out_q is None:
+        oq, ldoq = q.new_empty((n, heads * d)), heads * d
+    else:
+        oq, ldoq = out_q, _rotary_out("q", q, out_q, (("q", q), ("k", k), ("positions", positions)), dtype, dev)
+    ok = None
     if k is not None:
-        ds.k, ds.out_k, ds.ldk, ds.ldok = k.data_ptr(), ok.data_ptr(), _ld(k), _ld(ok)
-    ds.positions, ds.ldp, ds.positions_f32 = positions.data_ptr(), _ld(positions), int(positions.dtype == torch.float32)
-    ds.turns, ds.axis, ds.pairs, ds.axes = table.turns.data_ptr(), table.axis.data_ptr(), table.pairs, table.axes
-    ds.tokens, ds.heads, ds.kv_heads, ds.d, ds.halves, ds.dtype = n, heads, kv_heads, d, int(pairing == "halves"), _DTYPES[q.dtype]
-    with _device_of(q.device) as stream:
-        table._use(stream)
-        check(_lib.load().mv_rotary_axes(C.byref(ds), stream), "mv_rotary_axes")
+        if out_k is None:
+            ok, ldok = q.new_empty((n, kv_heads * d)), kv_heads * d
+        else:
+            ok, ldok = out_k, _rotary_out("k", k, out_k, (("q", q), ("k", k), ("positions", positions)), dtype, dev)
+            if out_q is not None:
+                _no_overlap(oq, "rotary_axes: out_q", (("out_k", ok),))
+        pok = ok.data_ptr()
+    _launch("mv_rotary_axes", _pack_rotary(q.data_ptr(), pk, oq.data_ptr(), pok, positions.data_ptr(), table._turns, table._axis, n, ldq, ldk, ldoq, ldok,
+                                           ldp, heads, kv_heads, d, table.pairs, table.axes, pairing == "halves", positions.dtype == torch.float32,
+                                           _DTYPES[dtype]), dev, (table,))
     return oq, ok
+
+
+def _rotary_out(nm: str, t: torch.Tensor, o: torch.Tensor, ins, dtype: torch.dtype, dev: int) -> int:
+    _, _, ld = _matrix(o, f"out_{nm}", dtype, dev)
+    if o.shape != t.shape:
+        raise ValueError(f"rotary_axes: out_{nm} {tuple(o.shape)}, {nm} {tuple(t.shape)}")
+    _no_overlap(o, f"rotary_axes: out_{nm}", ins, (nm,))
+    return ld
 
 
 # ---- gated residual norm ----------------------------------------------------------------------------------------------------------
 Affine = Tuple[Optional[torch.Tensor], Optional[torch.Tensor], float]   # (gamma, beta, eps)
 
 
-def _affine(t: Optional[torch.Tensor], name: str, c: int, like: torch.Tensor) -> Optional[int]:
+def _affine(t: Optional[torch.Tensor], name: str, c: int, dtype: torch.dtype, dev: int) -> int:
     if t is None:
-        return None
-    if t.dtype != like.dtype or t.device != like.device or not t.is_contiguous() or t.numel() != c:
-        raise ValueError(f"{name}: expected a contiguous {like.dtype} tensor of {c} elements on {like.device}")
+        return 0
+    if t.dtype != dtype or t.get_device() != dev or not t.is_contiguous() or t.numel() != c:
+        raise ValueError(f"{name}: expected a contiguous {dtype} tensor of {c} elements on device {dev}")
     return t.data_ptr()
 
 
@@ -358,73 +372,76 @@ def gated_residual_norm(x: torch.Tensor, f: torch.Tensor, *, kind: str = "layer"
     N: ``kind`` "rms" or "layer"; a gamma or beta may be ``None``.  ``gate`` / ``scale`` / ``shift``: [groups, C] matrices, g the row's group --
     ``group_index`` (int32 per row: packed sequences) or row // ``rows_per_group``; with one group neither is needed.  A row whose
     group_index is no group is filled with NaN.  Returns (s, h), h ``None`` without ``pre``.  ``out`` may be ``x`` or ``f`` itself, ``norm_out`` too."""
-    x = _matrix(x, "x")
-    rows, c = x.shape
-    _matrix(f, "f", x.dtype, x.device)
-    if f.shape != x.shape:
-        raise ValueError(f"gated_residual_norm: x {tuple(x.shape)}, f {tuple(f.shape)}")
+    rows, c, ldx = _matrix(x, "x")
+    dtype, dev = x.dtype, x.get_device()
+    frows, fc, ldf = _matrix(f, "f", dtype, dev)
+    if frows != rows or fc != c:
+        raise ValueError(f"gated_residual_norm: x {(rows, c)}, f {(frows, fc)}")
     if kind not in ("rms", "layer"):
         raise ValueError(f"gated_residual_norm: kind {kind!r} (rms, layer)")
     if not 1 <= c <= 16384:
         raise ValueError(f"gated_residual_norm: {c} columns (1 .. 16384)")
     if pre is None and (scale is not None or shift is not None or norm_out is not None):
         raise ValueError("gated_residual_norm: scale / shift / norm_out belong to the norm in front of the next block (pre)")
-    ds = GatedNormDesc()
-    groups = None
+    groups, mods = 0, []
     for nm, t in (("gate", gate), ("scale", scale), ("shift", shift)):
         if t is None:
+            mods.append((0, 0))
             continue
-        _matrix(t, nm, x.dtype, x.device)
-        if t.shape[1] != c or t.shape[0] < 1 or (groups is not None and t.shape[0] != groups):
-            raise ValueError(f"gated_residual_norm: {nm} {tuple(t.shape)} for {c} columns" + (f" and {groups} groups" if groups else ""))
-        groups = t.shape[0]
-    if rows_per_group is not None and group_index is not None:
-        raise ValueError("gated_residual_norm: rows_per_group or group_index, not both")
+        grows, gc, ld = _matrix(t, nm, dtype, dev)
+        if gc != c or grows < 1 or (groups and grows != groups):
+            raise ValueError(f"gated_residual_norm: {nm} {(grows, gc)} for {c} columns" + (f" and {groups} groups" if groups else ""))
+        groups = grows
+        mods.append((t.data_ptr(), ld))
+    index = per = 0
     if group_index is not None:
-        if groups is None:
+        if rows_per_group is not None:
+            raise ValueError("gated_residual_norm: rows_per_group or group_index, not both")
+        if not groups:
             raise ValueError("gated_residual_norm: group_index without gate, scale or shift")
-        if group_index.dtype != torch.int32 or group_index.shape != (rows,) or not group_index.is_contiguous() or group_index.device != x.device:
+        if group_index.dtype != torch.int32 or group_index.shape != (rows,) or not group_index.is_contiguous() or group_index.get_device() != dev:
             raise ValueError(f"gated_residual_norm: group_index must be contiguous int32 [{rows}] on {x.device}")
-        ds.group_index = group_index.data_ptr()
+        index = group_index.data_ptr()
     elif rows_per_group is not None:
-        rows_per_group = int(rows_per_group)
-        if groups is None or rows_per_group < 1 or groups * rows_per_group < rows:
-            raise ValueError(f"gated_residual_norm: {groups} groups of {rows_per_group} rows do not cover {rows}")
-        ds.rows_per_group = min(rows_per_group, _I32_MAX)
-    elif groups is not None and groups > 1:
+        per = int(rows_per_group)
+        if not groups or per < 1 or groups * per < rows:
+            raise ValueError(f"gated_residual_norm: {groups} groups of {per} rows do not cover {rows}")
+        per = min(per, _I32_MAX)
+    elif groups > 1:
         raise ValueError(f"gated_residual_norm: {groups} groups need rows_per_group or group_index")
-    ins = (("x", x), ("f", f), ("gate", gate), ("scale", scale), ("shift", shift), ("group_index", group_index))
+    given = out is not None or norm_out is not None
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out, lds = x.new_empty((rows, c)), c
     else:
-        _matrix(out, "out", x.dtype, x.device)
+        lds = _matrix(out, "out", dtype, dev)[2]
         if out.shape != x.shape:
-            raise ValueError(f"gated_residual_norm: out {tuple(out.shape)}, x {tuple(x.shape)}")
-        _no_overlap(out, "gated_residual_norm: out", ins, ("x", "f"))
+            raise ValueError(f"gated_residual_norm: out {tuple(out.shape)}, x {(rows, c)}")
+    pre_gamma = pre_beta = ldh = ph = 0
+    pre_eps = 0.0
     if pre is not None:
+        pre_gamma, pre_beta, pre_eps = _affine(pre[0], "pre gamma", c, dtype, dev), _affine(pre[1], "pre beta", c, dtype, dev), pre[2]
         if norm_out is None:
-            norm_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            norm_out, ldh = x.new_empty((rows, c)), c
         else:
-            _matrix(norm_out, "norm_out", x.dtype, x.device)
+            ldh = _matrix(norm_out, "norm_out", dtype, dev)[2]
             if norm_out.shape != x.shape:
-                raise ValueError(f"gated_residual_norm: norm_out {tuple(norm_out.shape)}, x {tuple(x.shape)}")
-            _no_overlap(norm_out, "gated_residual_norm: norm_out", ins, ("x", "f"))
-        _no_overlap(norm_out, "gated_residual_norm: norm_out", (("out", out),))
-        ds.pre_gamma, ds.pre_beta, ds.pre_eps = _affine(pre[0], "pre gamma", c, x), _affine(pre[1], "pre beta", c, x), float(pre[2])
-        ds.norm_out, ds.ldh = norm_out.data_ptr(), _ld(norm_out)
+                raise ValueError(f"gated_residual_norm: norm_out {tuple(norm_out.shape)}, x {(rows, c)}")
+        ph = norm_out.data_ptr()
+    post_gamma = post_beta = 0
+    post_eps = 0.0
     if post is not None:
-        ds.post, ds.post_eps = 1, float(post[2])
-        ds.post_gamma, ds.post_beta = _affine(post[0], "post gamma", c, x), _affine(post[1], "post beta", c, x)
-    ds.x, ds.f, ds.stream_out = x.data_ptr(), f.data_ptr(), out.data_ptr()
-    ds.ldx, ds.ldf, ds.lds = _ld(x), _ld(f), _ld(out)
-    for nm, t, ld in (("gate", gate, "ldg"), ("scale", scale, "ldsc"), ("shift", shift, "ldsh")):
-        if t is not None:
-            setattr(ds, nm, t.data_ptr())
-            setattr(ds, ld, _ld(t))
-    ds.rows, ds.groups, ds.c = rows, groups or 1, c
-    ds.layer, ds.dtype, ds.alpha = int(kind == "layer"), _DTYPES[x.dtype], float(alpha)
-    with _device_of(x.device) as stream:
-        check(_lib.load().mv_gated_residual_norm(C.byref(ds), stream), "mv_gated_residual_norm")
+        post_gamma, post_beta, post_eps = _affine(post[0], "post gamma", c, dtype, dev), _affine(post[1], "post beta", c, dtype, dev), post[2]
+    if given:
+        ins = (("x", x), ("f", f), ("gate", gate), ("scale", scale), ("shift", shift), ("group_index", group_index)) + tuple(
+            (nm, t) for nm, a in (("post", post), ("pre", pre)) if a is not None for t in a[:2])
+        _no_overlap(out, "gated_residual_norm: out", ins, ("x", "f"))
+        if norm_out is not None:
+            _no_overlap(norm_out, "gated_residual_norm: norm_out", ins, ("x", "f"))
+            _no_overlap(norm_out, "gated_residual_norm: norm_out", (("out", out),))
+    (pg, ldg), (psc, ldsc), (psh, ldsh) = mods
+    _launch("mv_gated_residual_norm", _pack_norm(x.data_ptr(), f.data_ptr(), out.data_ptr(), ph, post_gamma, post_beta, pre_gamma, pre_beta, pg, psc, psh,
+                                                 index, rows, groups or 1, per, c, ldx, ldf, lds, ldh, ldg, ldsc, ldsh, post is not None, kind == "layer",
+                                                 _DTYPES[dtype], alpha, post_eps, pre_eps), dev)
     return out, norm_out
 
 
@@ -433,8 +450,12 @@ class Int8Rows(_Held):
     """int8 rows with one scale each: row m stands for ``codes[m, :k] * scale[m]``.  ``codes`` is padded with zeros to a multiple of 128 columns."""
 
     def __init__(self, codes: torch.Tensor, scale: torch.Tensor, k: int):
-        self.codes, self.scale, self.k, self.rows = codes, scale, k, codes.shape[0]
+        if codes.dtype != torch.int8 or codes.ndim != 2 or not codes.is_contiguous() or codes.shape[1] != -(-k // 128) * 128 or \
+                scale.dtype != torch.float32 or scale.shape != codes.shape[:1] or not scale.is_contiguous() or scale.device != codes.device:
+            raise ValueError(f"Int8Rows: codes must be contiguous int8 [rows, {k} rounded up to 128] and scale contiguous fp32 [rows] beside them")
+        self.codes, self.scale, self.k, self.rows, self.kp = codes, scale, k, codes.shape[0], codes.shape[1]
         self._hold(codes, scale)
+        self._codes, self._scale = codes.data_ptr(), scale.data_ptr()
 
 
 def pack_weight_i8(codes: torch.Tensor, scale: torch.Tensor) -> Int8Rows:
@@ -453,46 +474,48 @@ def pack_weight_i8(codes: torch.Tensor, scale: torch.Tensor) -> Int8Rows:
 def quantize_rows_i8(x: torch.Tensor) -> Int8Rows:
     """Each row of ``x`` [M, K] (fp16 | bf16) as int8 codes and one scale: scale = max|x| / 127, code = 127 x / max|x| rounded to nearest, ties
     to even.  A row of zeros has scale 0; a row that holds an infinity or NaN keeps that as its scale (its products are NaN)."""
-    x = _matrix(x, "x")
-    m, k = x.shape
+    m, k, ld = _matrix(x, "x")
     if not 1 <= k <= 131072:
         raise ValueError(f"quantize_rows_i8: {k} columns (1 .. 131072)")
-    codes = torch.empty((m, -(-k // 128) * 128), dtype=torch.int8, device=x.device)
+    kp = -(-k // 128) * 128
+    codes = torch.empty((m, kp), dtype=torch.int8, device=x.device)
     scale = torch.empty((m,), dtype=torch.float32, device=x.device)
-    with _device_of(x.device) as stream:
-        check(_lib.load().mv_quantize_rows_i8(x.data_ptr(), _ld(x), m, k, _DTYPES[x.dtype], codes.data_ptr(), codes.shape[1], scale.data_ptr(), stream),
+    dev = x.get_device()
+    with torch.cuda.device(dev):
+        check(_lib.load().mv_quantize_rows_i8(x.data_ptr(), ld, m, k, _DTYPES[x.dtype], codes.data_ptr(), kp, scale.data_ptr(), _raw_stream(dev)),
               "mv_quantize_rows_i8")
     return Int8Rows(codes, scale, k)
 
 
-def _i8_checks(what: str, m: int, w: Int8Rows, device, dtype, bias, residual, act, out):
+def _i8_result(what: str, m: int, w: Int8Rows, like: torch.Tensor, dtype, bias, residual, act, out):
+    """checks what the product is finished with; (bias, residual, out pointers, row strides of residual and out, out)"""
+    dev, n = like.get_device(), w.rows
     if dtype not in _DTYPES:
         raise ValueError(f"{what}: dtype {dtype} (fp16, bf16)")
     if act not in (MV_ACT_NONE, MV_ACT_SILU):
         raise ValueError(f"{what}: activation {act}")
-    if w.device != device:
-        raise ValueError(f"{what}: weight on {w.device}, rows on {device}")
-    n = w.rows
+    if w._dev != dev:
+        raise ValueError(f"{what}: weight on {w.device}, rows on {like.device}")
     if n < 1:
         raise ValueError(f"{what}: a weight without rows")
-    ds = GemmI8Desc()
+    pb = pr = ldr = 0
     if bias is not None:
-        if bias.dtype != dtype or bias.device != device or not bias.is_contiguous() or bias.numel() != n:
-            raise ValueError(f"{what}: bias must be a contiguous {dtype} tensor of {n} elements on {device}")
-        ds.bias = bias.data_ptr()
+        if bias.dtype != dtype or bias.get_device() != dev or not bias.is_contiguous() or bias.numel() != n:
+            raise ValueError(f"{what}: bias must be a contiguous {dtype} tensor of {n} elements on {like.device}")
+        pb = bias.data_ptr()
     if residual is not None:
-        _matrix(residual, "residual", dtype, device)
-        if residual.shape != (m, n):
-            raise ValueError(f"{what}: residual {tuple(residual.shape)}, the product is {(m, n)}")
-        ds.residual, ds.ldr = residual.data_ptr(), _ld(residual)
-    if out is not None:
-        _matrix(out, "out", dtype, device)
-        if out.shape != (m, n):
-            raise ValueError(f"{what}: out {tuple(out.shape)}, the product is {(m, n)}")
+        rows, cols, ldr = _matrix(residual, "residual", dtype, dev)
+        if rows != m or cols != n:
+            raise ValueError(f"{what}: residual {(rows, cols)}, the product is {(m, n)}")
+        pr = residual.data_ptr()
+    if out is None:
+        out, ldo = torch.empty((m, n), dtype=dtype, device=like.device), n
+    else:
+        rows, cols, ldo = _matrix(out, "out", dtype, dev)
+        if rows != m or cols != n:
+            raise ValueError(f"{what}: out {(rows, cols)}, the product is {(m, n)}")
         _no_overlap(out, f"{what}: out", (("residual", residual), ("bias", bias)), ("residual",))
-    ds.M, ds.N, ds.kp, ds.ldw = m, n, w.codes.shape[1], w.codes.shape[1]
-    ds.w, ds.w_scale, ds.act, ds.dtype = w.codes.data_ptr(), w.scale.data_ptr(), int(act), _DTYPES[dtype]
-    return ds
+    return pb, pr, out.data_ptr(), ldr, ldo, out
 
 
 def gemm_i8(a: Int8Rows, w: Int8Rows, *, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None, act: int = MV_ACT_NONE,
@@ -501,23 +524,24 @@ def gemm_i8(a: Int8Rows, w: Int8Rows, *, bias: Optional[torch.Tensor] = None, re
     ``out`` may be ``residual`` itself."""
     if a.k != w.k:
         raise ValueError(f"gemm_i8: rows of {a.k}, weight of {w.k}")
-    ds = _i8_checks("gemm_i8", a.rows, w, a.device, dtype, bias, residual, act, out)
-    if out is None:
-        out = torch.empty((a.rows, w.rows), dtype=dtype, device=a.device)
-    ds.a, ds.a_scale, ds.lda, ds.out, ds.ldo = a.codes.data_ptr(), a.scale.data_ptr(), a.codes.shape[1], out.data_ptr(), _ld(out)
-    with _device_of(a.device) as stream:
-        a._use(stream)
-        w._use(stream)
-        check(_lib.load().mv_gemm_i8(C.byref(ds), stream), "mv_gemm_i8")
+    pb, pr, po, ldr, ldo, out = _i8_result("gemm_i8", a.rows, w, a.codes, dtype, bias, residual, act, out)
+    _launch("mv_gemm_i8", _pack_gemm(a._codes, w._codes, a._scale, w._scale, pb, pr, po, a.rows, w.rows, w.kp, a.kp, w.kp, ldr, ldo, act, _DTYPES[dtype]),
+            a._dev, (a, w))
     return out
 
 
 def linear_i8(x: torch.Tensor, w: Int8Rows, *, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None, act: int = MV_ACT_NONE,
               out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """:func:`gemm_i8` of :func:`quantize_rows_i8` (``x``): a projection whose weight and activations are multiplied in 8 bits."""
-    x = _matrix(x, "x")
-    if x.shape[1] != w.k:
-        raise ValueError(f"linear_i8: x {tuple(x.shape)}, weight of {w.k}")
-    if out is not None and isinstance(out, torch.Tensor) and out.dim() == 2:
+    """:func:`gemm_i8` of :func:`quantize_rows_i8` (``x``) in one call: a projection whose weight and activations are multiplied in 8 bits."""
+    m, k, ldx = _matrix(x, "x")
+    dtype = x.dtype
+    if k != w.k:
+        raise ValueError(f"linear_i8: x {(m, k)}, weight of {w.k}")
+    given = out is not None
+    pb, pr, po, ldr, ldo, out = _i8_result("linear_i8", m, w, x, dtype, bias, residual, act, out)
+    if given:
         _no_overlap(out, "linear_i8: out", (("x", x),))
-    return gemm_i8(quantize_rows_i8(x), w, bias=bias, residual=residual, act=act, dtype=x.dtype, out=out)
+    ws = torch.empty(m * (w.kp + 4), dtype=torch.uint8, device=x.device)   # mv_linear_i8: the rows' codes, then their scales
+    _launch("mv_linear_i8", _pack_linear(x.data_ptr(), w._codes, w._scale, pb, pr, po, ws.data_ptr(), m, w.rows, k, w.kp, ldx, w.kp, ldr, ldo, act,
+                                         _DTYPES[dtype]), x.get_device(), (w,))
+    return out

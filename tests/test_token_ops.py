@@ -67,7 +67,7 @@ def test_entry_points_refuse_without_a_gpu():
 
     def refused(rc, text):
         assert rc == -1 and text in lib.mv_last_error(), (rc, lib.mv_last_error())
-    for fn in (lib.mv_attention_packed, lib.mv_rotary_axes, lib.mv_gated_residual_norm, lib.mv_gemm_i8):
+    for fn in (lib.mv_attention_packed, lib.mv_rotary_axes, lib.mv_gated_residual_norm, lib.mv_gemm_i8, lib.mv_linear_i8):
         refused(fn(None, None), b"null descriptor")
     a = _lib.AttnPackedDesc()
     a.q = a.k = a.v = a.out = a.items = 16
@@ -106,6 +106,14 @@ def test_entry_points_refuse_without_a_gpu():
         setattr(g, name, bad)
         refused(lib.mv_gemm_i8(C.byref(g), None), text)
         setattr(g, name, old)
+    ln = _lib.LinearI8Desc()
+    ln.x = ln.w = ln.w_scale = ln.out = ln.workspace = 16
+    ln.M, ln.N, ln.K, ln.kp, ln.ldx, ln.ldw, ln.ldo = 4, 8, 100, 128, 100, 128, 8
+    for name, bad, text in (("kp", 256, b"kp"), ("K", 0, b"K 0"), ("workspace", 0, b"workspace"), ("x", 0, b"null")):
+        old = getattr(ln, name)
+        setattr(ln, name, bad)
+        refused(lib.mv_linear_i8(C.byref(ln), None), text)
+        setattr(ln, name, old)
     refused(lib.mv_quantize_rows_i8(16, 64, 4, 64, 0, 16, 64, 16, None), b"code rows")
     refused(lib.mv_quantize_rows_i8(16, 64, 4, 0, 0, 16, 128, 16, None), b"131072")
 
@@ -159,7 +167,7 @@ def test_plan_covers_every_visible_key_once(seed):
         kvh, group = r.choice([1, 2, 8]), r.choice([1, 3, 4, 8])
         plan = to.attention_plan(ql, kl, heads=kvh * group, kv_heads=kvh, d=64, causal=causal, device="cpu")
         items, joins = (t.tolist() for t in plan._tensors)
-        d = plan._desc
+        d = plan
         assert len(items) == d.n_items + d.n_few and len(joins) == d.n_joins
         _cover(items[:d.n_items], items[d.n_items:], joins, d.ws_rows, ql, kl, group, causal)
         from musev_amd import _lib
@@ -207,16 +215,8 @@ def on_cpu(monkeypatch):
         raise Launched
     monkeypatch.setattr(to._lib, "load", load)
 
-    class Here:
-        def __init__(self, dev):
-            pass
-
-        def __enter__(self):
-            return 0
-
-        def __exit__(self, *a):
-            pass
-    monkeypatch.setattr(to, "_device_of", Here)
+    monkeypatch.setattr(to, "_current_device", lambda: -1)    # (what get_device() says of a CPU tensor)
+    monkeypatch.setattr(to, "_raw_stream", lambda dev: 0)
     monkeypatch.setattr(to._Held, "_use", lambda self, s: None)
     return Launched
 
@@ -290,6 +290,9 @@ def test_refusals_of_the_int8_projection(on_cpu):
             ops.gemm_i8(a, w, **kw)
     with pytest.raises(ValueError, match="rows of"):
         ops.gemm_i8(ops.Int8Rows(a.codes, a.scale, 41), w)
+    for codes, scale, k in ((a.codes, a.scale, 129), (a.codes[:, :64], a.scale, 40), (a.codes, a.scale[:5], 40), (a.codes.int(), a.scale, 40)):
+        with pytest.raises(ValueError, match="Int8Rows"):
+            ops.Int8Rows(codes, scale, k)
     x = torch.zeros(6, 40, dtype=torch.float16)
     with pytest.raises(ValueError, match="weight of"):
         ops.linear_i8(x[:, :39], w)
