@@ -25,7 +25,7 @@ int mv_tokens_abi_version(void);
  *   out[i] = sum_j softmax_j(scale * q_i . k_j) v_j   over the keys j < kv_len of i's sequence, with `causal` only
  *   j <= i + kv_len - q_len (the last query sees every key);  a row that sees no key is 0.
  * A (sequence, key / value head) has q_len * group packed rows: row r is query r / group, head r % group of the group.
- * `items` (device, 8 int32 each), made by musev_amd.token_ops.attention_plan: n_items of 128 packed rows, then n_few of 32:
+ * `items` (device, 8 int32 each), made by musev_amd.token_ops.attention_plan, 128 packed rows each:
  *   {first query row, q_len, first key row, kv_len, first packed row, key begin, key end, first workspace row or -1}
  * An item with a workspace row writes its unnormalised sums and the rows' references / sums there; `joins` (device, 8 int32 each:
  *   {first query row, q_len, kv_len, first packed row, first workspace row, parts, rows per part, 0}) says which parts make up which rows.
@@ -36,7 +36,7 @@ typedef struct mv_attn_packed_desc {
     const int32_t *items, *joins;
     void* workspace;               /* with joins: mv_attention_packed_workspace_bytes(ws_rows, kv_heads, d) bytes, 16-byte aligned */
     int64_t workspace_bytes, ws_rows;
-    int32_t n_items, n_few, n_joins;
+    int32_t n_items, n_joins, join_rows;   /* join_rows: the most rows of a join */
     int32_t ldq, ldk, ldv, ldo;
     int32_t heads, kv_heads, d, dtype, causal;
     float scale;

@@ -146,7 +146,7 @@ class AttnPackedDesc(C.Structure):
     _fields_ = [
         ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("out", C.c_void_p), ("items", C.c_void_p), ("joins", C.c_void_p),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("ws_rows", C.c_int64),
-        ("n_items", C.c_int32), ("n_few", C.c_int32), ("n_joins", C.c_int32),
+        ("n_items", C.c_int32), ("n_joins", C.c_int32), ("join_rows", C.c_int32),
         ("ldq", C.c_int32), ("ldk", C.c_int32), ("ldv", C.c_int32), ("ldo", C.c_int32),
         ("heads", C.c_int32), ("kv_heads", C.c_int32), ("d", C.c_int32), ("dtype", C.c_int32), ("causal", C.c_int32),
         ("scale", C.c_float),

@@ -10,10 +10,9 @@
 // K and V tiles go global -> LDS directly (16 bytes per lane).  LDS rows are 128 or 256 bytes; the 16-byte slots of a row are permuted by
 // an XOR with row bits, applied to the source column each lane fetches, so that both the 16-byte reads of K (16 rows, one column) and the
 // transposing reads of V (4 rows x 64 bytes per half wave) touch every bank once.
-// Two forms of one kernel:
-//   wide (FEW = false): 4 waves x 32 packed rows share 64-key tiles, two stages, one barrier per tile; two blocks per CU
-//   few rows (FEW = true): 32 packed rows (a token of a group of heads); the 4 waves walk different 32-key tiles of their own and are joined
-//                  at the end: what counts here is the number of bytes in flight
+// 4 waves x 32 packed rows share 64-key tiles, two stages, one barrier per tile, two blocks per CU: 64 KB on its way per CU, enough to stream the
+// cache of a single token too, where one wave alone has rows (a form whose 4 waves walked tiles of their own for up to 32 rows was no faster:
+// 16 requests over 86 k keys 82 against 77 us).
 #include "tok_common.h"
 
 extern "C" int mv_tokens_abi_version(void) { return MV_TOKENS_ABI_VERSION; }
@@ -32,17 +31,14 @@ template <typename T> struct ExpBits;   // both elements of a dword: exponent ma
 template <> struct ExpBits<half_t> { static constexpr unsigned mask = 0x7c007c00u, one = 0x04000400u; };
 template <> struct ExpBits<bf16_t> { static constexpr unsigned mask = 0x7f807f80u, one = 0x00800080u; };
 
-template <int DC, bool FEW>
+template <int DC>
 struct PackedCfg {
     static constexpr int RS = DC <= 64 ? 64 : 128;     // elements per LDS row
     static constexpr int SLOTS = RS / 8;               // 16-byte slots per LDS row
-    static constexpr int KT = FEW ? 32 : 64;           // keys per tile
+    static constexpr int KT = 64;                      // keys per tile
     static constexpr int TILE = KT * RS;               // elements of a K (or V) tile
-    static constexpr int PIECES = TILE * 2 / 1024;     // 1-KiB pieces of a tile
-    static constexpr int PPW = FEW ? PIECES : PIECES / 4;   // ... that one wave fetches, of K and of V each
-    static constexpr int RINGS = FEW ? 4 : 1;          // few rows: a ring per wave
-    static constexpr int RING = 2 * 2 * TILE;          // elements of a ring: two stages of K, V
-    static constexpr int LDS_BYTES = RINGS * RING * 2;
+    static constexpr int PPW = TILE * 2 / 1024 / 4;    // 1-KiB pieces of it that one wave fetches
+    static constexpr int LDS_BYTES = 2 * 2 * TILE * 2; // two stages of K, V
     static constexpr int NS = KT / 32, NB = DC / 32;   // 32-key score blocks of a tile, 32-column blocks of the output
 };
 
@@ -51,18 +47,18 @@ struct PackedCfg {
 template <int RS> __device__ __forceinline__ int swz_k(int row) { return RS == 128 ? (row & 15) : ((row >> 1) & 7); }
 template <int RS> __device__ __forceinline__ int swz_v(int row) { return RS == 128 ? ((row & 3) << 2) : (((row >> 1) & 1) << 2); }
 
-template <typename T, int DC, bool FEW>
-__global__ __launch_bounds__(256, FEW ? 1 : 2) void attention_packed_kernel(const mv_attn_packed_desc p, const int item0) {
-    using C = PackedCfg<DC, FEW>;
+template <typename T, int DC>
+__global__ __launch_bounds__(256, 2) void attention_packed_kernel(const mv_attn_packed_desc p) {
+    using C = PackedCfg<DC>;
     typedef typename Vec8<T>::type V8;
     typedef __attribute__((address_space(3))) T lds_t;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const PackedItem it = ((const PackedItem*)p.items)[item0 + blockIdx.x / p.kv_heads];
+    const PackedItem it = ((const PackedItem*)p.items)[blockIdx.x / p.kv_heads];
     const int kvh = blockIdx.x % p.kv_heads, group = p.heads / p.kv_heads;
     const int rows = it.q_len * group;
-    const int row0 = it.m0 + (FEW ? 0 : wave * 32);
+    const int row0 = it.m0 + wave * 32;
     const bool active = row0 < rows;                       // (wave-uniform) the last tile's waves may have no row
     const int r = min(row0 + l31, rows - 1);               // this lane's packed row (padding lanes repeat the last one)
     const int qi = r / group, hq = kvh * group + (r - qi * group);
@@ -92,11 +88,11 @@ __global__ __launch_bounds__(256, FEW ? 1 : 2) void attention_packed_kernel(cons
     float m = -1.0e30f, l = 0.f;    // reference of the exponents (score units; m * c stays finite), sum of this lane's own keys
 
     // ---- global -> LDS ----
-    lds_t* ring = (lds_t*)((__attribute__((address_space(3))) char*)smem) + (FEW ? wave * C::RING : 0);
+    lds_t* ring = (lds_t*)((__attribute__((address_space(3))) char*)smem);
     unsigned ok[C::PPW], ov[C::PPW];   // byte offset of this lane's 16 bytes from the tile's first row; columns past d: out of range, read as 0
 #pragma unroll
     for (int j = 0; j < C::PPW; ++j) {
-        const int at = ((FEW ? 0 : wave * C::PPW) + j) * 64 + lane;
+        const int at = (wave * C::PPW + j) * 64 + lane;
         const int row = at / C::SLOTS, slot = at % C::SLOTS;
         const int sk = slot ^ swz_k<C::RS>(row), sv = slot ^ swz_v<C::RS>(row);
         ok[j] = sk * 8 < p.d ? (unsigned)((row * p.ldk + sk * 8) * 2) : 0x80000000u;
@@ -110,7 +106,7 @@ __global__ __launch_bounds__(256, FEW ? 1 : 2) void attention_packed_kernel(cons
         const int left = min(it.kv_len - key, C::KT);
         const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)(kbase + (int64_t)key * p.ldk * 2), 0, (unsigned)(((left - 1) * p.ldk + p.d) * 2), 0x00020000);
         const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)(vbase + (int64_t)key * p.ldv * 2), 0, (unsigned)(((left - 1) * p.ldv + p.d) * 2), 0x00020000);
-        lds_t* dst = ring + stage * 2 * C::TILE + (FEW ? 0 : wave * C::PPW * 512);
+        lds_t* dst = ring + stage * 2 * C::TILE + wave * C::PPW * 512;
 #pragma unroll
         for (int j = 0; j < C::PPW; ++j)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (__attribute__((address_space(3))) void*)(dst + j * 512), 16, (int)ok[j], 0, 0, 0);
@@ -233,154 +229,106 @@ __global__ __launch_bounds__(256, FEW ? 1 : 2) void attention_packed_kernel(cons
     };
 
     const int tiles = (it.key_end - it.key_begin + C::KT - 1) / C::KT;
-    if constexpr (!FEW) {
-        if (tiles > 0) issue(it.key_begin, 0);
+    if (tiles > 0) issue(it.key_begin, 0);
 #pragma unroll 1
-        for (int t = 0; t < tiles; ++t) {
-            const int key = it.key_begin + t * C::KT;
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // this wave's share of tile t has landed ...
-            __builtin_amdgcn_s_barrier();                        // ... and everyone's; everyone has left tile t - 1 and its stage
-            asm volatile("" ::: "memory");
-            if (t + 1 < tiles) issue(key + C::KT, (t + 1) & 1);
-            if (active && key < lim_hi) compute(key, t & 1);
-        }
-    } else {
-        // tiles wave, wave + 4, ...: this wave's own ring, no barrier
-        if (wave < tiles) issue(it.key_begin + wave * C::KT, 0);
-        if (wave + 4 < tiles) issue(it.key_begin + (wave + 4) * C::KT, 1);
-        int stage = 0;
-#pragma unroll 1
-        for (int t = wave; t < tiles; t += 4) {
-            if (t + 4 < tiles) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * C::PPW) : "memory");
-            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            compute(it.key_begin + t * C::KT, stage);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the stage's reads are done before it is filled again
-            if (t + 8 < tiles) issue(it.key_begin + (t + 8) * C::KT, stage);
-            stage ^= 1;
-        }
+    for (int t = 0; t < tiles; ++t) {
+        const int key = it.key_begin + t * C::KT;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // this wave's share of tile t has landed ...
+        __builtin_amdgcn_s_barrier();                        // ... and everyone's; everyone has left tile t - 1 and its stage
+        asm volatile("" ::: "memory");
+        if (t + 1 < tiles) issue(key + C::KT, (t + 1) & 1);
+        if (active && key < lim_hi) compute(key, t & 1);
     }
     l += __shfl_xor(l, 32, 64);
 
-    if constexpr (FEW) {
-        // ---- the four waves' parts, joined through LDS: [wave][row][DC + 4] unnormalised sums, then [wave][row] references and sums ----
-        constexpr int PR = DC + 4;
-        float* part = (float*)smem;
-        float* ml = part + 4 * 32 * PR;
-        static_assert((4 * 32 * PR + 4 * 32 * 2) * 4 <= C::LDS_BYTES, "the joined parts fit the rings");
-        __syncthreads();
-#pragma unroll
-        for (int b = 0; b < C::NB; ++b)
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-                *(float4v*)(part + (wave * 32 + l31) * PR + 32 * b + 8 * g + 4 * h) = float4v{acc[b][4 * g], acc[b][4 * g + 1], acc[b][4 * g + 2], acc[b][4 * g + 3]};
-        if (h == 0) {
-            ml[(wave * 32 + l31) * 2] = m;
-            ml[(wave * 32 + l31) * 2 + 1] = l;
-        }
-        __syncthreads();
-        const int n = min(32, rows - it.m0), quads = p.d / 4;
-        for (int x = tid; x < n * quads; x += 256) {
-            const int q = x / quads, col = (x - q * quads) * 4;
-            float mm = ml[q * 2];
-#pragma unroll
-            for (int w = 1; w < 4; ++w) mm = fmaxf(mm, ml[(w * 32 + q) * 2]);
-            float ll = 0.f;
-            float4v o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float a = __builtin_amdgcn_exp2f((ml[(w * 32 + q) * 2] - mm) * c), lw = ml[(w * 32 + q) * 2 + 1];
-                ll += a * lw;
-                // a wave that saw no key of the row has a sum of 0 and adds nothing
-                if (lw != 0.f) o += *(const float4v*)(part + (w * 32 + q) * PR + col) * a;
-            }
-            const int rr = it.m0 + q, i = rr / group, head = kvh * group + (rr - i * group);
-            if (it.ws_row >= 0) {
-                float* ws = (float*)p.workspace;
-                const int64_t at = (int64_t)kvh * p.ws_rows + it.ws_row + q;
-                *(float4v*)(ws + at * p.d + col) = o;
-                if (col == 0) {
-                    float* wml = ws + (int64_t)p.kv_heads * p.ws_rows * p.d + at * 2;
-                    wml[0] = mm * c;
-                    wml[1] = ll;
-                }
-            } else {
-                const int see = p.causal ? i + it.kv_len - it.q_len + 1 : it.kv_len;
-                const float inv = 1.0f / ll;
-                T* out = (T*)p.out + (int64_t)(it.q_row + i) * p.ldo + (int64_t)head * p.d + col;
-                T w4[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w4[e] = see > 0 ? (T)(o[e] * inv) : (T)0.f;
-                *(uint2*)out = *(const uint2*)w4;
-            }
-        }
-    } else {
-        if (row0 + l31 >= rows) return;
-        if (it.ws_row >= 0) {
-            float* ws = (float*)p.workspace;
-            const int64_t at = (int64_t)kvh * p.ws_rows + it.ws_row + wave * 32 + l31;
-#pragma unroll
-            for (int b = 0; b < C::NB; ++b)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int col = 32 * b + 8 * g + 4 * h;
-                    if (col < p.d) *(float4v*)(ws + at * p.d + col) = float4v{acc[b][4 * g], acc[b][4 * g + 1], acc[b][4 * g + 2], acc[b][4 * g + 3]};
-                }
-            if (h == 0) {
-                float* wml = ws + (int64_t)p.kv_heads * p.ws_rows * p.d + at * 2;
-                wml[0] = m * c;
-                wml[1] = l;
-            }
-            return;
-        }
-        const float inv = 1.0f / l;
-        T* out = (T*)p.out + (int64_t)(it.q_row + qi) * p.ldo + (int64_t)hq * p.d;
+    if (row0 + l31 >= rows) return;
+    if (it.ws_row >= 0) {
+        float* ws = (float*)p.workspace;
+        const int64_t at = (int64_t)kvh * p.ws_rows + it.ws_row + wave * 32 + l31;
 #pragma unroll
         for (int b = 0; b < C::NB; ++b)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int col = 32 * b + 8 * g + 4 * h;
-                if (col >= p.d) continue;
-                T w4[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w4[e] = seen > 0 ? (T)(acc[b][4 * g + e] * inv) : (T)0.f;
-                *(uint2*)(out + col) = *(const uint2*)w4;
+                if (col < p.d) *(float4v*)(ws + at * p.d + col) = float4v{acc[b][4 * g], acc[b][4 * g + 1], acc[b][4 * g + 2], acc[b][4 * g + 3]};
             }
+        if (h == 0) {
+            float* wml = ws + (int64_t)p.kv_heads * p.ws_rows * p.d + at * 2;
+            wml[0] = m * c;
+            wml[1] = l;
+        }
+        return;
     }
+    const float inv = 1.0f / l;
+    T* out = (T*)p.out + (int64_t)(it.q_row + qi) * p.ldo + (int64_t)hq * p.d;
+#pragma unroll
+    for (int b = 0; b < C::NB; ++b)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int col = 32 * b + 8 * g + 4 * h;
+            if (col >= p.d) continue;
+            T w4[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w4[e] = seen > 0 ? (T)(acc[b][4 * g + e] * inv) : (T)0.f;
+            *(uint2*)(out + col) = *(const uint2*)w4;
+        }
 }
 
-// joins the parts of rows whose keys were split over several items; one wave per packed row
-template <typename T>
+// Joins the parts of rows whose keys were split over several items.  WPR waves per packed row take its parts in turn, four loads of each on their
+// way at once: the parts were just written by other XCDs, and what the join of a few rows costs is those loads' latency (one token of 8 k keys, 8
+// key / value heads: 13.8 us with four waves per row, 21.9 with one).  With many rows the other rows hide it and one wave per row is right (a
+// prompt of 1024, 16 heads: 21 against 31 us).
+template <typename T, int WPR>
 __global__ __launch_bounds__(256) void attention_join_kernel(const mv_attn_packed_desc p) {
-    const int blocks = 128 / 4;   // (a join has at most 128 rows, a block 4)
-    const PackedJoin jn = ((const PackedJoin*)p.joins)[blockIdx.x / (p.kv_heads * blocks)];
-    const int kvh = (blockIdx.x / blocks) % p.kv_heads, group = p.heads / p.kv_heads;
-    const int row = (blockIdx.x % blocks) * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int rr = jn.m0 + row;
-    if (row >= jn.rows || rr >= jn.q_len * group) return;
-    const int i = rr / group, head = kvh * group + (rr - i * group);
+    __shared__ float2v other[3][64];
+    const int lane = threadIdx.x & 63, wave = WPR == 1 ? 0 : threadIdx.x >> 6, group = p.heads / p.kv_heads;
+    const int at_row = WPR == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    const int join = at_row / (p.kv_heads * p.join_rows), rest = at_row - join * (p.kv_heads * p.join_rows);
+    if (join >= p.n_joins) return;
+    const int kvh = rest / p.join_rows, row = rest - kvh * p.join_rows;
+    const PackedJoin jn = ((const PackedJoin*)p.joins)[join];
+    if (row >= jn.rows) return;   // (joins differ in their rows; with WPR = 4 the whole block)
+    const int rr = jn.m0 + row, i = rr / group, head = kvh * group + (rr - i * group);
     const float* ws = (const float*)p.workspace;
     const int64_t at = (int64_t)kvh * p.ws_rows + jn.ws_row + row;
     const float* ml = ws + (int64_t)p.kv_heads * p.ws_rows * p.d;
-    float mm = -3.0e38f;
-    for (int s = 0; s < jn.parts; ++s) mm = fmaxf(mm, ml[(at + (int64_t)s * jn.rows) * 2]);
-    float ll = 0.f, o0 = 0.f, o1 = 0.f;
-    const int col = lane * 2;
-    for (int s = 0; s < jn.parts; ++s) {
-        const int64_t r = at + (int64_t)s * jn.rows;
-        const float lw = ml[r * 2 + 1], a = __builtin_amdgcn_exp2f(ml[r * 2] - mm);
-        if (lw == 0.f) continue;   // no key of this part was seen
-        ll += a * lw;
-        if (col < p.d) {
-            const float2v w = *(const float2v*)(ws + r * p.d + col);
-            o0 = __builtin_fmaf(a, w.x, o0);
-            o1 = __builtin_fmaf(a, w.y, o1);
+    const int col = min(lane * 2, p.d - 2);
+    float mm = -3.0e38f, ll = 0.f, o0 = 0.f, o1 = 0.f;
+    for (int s0 = 0; s0 < jn.parts; s0 += 64) {
+        const int n = min(64, jn.parts - s0);
+        float2v w = {-3.0e38f, 0.f};   // lane s: part s's reference and sum
+        if (lane < n) w = *(const float2v*)(ml + (at + (int64_t)(s0 + lane) * jn.rows) * 2);
+        const float mn = fmaxf(mm, wave_max(w.x)), old = __builtin_amdgcn_exp2f(mm - mn);
+        const float a = w.y != 0.f ? __builtin_amdgcn_exp2f(w.x - mn) : 0.f;   // (a part that saw no key adds nothing)
+        mm = mn;
+        ll = ll * old + wave_sum(a * w.y);
+        o0 *= old;
+        o1 *= old;
+        for (int s = wave; s < n; s += 4 * WPR) {
+            float2v v[4];
+            float as[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int sx = min(s + WPR * x, n - 1);
+                v[x] = *(const float2v*)(ws + (at + (int64_t)(s0 + sx) * jn.rows) * p.d + col);
+                as[x] = s + WPR * x < n ? __shfl(a, sx, 64) : 0.f;
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                if (as[x] != 0.f) o0 = __builtin_fmaf(as[x], v[x].x, o0), o1 = __builtin_fmaf(as[x], v[x].y, o1);
         }
     }
-    const int see = p.causal ? i + jn.kv_len - jn.q_len + 1 : jn.kv_len;
-    if (col < p.d) {
-        T w2[2] = {see > 0 ? (T)(o0 / ll) : (T)0.f, see > 0 ? (T)(o1 / ll) : (T)0.f};
-        *(unsigned*)((T*)p.out + (int64_t)(jn.q_row + i) * p.ldo + (int64_t)head * p.d + col) = *(const unsigned*)w2;
+    if constexpr (WPR > 1) {
+        if (wave > 0) other[wave - 1][lane] = float2v{o0, o1};
+        __syncthreads();
+        if (wave > 0) return;
+#pragma unroll
+        for (int x = 0; x < 3; ++x) o0 += other[x][lane].x, o1 += other[x][lane].y;
     }
+    if (lane * 2 >= p.d) return;
+    const int see = p.causal ? i + jn.kv_len - jn.q_len + 1 : jn.kv_len;
+    T w2[2] = {see > 0 ? (T)(o0 / ll) : (T)0.f, see > 0 ? (T)(o1 / ll) : (T)0.f};
+    *(unsigned*)((T*)p.out + (int64_t)(jn.q_row + i) * p.ldo + (int64_t)head * p.d + col) = *(const unsigned*)w2;
 }
 
 extern "C" int64_t mv_attention_packed_workspace_bytes(int64_t ws_rows, int32_t kv_heads, int32_t d) {
@@ -388,36 +336,26 @@ extern "C" int64_t mv_attention_packed_workspace_bytes(int64_t ws_rows, int32_t 
     return ws_rows * kv_heads * (d + 2) * 4;
 }
 
-template <typename T, int DC, bool FEW>
-static int launch_packed(const mv_attn_packed_desc* d, int item0, int n, hipStream_t st) {
-    using C = PackedCfg<DC, FEW>;
-    const auto kernel = attention_packed_kernel<T, DC, FEW>;
-    if (C::LDS_BYTES > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS_BYTES);
-        if (e != hipSuccess) {
-            mv_set_error("mv_attention_packed: %s", hipGetErrorString(e));
-            return MV_ERR_LAUNCH;
-        }
-    }
-    kernel<<<(unsigned)(n * d->kv_heads), 256, C::LDS_BYTES, st>>>(*d, item0);
+constexpr int64_t JOIN_FEW = 2048;   // packed rows up to which four waves join a row: two blocks of them per SIMD of the chip
+
+template <typename T, int DC>
+static int launch_packed(const mv_attn_packed_desc* d, hipStream_t st) {
+    static_assert(PackedCfg<DC>::LDS_BYTES <= 64 * 1024, "dynamic LDS without an attribute");
+    attention_packed_kernel<T, DC><<<(unsigned)(d->n_items * d->kv_heads), 256, PackedCfg<DC>::LDS_BYTES, st>>>(*d);
     MV_CHECK_LAUNCH("mv_attention_packed");
+    if (d->n_joins > 0) {
+        const int64_t rows = (int64_t)d->n_joins * d->kv_heads * d->join_rows;
+        if (rows <= JOIN_FEW) attention_join_kernel<T, 4><<<(unsigned)rows, 256, 0, st>>>(*d);
+        else attention_join_kernel<T, 1><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(*d);
+        MV_CHECK_LAUNCH("mv_attention_packed (join)");
+    }
     return MV_OK;
 }
 
+// head dims up to 64, 96 and 128: the columns a tile is multiplied over
 template <typename T>
-static int launch_all(const mv_attn_packed_desc* d, hipStream_t st) {
-    int rc = MV_OK;
-    if (d->n_items > 0)
-        rc = d->d <= 64 ? launch_packed<T, 64, false>(d, 0, d->n_items, st)
-           : d->d <= 96 ? launch_packed<T, 96, false>(d, 0, d->n_items, st) : launch_packed<T, 128, false>(d, 0, d->n_items, st);
-    if (rc == MV_OK && d->n_few > 0)
-        rc = d->d <= 64 ? launch_packed<T, 64, true>(d, d->n_items, d->n_few, st)
-           : d->d <= 96 ? launch_packed<T, 96, true>(d, d->n_items, d->n_few, st) : launch_packed<T, 128, true>(d, d->n_items, d->n_few, st);
-    if (rc == MV_OK && d->n_joins > 0) {
-        attention_join_kernel<T><<<(unsigned)(d->n_joins * d->kv_heads * 32), 256, 0, st>>>(*d);
-        MV_CHECK_LAUNCH("mv_attention_packed (join)");
-    }
-    return rc;
+static int launch_head_dim(const mv_attn_packed_desc* d, hipStream_t st) {
+    return d->d <= 64 ? launch_packed<T, 64>(d, st) : d->d <= 96 ? launch_packed<T, 96>(d, st) : launch_packed<T, 128>(d, st);
 }
 
 extern "C" int mv_attention_packed(const mv_attn_packed_desc* d, void* stream) {
@@ -427,9 +365,10 @@ extern "C" int mv_attention_packed(const mv_attn_packed_desc* d, void* stream) {
     MV_REQUIRE(d->kv_heads >= 1 && d->heads >= d->kv_heads && d->heads % d->kv_heads == 0, "mv_attention_packed: %d heads over %d key / value heads",
                d->heads, d->kv_heads);
     MV_REQUIRE(d->scale >= -1e6f && d->scale <= 1e6f, "mv_attention_packed: scale %g (at most 1e6 in size)", (double)d->scale);
-    MV_REQUIRE(d->n_items >= 0 && d->n_few >= 0 && d->n_joins >= 0 && ((int64_t)d->n_items + d->n_few) * d->kv_heads < (1ll << 31) &&
-               (int64_t)d->n_joins * d->kv_heads * 32 < (1ll << 31), "mv_attention_packed: %d + %d items, %d joins", d->n_items, d->n_few, d->n_joins);
-    if (d->n_items + d->n_few == 0) return MV_OK;
+    MV_REQUIRE(d->n_items >= 0 && d->n_joins >= 0 && (int64_t)d->n_items * d->kv_heads < (1ll << 31) && d->join_rows >= 0 && d->join_rows <= 128 &&
+               (int64_t)d->n_joins * d->kv_heads * 128 < (1ll << 31), "mv_attention_packed: %d items, %d joins of up to %d rows", d->n_items, d->n_joins,
+               d->join_rows);
+    if (d->n_items == 0) return MV_OK;
     MV_REQUIRE(d->q && d->k && d->v && d->out && d->items, "mv_attention_packed: null pointer");
     MV_REQUIRE((((uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v | (uintptr_t)d->out) & 15) == 0 && ((d->ldq | d->ldk | d->ldv | d->ldo) & 7) == 0,
                "mv_attention_packed: rows must be 16-byte aligned");
@@ -437,5 +376,5 @@ extern "C" int mv_attention_packed(const mv_attn_packed_desc* d, void* stream) {
     MV_REQUIRE(d->n_joins == 0 || (d->joins && d->workspace && ((uintptr_t)d->workspace & 15) == 0 &&
                d->workspace_bytes >= mv_attention_packed_workspace_bytes(d->ws_rows, d->kv_heads, d->d)),
                "mv_attention_packed: the workspace is missing, unaligned or too small");
-    return d->dtype == MV_F16 ? launch_all<half_t>(d, (hipStream_t)stream) : launch_all<bf16_t>(d, (hipStream_t)stream);
+    return d->dtype == MV_F16 ? launch_head_dim<half_t>(d, (hipStream_t)stream) : launch_head_dim<bf16_t>(d, (hipStream_t)stream);
 }

@@ -135,11 +135,11 @@ class _Held:
 class AttentionPlan(_Held):
     """the work list of :func:`attention_packed` for one set of sequence lengths (:func:`attention_plan`)"""
 
-    def __init__(self, q_lens, kv_lens, heads, kv_heads, d, causal, scale, n_items, n_few, items, joins, ws_rows):
+    def __init__(self, q_lens, kv_lens, heads, kv_heads, d, causal, scale, items, joins, join_rows, ws_rows):
         self.q_lens, self.kv_lens = tuple(q_lens), tuple(kv_lens)
         self.heads, self.kv_heads, self.d, self.causal, self.scale = heads, kv_heads, d, causal, scale
         self.total_q, self.total_kv = sum(q_lens), sum(kv_lens)
-        self.n_items, self.n_few, self.n_joins, self.ws_rows = n_items, n_few, joins.shape[0], ws_rows
+        self.n_items, self.n_joins, self.join_rows, self.ws_rows = items.shape[0], joins.shape[0], join_rows, ws_rows
         self._hold(items, joins)
         self._tables = items.data_ptr(), joins.data_ptr()
         self._workspace = 4 * ws_rows * kv_heads * (d + 2)   # mv_attention_packed_workspace_bytes
@@ -156,44 +156,39 @@ def _lens(v, name: str) -> List[int]:
     return v
 
 
-WIDE_ROWS, FEW_ROWS = 128, 32   # packed rows per item of the two kernel forms
+TILE_ROWS = 128   # packed rows per item
 # Keys of an item that is worth a split: an item's parts each write and the join reads back (d + 2) fp32 per row.
-MIN_PART_WIDE, MIN_PART_FEW = 512, 256
-BLOCKS = 512                    # two blocks on each of the 256 CUs
+MIN_PART = 128
+BLOCKS = 512      # two blocks on each of the 256 CUs
 
 
 def _plan_items(ql: Sequence[int], kl: Sequence[int], group: int, kv_heads: int, causal: bool):
-    """(wide items, few-row items, joins, workspace rows): see include/musev_tokens.h.  A sequence of at most FEW_ROWS packed rows makes one
-    few-row item.  An item's keys end with what its last query sees.  Where the items alone would leave CUs idle, or one item would outlast
-    the others, its keys are split into parts of about 1 / BLOCKS of all the work; the longest items come first."""
-    tiles, q_row, k_row = ([], []), 0, 0
+    """(items, joins, workspace rows): see include/musev_tokens.h.  An item's keys end with what its last query sees.  Where the items alone would
+    leave CUs idle, or one item would outlast the others, its keys are split into parts of about 1 / BLOCKS of all the work; the longest items
+    come first."""
+    tiles, q_row, k_row = [], 0, 0
     for q, kv in zip(ql, kl):
-        rows = q * group
-        few = rows <= FEW_ROWS
-        for m0 in range(0, rows, FEW_ROWS if few else WIDE_ROWS):
-            last = min(m0 + (FEW_ROWS if few else WIDE_ROWS), rows) - 1
-            end = max(0, min(kv, last // group + kv - q + 1)) if causal else kv
-            tiles[few].append((q_row, q, k_row, kv, m0, end))
+        for m0 in range(0, q * group, TILE_ROWS):
+            last = min(m0 + TILE_ROWS, q * group) - 1
+            tiles.append((q_row, q, k_row, kv, m0, max(0, min(kv, last // group + kv - q + 1)) if causal else kv))
         q_row, k_row = q_row + q, k_row + kv
-    out, joins, ws = ([], []), [], 0
-    for few in (False, True):
-        width, least = (FEW_ROWS, MIN_PART_FEW) if few else (WIDE_ROWS, MIN_PART_WIDE)
-        part = max(least, -(-sum(t[5] for t in tiles[few]) * kv_heads // BLOCKS))
-        part = -(-part // 64) * 64
-        for q_row, q, k_row, kv, m0, end in tiles[few]:
-            n = max(1, (end + part // 2) // part)
-            if n == 1:
-                out[few].append((q_row, q, k_row, kv, m0, 0, end, -1))
-                continue
-            size = -(-(-(-end // n)) // 64) * 64
-            n = -(-end // size)
-            rows = min(width, q * group - m0)
-            for s in range(n):
-                out[few].append((q_row, q, k_row, kv, m0, s * size, min(end, (s + 1) * size), ws + s * rows))
-            joins.append((q_row, q, kv, m0, ws, n, rows, 0))
-            ws += n * rows
-        out[few].sort(key=lambda i: i[5] - i[6])
-    return out[0], out[1], joins, ws
+    items, joins, ws = [], [], 0
+    part = max(MIN_PART, -(-sum(t[5] for t in tiles) * kv_heads // BLOCKS))
+    part = -(-part // 64) * 64
+    for q_row, q, k_row, kv, m0, end in tiles:
+        n = max(1, (end + part // 2) // part)
+        if n == 1:
+            items.append((q_row, q, k_row, kv, m0, 0, end, -1))
+            continue
+        size = -(-(-(-end // n)) // 64) * 64
+        n = -(-end // size)
+        rows = min(TILE_ROWS, q * group - m0)
+        for s in range(n):
+            items.append((q_row, q, k_row, kv, m0, s * size, min(end, (s + 1) * size), ws + s * rows))
+        joins.append((q_row, q, kv, m0, ws, n, rows, 0))
+        ws += n * rows
+    items.sort(key=lambda i: i[5] - i[6])
+    return items, joins, ws
 
 
 def attention_plan(q_lens: Sequence[int], kv_lens: Optional[Sequence[int]] = None, *, heads: int, kv_heads: Optional[int] = None, d: int,
@@ -219,11 +214,10 @@ def attention_plan(q_lens: Sequence[int], kv_lens: Optional[Sequence[int]] = Non
     dev = torch.device(device)
     if dev.type == "cuda" and dev.index is None:
         dev = torch.device("cuda", torch.cuda.current_device())
-    wide, few, joins, ws_rows = _plan_items(ql, kl, heads // kv_heads, kv_heads, bool(causal))
-    # one upload for both tables
-    table = torch.tensor((wide + few + joins) or [(0,) * 8], dtype=torch.int32).to(dev)
-    n = len(wide) + len(few)
-    return AttentionPlan(ql, kl, heads, kv_heads, d, bool(causal), scale, len(wide), len(few), table[:n], table[n:n + len(joins)], ws_rows)
+    items, joins, ws_rows = _plan_items(ql, kl, heads // kv_heads, kv_heads, bool(causal))
+    table = torch.tensor((items + joins) or [(0,) * 8], dtype=torch.int32).to(dev)   # (one upload)
+    n = len(items)
+    return AttentionPlan(ql, kl, heads, kv_heads, d, bool(causal), scale, table[:n], table[n:n + len(joins)], max((j[6] for j in joins), default=0), ws_rows)
 
 
 def attention_packed(plan: AttentionPlan, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -257,7 +251,7 @@ def attention_packed(plan: AttentionPlan, q: torch.Tensor, k: torch.Tensor, v: t
     ws = torch.empty(plan._workspace, dtype=torch.uint8, device=q.device) if plan._workspace else None
     items, joins = plan._tables
     _launch("mv_attention_packed", _pack_attention(pq, pk or pq, pv or pq, po, items, joins, ws.data_ptr() if ws is not None else 0,   # (no key: not read)
-                                                   plan._workspace, plan.ws_rows, plan.n_items, plan.n_few, plan.n_joins, ldq, ldk, ldv, ldo,
+                                                   plan._workspace, plan.ws_rows, plan.n_items, plan.n_joins, plan.join_rows, ldq, ldk, ldv, ldo,
                                                    plan.heads, plan.kv_heads, plan.d, _DTYPES[dtype], plan.causal, plan.scale), dev, (plan,))
     return out
 

@@ -118,16 +118,16 @@ def test_entry_points_refuse_without_a_gpu():
     refused(lib.mv_quantize_rows_i8(16, 64, 4, 0, 0, 16, 128, 16, None), b"131072")
 
 
-def _cover(wide, few, joins, ws_rows, ql, kl, group, causal):
+def _cover(items, joins, ws_rows, ql, kl, group, causal):
     """every packed row's every visible key is walked by exactly one item, the parts of a row are joined for exactly that row, and no two
     parts share workspace rows"""
     want, q_at, k_at = set(), 0, 0
     for q, kv in zip(ql, kl):
-        for m0 in range(0, q * group, 32 if q * group <= 32 else 128):
+        for m0 in range(0, q * group, 128):
             want.add((q_at, q, k_at, kv, m0))
         q_at, k_at = q_at + q, k_at + kv
     tiles = {}
-    for it in wide + few:
+    for it in items:
         tiles.setdefault(tuple(it[:5]), []).append(it)
     assert set(tiles) == want
     joined = {(j[0], j[1], j[2], j[3]): j for j in joins}
@@ -135,9 +135,7 @@ def _cover(wide, few, joins, ws_rows, ql, kl, group, causal):
     used = set()
     for key, items in tiles.items():
         q_row, q, k_row, kv, m0 = key
-        small = q * group <= 32
-        assert all((it in few) == small for it in items)
-        rows = min(32 if small else 128, q * group - m0)
+        rows = min(128, q * group - m0)
         last = (m0 + rows - 1) // group
         vis = kv if not causal else max(0, min(kv, last + kv - q + 1))
         items.sort(key=lambda i: i[5])
@@ -168,8 +166,8 @@ def test_plan_covers_every_visible_key_once(seed):
         plan = to.attention_plan(ql, kl, heads=kvh * group, kv_heads=kvh, d=64, causal=causal, device="cpu")
         items, joins = (t.tolist() for t in plan._tensors)
         d = plan
-        assert len(items) == d.n_items + d.n_few and len(joins) == d.n_joins
-        _cover(items[:d.n_items], items[d.n_items:], joins, d.ws_rows, ql, kl, group, causal)
+        assert len(items) == d.n_items and len(joins) == d.n_joins and d.join_rows == max((j[6] for j in joins), default=0)
+        _cover(items, joins, d.ws_rows, ql, kl, group, causal)
         from musev_amd import _lib
         assert plan._workspace == _lib.load().mv_attention_packed_workspace_bytes(d.ws_rows, kvh, 64)
 
