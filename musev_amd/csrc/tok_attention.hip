@@ -31,6 +31,8 @@ template <typename T> struct ExpBits;   // both elements of a dword: exponent ma
 template <> struct ExpBits<half_t> { static constexpr unsigned mask = 0x7c007c00u, one = 0x04000400u; };
 template <> struct ExpBits<bf16_t> { static constexpr unsigned mask = 0x7f807f80u, one = 0x00800080u; };
 
+template <bool B> struct Masked { static constexpr bool value = B; };
+
 template <int DC>
 struct PackedCfg {
     static constexpr int RS = DC <= 64 ? 64 : 128;     // elements per LDS row
@@ -64,7 +66,7 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(const mv_attn_
     const int qi = r / group, hq = kvh * group + (r - qi * group);
     const int seen = p.causal ? max(0, qi + it.kv_len - it.q_len + 1) : it.kv_len;
     const int lim = min(seen, it.key_end);                 // this row walks the keys [key_begin, lim)
-    const int lim_lo = __builtin_amdgcn_readlane(lim, 0), lim_hi = __builtin_amdgcn_readlane(lim, 31);
+    const int lim_hi = __builtin_amdgcn_readlane(lim, 31);
 
     // ---- Q (second operand of S^T): row in the lane, 8 columns per half wave and step; a negative scale turns its sign here ----
     const float c = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-30f);   // scores in powers of two
@@ -126,7 +128,8 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(const mv_attn_
         const int row = 4 * h + (i16 >> 2), slot = 4 * b + 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
         va[b] = row * C::RS + (slot ^ swz_v<C::RS>(row)) * 8 + (i16 & 1) * 4;
     }
-    auto compute = [&](int key, int stage) __attribute__((always_inline)) {
+    auto compute = [&](int key, int stage, auto tag) __attribute__((always_inline)) {
+        constexpr bool masked = decltype(tag)::value;   // some row may not see all of the tile
         const lds_t* sk = ring + stage * 2 * C::TILE;
         const lds_t* sv = sk + C::TILE;
         float16v s[C::NS];
@@ -143,8 +146,7 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(const mv_attn_
                 s[n] = mfma_32x32x16(kf, qf[k], s[n]);
             }
         __builtin_amdgcn_s_setprio(0);
-        const bool masked = key + C::KT > lim_lo;   // (wave-uniform) some row does not see all of the tile
-        if (masked) {
+        if constexpr (masked) {
             const int left = lim - key - 4 * h;
 #pragma unroll
             for (int n = 0; n < C::NS; ++n)
@@ -182,7 +184,7 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(const mv_attn_
                 pf[2 * n + (e >> 3)][e & 7] = (T)pe;   // P in the input type: half a step of it, relative, on each weight
             }
         l += t0 + t1;
-        if (masked) {
+        if constexpr (masked) {
             // a masked weight is 0, but 0 x infinity is not: where the tile's values are not all finite, the rows take their visible keys one
             // by one instead
             unsigned bad = 0;
@@ -228,17 +230,23 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(const mv_attn_
         __builtin_amdgcn_s_setprio(0);
     };
 
+    // The tiles that the item's first row sees whole -- all its rows do -- run without masks; at most (127 / group + 63) / 64 + 1 follow them.
     const int tiles = (it.key_end - it.key_begin + C::KT - 1) / C::KT;
-    if (tiles > 0) issue(it.key_begin, 0);
-#pragma unroll 1
-    for (int t = 0; t < tiles; ++t) {
+    const int first_lim = p.causal ? min(it.m0 / group + it.kv_len - it.q_len + 1, it.key_end) : it.key_end;
+    const int whole = max(0, first_lim - it.key_begin) / C::KT;
+    auto walk = [&](int t, auto tag) __attribute__((always_inline)) {
         const int key = it.key_begin + t * C::KT;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // this wave's share of tile t has landed ...
         __builtin_amdgcn_s_barrier();                        // ... and everyone's; everyone has left tile t - 1 and its stage
         asm volatile("" ::: "memory");
         if (t + 1 < tiles) issue(key + C::KT, (t + 1) & 1);
-        if (active && key < lim_hi) compute(key, t & 1);
-    }
+        if (active && (!decltype(tag)::value || key < lim_hi)) compute(key, t & 1, tag);
+    };
+    if (tiles > 0) issue(it.key_begin, 0);
+#pragma unroll 1
+    for (int t = 0; t < whole; ++t) walk(t, Masked<false>{});
+#pragma unroll 1
+    for (int t = whole; t < tiles; ++t) walk(t, Masked<true>{});
     l += __shfl_xor(l, 32, 64);
 
     if (row0 + l31 >= rows) return;
