@@ -15,9 +15,10 @@ template <> struct Vec8<bf16_t> { typedef bf16x8 type; };
 template <typename T> struct Loose8 {
     typedef unsigned short raw __attribute__((ext_vector_type(8)));
     struct __attribute__((packed, aligned(2))) bytes { raw v; };
+    typedef raw anywhere __attribute__((aligned(2)));
 };
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, int n, float* out) {
+__device__ __forceinline__ typename Vec8<T>::type load8_raw(const T* p, int n) {
     typedef typename Vec8<T>::type V;
     V v;
     if (n >= 8) v = __builtin_bit_cast(V, ((const typename Loose8<T>::bytes*)p)->v);
@@ -27,6 +28,11 @@ __device__ __forceinline__ void load8(const T* p, int n, float* out) {
         for (int e = 0; e < 7; ++e)
             if (e < n) v[e] = p[e];
     }
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int n, float* out) {
+    const typename Vec8<T>::type v = load8_raw(p, n);
 #pragma unroll
     for (int e = 0; e < 8; ++e) out[e] = (float)v[e];
 }
@@ -40,6 +46,33 @@ __device__ __forceinline__ void store8(T* p, int n, const float* in) {
     else
         for (int e = 0; e < 7; ++e)
             if (e < n) p[e] = v[e];
+}
+
+// the same for a result that the caches need not keep for this kernel (non-temporal: 13 312 x 1280 x 4 streams of the gated norm 130 -> 112 us)
+template <typename T>
+__device__ __forceinline__ void store8_stream(T* p, int n, const float* in) {
+    typedef typename Vec8<T>::type V;
+    if (n >= 8) {
+        V v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (T)in[e];
+        __builtin_nontemporal_store(__builtin_bit_cast(typename Loose8<T>::raw, v), (typename Loose8<T>::anywhere*)p);
+    } else store8(p, n, in);
+}
+
+// sum over a wave: within 16 lanes by cross-lane moves of the VALU, then two exchanges
+template <int CTRL>
+__device__ __forceinline__ float lane_move(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float wave_sum_fast(float v) {
+    v += lane_move<0xB1>(v);    // lanes 1 0 3 2 of a quad
+    v += lane_move<0x4E>(v);    // lanes 2 3 0 1
+    v += lane_move<0x141>(v);   // mirrored within 8
+    v += lane_move<0x140>(v);   // mirrored within 16
+    v += __shfl_xor(v, 16, 64);
+    v += __shfl_xor(v, 32, 64);
+    return v;
 }
 
 // calls body(T{}) with the element type of a descriptor

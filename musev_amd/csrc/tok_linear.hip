@@ -286,7 +286,9 @@ __global__ __launch_bounds__((GemmI8Cfg<BM, BN, WM, WN, BK, NST>::THREADS), 2) v
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] += r[e];
             }
-            store8((T*)p.out + m * p.ldo + n, left, v);
+            // (the small tile's results are small: the next kernel may find them in the caches)
+            if constexpr (BM > 64) store8_stream((T*)p.out + m * p.ldo + n, left, v);
+            else store8((T*)p.out + m * p.ldo + n, left, v);
         }
     }
 }

@@ -4,7 +4,7 @@
 // sums over a row held by WAVES waves
 template <int WAVES>
 __device__ __forceinline__ float row_sum(float v, float* red) {
-    v = wave_sum(v);
+    v = wave_sum_fast(v);
     if constexpr (WAVES > 1) {
         __syncthreads();   // (the previous sum's readers are through)
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
@@ -104,7 +104,7 @@ __global__ __launch_bounds__(256) void gated_norm_kernel(const mv_gated_norm_des
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) s[j][e] = col + e < c ? __builtin_fmaf(p.alpha, s[j][e], y[j][e]) : 0.f;
-        store8(so + col, c - col, s[j]);
+        store8_stream(so + col, c - col, s[j]);
     }
     if (!p.norm_out) return;
     statistics(s, p.pre_eps, mean, rstd);
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(256) void gated_norm_kernel(const mv_gated_norm_des
 #pragma unroll
             for (int e = 0; e < 8; ++e) s[j][e] += w[e];
         }
-        store8(ho + col, c - col, s[j]);
+        store8_stream(ho + col, c - col, s[j]);
     }
 }
 
