@@ -336,6 +336,74 @@ __global__ __launch_bounds__(512) void gemm_i8_few_kernel(const mv_gemm_i8_desc 
     }
 }
 
+// Quantisation and product in one launch, for so few activations that every block can quantise them for itself: M <= 16 rows and at most
+// ONE_LAUNCH codes.  All 512 threads read x (each keeps its elements in registers between the row's maximum and the codes), the codes go to LDS
+// and the weights stream as above, their first two units already on their way meanwhile.
+constexpr int ONE_LAUNCH = 16384;
+static bool one_launch(int64_t m, int64_t kp) { return m <= 16 && m * kp <= ONE_LAUNCH; }
+
+template <typename T>
+__global__ __launch_bounds__(512) void linear_i8_few_kernel(const mv_linear_i8_desc p) {
+    __shared__ int part[8][256];
+    __shared__ unsigned tops[16];
+    __shared__ __attribute__((aligned(16))) int8_t codes[ONE_LAUNCH + 16 * 16];   // rows kp + 16 bytes apart: 16 rows' fragments on different banks
+    const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n0 = blockIdx.x * 16, m_rows = (int)p.M, kp = (int)p.kp, stride = kp + 16;
+    const int8_t* w = p.w + (int64_t)min(n0 + l15, p.N - 1) * p.ldw + 32 * g;
+    int4v w0[2], w1[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int k = min((wave + 8 * u) * 128, kp - 128);
+        w0[u] = *(const int4v*)(w + k);
+        w1[u] = *(const int4v*)(w + k + 16);
+    }
+    if (tid < 16) tops[tid] = 0;
+    __syncthreads();
+    constexpr int NC = ONE_LAUNCH / 8 / 512;   // chunks of 8 codes per thread
+    const int per_row = kp / 8, total = m_rows * per_row;
+    float v[NC][8];
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+        const int ch = tid + 512 * j, m = ch / per_row, col = (ch - m * per_row) * 8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
+        if (ch < total && col < p.K) {
+            load8((const T*)p.x + m * p.ldx + col, p.K - col, v[j]);
+            unsigned top = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = max(top, abs_bits(v[j][e]));
+            atomicMax(&tops[m], top);   // (a maximum does not depend on the order)
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+        const int ch = tid + 512 * j, m = ch / per_row, col = (ch - m * per_row) * 8;
+        if (ch < total) *(uint2*)(codes + m * stride + col) = eight_codes(v[j], row_scale(tops[m]));
+    }
+    __syncthreads();
+    int4v acc = {0, 0, 0, 0};
+    const int8_t* a = codes + min(l15, m_rows - 1) * stride + 32 * g;
+    int u = 0;
+    for (int k = wave * 128; k < kp; k += 8 * 128, ++u) {
+        const int4v b0 = u == 0 ? w0[0] : u == 1 ? w0[1] : *(const int4v*)(w + k), b1 = u == 0 ? w1[0] : u == 1 ? w1[1] : *(const int4v*)(w + k + 16);
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(b0, *(const int4v*)(a + k), acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(b1, *(const int4v*)(a + k + 16), acc, 0, 0, 0);
+    }
+    *(int4v*)(&part[wave][l15 * 16 + 4 * g]) = acc;
+    __syncthreads();
+    const int m = tid >> 4, n = n0 + (tid & 15);
+    if (m >= m_rows || n >= p.N) return;
+    int sum = 0;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) sum += part[x][tid];
+    float r = __builtin_fmaf((float)sum * row_scale(tops[m]).scale, p.w_scale[n], p.bias ? (float)((const T*)p.bias)[n] : 0.f);
+    if (p.act == MV_ACT_SILU) r = mv_silu(r);
+    if (p.residual) r += (float)((const T*)p.residual)[m * p.ldr + n];
+    ((T*)p.out)[m * p.ldo + n] = (T)r;
+}
+
 template <typename T, int BM, int BN, int WM, int WN, int BK, int NST>
 static int launch_gemm_i8(const mv_gemm_i8_desc* d, hipStream_t st) {
     using C = GemmI8Cfg<BM, BN, WM, WN, BK, NST>;
@@ -391,6 +459,16 @@ extern "C" int mv_linear_i8(const mv_linear_i8_desc* d, void* stream) {
     MV_REQUIRE(d, "mv_linear_i8: null descriptor");
     MV_REQUIRE(d->M >= 0 && d->K >= 1 && d->kp >= d->K && d->kp < d->K + 128 && d->kp % 128 == 0, "mv_linear_i8: M %ld, K %d, kp %ld", (long)d->M, d->K, (long)d->kp);
     if (d->M == 0) return MV_OK;
+    if (one_launch(d->M, d->kp)) {
+        MV_REQUIRE(d->dtype == MV_F16 || d->dtype == MV_BF16, "mv_linear_i8: element type %d", d->dtype);
+        MV_REQUIRE(d->act == MV_ACT_NONE || d->act == MV_ACT_SILU, "mv_linear_i8: activation %d", d->act);
+        MV_REQUIRE(d->N >= 1 && d->ldw % 128 == 0 && d->ldw >= d->kp, "mv_linear_i8: N %d, ldw %ld for kp %ld", d->N, (long)d->ldw, (long)d->kp);
+        MV_REQUIRE(d->x && d->w && d->w_scale && d->out && ((uintptr_t)d->w & 15) == 0, "mv_linear_i8: null or unaligned pointer");
+        const unsigned grid = (d->N + 15) / 16;
+        MV_DISPATCH_TYPE(d->dtype, (linear_i8_few_kernel<T><<<grid, 512, 0, (hipStream_t)stream>>>(*d)));
+        MV_CHECK_LAUNCH("mv_linear_i8");
+        return MV_OK;
+    }
     MV_REQUIRE(d->workspace, "mv_linear_i8: null workspace");
     mv_gemm_i8_desc g;
     g.a = (const int8_t*)d->workspace;

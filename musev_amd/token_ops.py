@@ -535,7 +535,8 @@ def linear_i8(x: torch.Tensor, w: Int8Rows, *, bias: Optional[torch.Tensor] = No
     pb, pr, po, ldr, ldo, out = _i8_result("linear_i8", m, w, x, dtype, bias, residual, act, out)
     if given:
         _no_overlap(out, "linear_i8: out", (("x", x),))
-    ws = torch.empty(m * (w.kp + 4), dtype=torch.uint8, device=x.device)   # mv_linear_i8: the rows' codes, then their scales
-    _launch("mv_linear_i8", _pack_linear(x.data_ptr(), w._codes, w._scale, pb, pr, po, ws.data_ptr(), m, w.rows, k, w.kp, ldx, w.kp, ldr, ldo, act,
+    # mv_linear_i8's workspace: the rows' codes, then their scales; none where it quantises and multiplies in one launch
+    ws = None if m <= 16 and m * w.kp <= 16384 else torch.empty(m * (w.kp + 4), dtype=torch.uint8, device=x.device)
+    _launch("mv_linear_i8", _pack_linear(x.data_ptr(), w._codes, w._scale, pb, pr, po, ws.data_ptr() if ws is not None else 0, m, w.rows, k, w.kp, ldx, w.kp, ldr, ldo, act,
                                          _DTYPES[dtype]), x.get_device(), (w,))
     return out

@@ -109,11 +109,14 @@ def test_entry_points_refuse_without_a_gpu():
     ln = _lib.LinearI8Desc()
     ln.x = ln.w = ln.w_scale = ln.out = ln.workspace = 16
     ln.M, ln.N, ln.K, ln.kp, ln.ldx, ln.ldw, ln.ldo = 4, 8, 100, 128, 100, 128, 8
-    for name, bad, text in (("kp", 256, b"kp"), ("K", 0, b"K 0"), ("workspace", 0, b"workspace"), ("x", 0, b"null")):
+    for name, bad, text in (("kp", 256, b"kp"), ("K", 0, b"K 0"), ("x", 0, b"null"), ("w", 8, b"aligned"), ("act", 3, b"activation"), ("dtype", 2, b"element type"),
+                            ("ldw", 64, b"ldw"), ("N", 0, b"N 0")):
         old = getattr(ln, name)
         setattr(ln, name, bad)
         refused(lib.mv_linear_i8(C.byref(ln), None), text)
         setattr(ln, name, old)
+    ln.M, ln.workspace = 17, 0
+    refused(lib.mv_linear_i8(C.byref(ln), None), b"workspace")
     refused(lib.mv_quantize_rows_i8(16, 64, 4, 64, 0, 16, 64, 16, None), b"code rows")
     refused(lib.mv_quantize_rows_i8(16, 64, 4, 0, 0, 16, 128, 16, None), b"131072")
 
@@ -713,7 +716,7 @@ def linear_oracle(x, codes, w_scale, bias, residual, silu):
     return y, half_step(x.dtype) * y.abs() + 2.0 ** -19 * size + subnormal(x.dtype)
 
 
-LIN = [(1, 128, 128), (1, 1280, 5120), (1, 1000, 1111), (2, 64, 7), (3, 40, 1), (5, 5120, 640), (8, 129, 33), (16, 1280, 320), (17, 1280, 320), (31, 384, 257),
+LIN = [(1, 16384, 40), (1, 16385, 40), (3, 5000, 100), (8, 2048, 64), (8, 2049, 64), (16, 1024, 48), (16, 1025, 48), (1, 1, 1), (4, 3, 5), (1, 128, 128), (1, 1280, 5120), (1, 1000, 1111), (2, 64, 7), (3, 40, 1), (5, 5120, 640), (8, 129, 33), (16, 1280, 320), (17, 1280, 320), (31, 384, 257),
        (33, 256, 96), (64, 640, 640), (65, 1000, 255), (127, 128, 256), (128, 256, 128), (129, 320, 129), (255, 2560, 320), (300, 1152, 1000),
        (1001, 1000, 1111), (1000, 5120, 1280), (4100, 640, 512), (513, 16, 513), (2, 9000, 48)]
 
