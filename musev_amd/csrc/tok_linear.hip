@@ -121,26 +121,30 @@ typedef int int16v __attribute__((ext_vector_type(16)));
 // row).  LDS rows are BK bytes = SLOTS slots of 16; 256 / BK rows share a 256-byte line of banks, so the slots of a row are permuted by the
 // line's number and a fragment read (16 rows, one slot) touches every bank once.  The permutation is applied to the column each lane
 // fetches (global -> LDS directly).
-template <int BM, int BN, int WM, int WN, int BK, int NST>
+// KS groups of waves share a block's tile and take the steps of K in turn, each with stages of its own: where a product has fewer tiles than
+// there are CUs and a long K, the latency of its steps is what it costs.  The groups' sums meet in LDS.
+template <int BM, int BN, int WM, int WN, int BK, int NST, int KS>
 struct GemmI8Cfg {
-    static constexpr int WAVES = (BM / WM) * (BN / WN), THREADS = 64 * WAVES;
+    static constexpr int WAVES = (BM / WM) * (BN / WN), THREADS = 64 * WAVES * KS;
     static constexpr int SLOTS = BK / 16, PROWS = 1024 / BK;            // slots of a row; rows of a 1-KiB piece
     static constexpr int STAGE = (BM + BN) * BK;
     static constexpr int PA = BM / PROWS / WAVES, PW = BN / PROWS / WAVES;   // pieces a wave fetches of each tile
     static constexpr int SROW = WN + 4;                                 // ints per row of the result staging
-    static constexpr int LDS = NST * STAGE > WAVES * 32 * SROW * 4 ? NST * STAGE : WAVES * 32 * SROW * 4;
+    static constexpr int STAGING = WAVES * 32 * SROW * 4, SUMS = WM * WN * 4;   // bytes; of a wave's sums
+    static constexpr int AFTER = STAGING + (KS - 1) * WAVES * SUMS;
+    static constexpr int LDS = KS * NST * STAGE > AFTER ? KS * NST * STAGE : AFTER;
     static_assert(BM % (PROWS * WAVES) == 0 && BN % (PROWS * WAVES) == 0, "every wave fetches whole pieces");
     static __device__ __forceinline__ int swz(int row) { return (row / (256 / BK)) % SLOTS; }
 };
 
-template <typename T, int BM, int BN, int WM, int WN, int BK, int NST>
-__global__ __launch_bounds__((GemmI8Cfg<BM, BN, WM, WN, BK, NST>::THREADS), 2) void gemm_i8_kernel(const mv_gemm_i8_desc p, const int tiles_m, const int tiles_n) {
-    using C = GemmI8Cfg<BM, BN, WM, WN, BK, NST>;
+template <typename T, int BM, int BN, int WM, int WN, int BK, int NST, int KS>
+__global__ __launch_bounds__((GemmI8Cfg<BM, BN, WM, WN, BK, NST, KS>::THREADS), 2) void gemm_i8_kernel(const mv_gemm_i8_desc p, const int tiles_m, const int tiles_n) {
+    using C = GemmI8Cfg<BM, BN, WM, WN, BK, NST, KS>;
     typedef __attribute__((address_space(3))) char lds_c;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     lds_c* const lds = (lds_c*)smem;
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave_id = __builtin_amdgcn_readfirstlane(tid >> 6), kg = wave_id / C::WAVES, wave = wave_id - kg * C::WAVES;
     int tm, tn;
     mv_tile_order(mv_xcd_remap(blockIdx.x, gridDim.x), tiles_m, tiles_n, MV_TILE_GROUP, &tm, &tn);
     const int64_t m0 = (int64_t)tm * BM;
@@ -164,7 +168,7 @@ __global__ __launch_bounds__((GemmI8Cfg<BM, BN, WM, WN, BK, NST>::THREADS), 2) v
         ow[j] = (unsigned)(row * p.ldw + ((pslot ^ C::swz(row)) << 4));
     }
     auto issue = [&](int k, int stage) __attribute__((always_inline)) {
-        lds_c* dst = lds + stage * C::STAGE;
+        lds_c* dst = lds + (kg * NST + stage) * C::STAGE;
 #pragma unroll
         for (int j = 0; j < C::PA; ++j)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void*)(dst + (wave * C::PA + j) * 1024), 16, (int)oa[j], k, 0, 0);
@@ -199,31 +203,32 @@ __global__ __launch_bounds__((GemmI8Cfg<BM, BN, WM, WN, BK, NST>::THREADS), 2) v
     auto residual_at = [&](int x) __attribute__((always_inline)) {
         return (const V8*)((const T*)p.residual + min(m0 + wm + 32 * (x / PASSES) + (x % PASSES) * RPP + frow, p.M - 1) * p.ldr + min(n, p.N - 8));
     };
-    const bool early = p.residual && p.kp >= 2 * BK && ((p.N | p.ldr) & 7) == 0 && ((uintptr_t)p.residual & 15) == 0;
+    const bool early = p.residual && kg == 0 && p.kp > KS * BK && ((p.N | p.ldr) & 7) == 0 && ((uintptr_t)p.residual & 15) == 0;
 
-    const int steps = p.kp / BK;   // (kp is a multiple of 128: at least two steps of 64)
+    const int steps = p.kp / BK, turns = (steps + KS - 1) / KS;   // this group's steps: kg, kg + KS, ...; the first group has one every turn
     int into = 0, from = 0;
 #pragma unroll
     for (int s = 0; s < NST - 1; ++s)
-        if (s < steps) issue(s * BK, into++);
+        if (s * KS + kg < steps) issue((s * KS + kg) * BK, into++);
 #pragma unroll 1
-    for (int t = 0; t < steps; ++t) {
-        // this wave's share of step t has landed ... (younger steps may be on their way)
-        if (t + 1 == steps && early) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(FIRST) : "memory");   // (the residual's loads are the youngest)
-        else if (NST > 2 && t + NST - 2 < steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * (C::PA + C::PW)) : "memory");
+    for (int t = 0; t < turns; ++t) {
+        // this wave's share of the step has landed ... (younger steps may be on their way)
+        if (t + 1 == turns && early) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(FIRST) : "memory");   // (the residual's loads are the youngest)
+        else if (NST > 2 && (t + NST - 2) * KS + kg < steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * (C::PA + C::PW)) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();                      // ... and everyone's; everyone has left the stage of step t - 1
+        __builtin_amdgcn_s_barrier();                      // ... and everyone's; everyone has left the stage of the step before
         asm volatile("" ::: "memory");
-        if (t + NST - 1 < steps) issue((t + NST - 1) * BK, into);
-        if (t + 2 == steps && early) {
+        if ((t + NST - 1) * KS + kg < steps) issue(((t + NST - 1) * KS + kg) * BK, into);
+        if (t + 2 == turns && early) {
             asm volatile("" ::: "memory");   // (behind the last stage's loads)
 #pragma unroll
             for (int x = 0; x < FIRST; ++x) res[x] = *residual_at(x);
             asm volatile("" ::: "memory");
         }
         into = into + 1 == NST ? 0 : into + 1;
-        const lds_c* sa = lds + from * C::STAGE + wm * BK;
-        const lds_c* sw = lds + from * C::STAGE + BM * BK + wn * BK;
+        if (KS > 1 && t * KS + kg >= steps) break;   // (the last turn: this group has no step left, nor a barrier)
+        const lds_c* sa = lds + (kg * NST + from) * C::STAGE + wm * BK;
+        const lds_c* sw = lds + (kg * NST + from) * C::STAGE + BM * BK + wn * BK;
         from = from + 1 == NST ? 0 : from + 1;
 #pragma unroll
         for (int s = 0; s < BK / 32; ++s) {
@@ -242,7 +247,34 @@ __global__ __launch_bounds__((GemmI8Cfg<BM, BN, WM, WN, BK, NST>::THREADS), 2) v
 #pragma unroll
         for (int x = FIRST; x < NRES; ++x) res[x] = *residual_at(x);
     }
-    __syncthreads();   // the stages become the waves' result staging
+    __syncthreads();   // the stages become the groups' sums and the waves' result staging
+    if constexpr (KS > 1) {
+        int4v* sums = (int4v*)(smem + C::STAGING) + lane;   // [group - 1][wave][block][quad of registers][lane]
+        if (kg > 0) {
+            sums += ((kg - 1) * C::WAVES + wave) * (C::SUMS / 16);
+#pragma unroll
+            for (int i = 0; i < WM / 32; ++i)
+#pragma unroll
+                for (int j = 0; j < WN / 32; ++j)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        sums[((i * (WN / 32) + j) * 4 + g) * 64] = int4v{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+        }
+        __syncthreads();
+        if (kg > 0) return;
+#pragma unroll
+        for (int o = 0; o < KS - 1; ++o)
+#pragma unroll
+            for (int i = 0; i < WM / 32; ++i)
+#pragma unroll
+                for (int j = 0; j < WN / 32; ++j)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const int4v v = sums[(o * C::WAVES + wave) * (C::SUMS / 16) + ((i * (WN / 32) + j) * 4 + g) * 64];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[i][j][4 * g + e] += v[e];
+                    }
+    }
 
     // 32 rows at a time through this wave's own LDS, so that rows are read (residual) and written 16 bytes per lane
     float* st = (float*)smem + wave * 32 * C::SROW;
@@ -404,10 +436,10 @@ __global__ __launch_bounds__(512) void linear_i8_few_kernel(const mv_linear_i8_d
     ((T*)p.out)[m * p.ldo + n] = (T)r;
 }
 
-template <typename T, int BM, int BN, int WM, int WN, int BK, int NST>
+template <typename T, int BM, int BN, int WM, int WN, int BK, int NST, int KS>
 static int launch_gemm_i8(const mv_gemm_i8_desc* d, hipStream_t st) {
-    using C = GemmI8Cfg<BM, BN, WM, WN, BK, NST>;
-    const auto kernel = gemm_i8_kernel<T, BM, BN, WM, WN, BK, NST>;
+    using C = GemmI8Cfg<BM, BN, WM, WN, BK, NST, KS>;
+    const auto kernel = gemm_i8_kernel<T, BM, BN, WM, WN, BK, NST, KS>;
     const int64_t tm = (d->M + BM - 1) / BM, tn = (d->N + BN - 1) / BN;
     MV_REQUIRE(tm * tn < (1ll << 31), "mv_gemm_i8: %ld x %ld tiles", (long)tm, (long)tn);
     if (C::LDS > 64 * 1024) {
@@ -424,7 +456,9 @@ static int launch_gemm_i8(const mv_gemm_i8_desc* d, hipStream_t st) {
 
 template <typename T>
 static int launch_gemm_i8_shape(const mv_gemm_i8_desc* d, hipStream_t st) {
-    if (d->M <= 32) {
+    // Up to 32 rows of a short K: the weight stream (us, stream / 32 x 32 tiles: 16 x 1280 x 5120 4.5 / 5.0; 20 x 640 x 640 3.2 / 4.7; from K =
+    // 2048 on its waves' turns add up, 32 x 5120 x 5120 16.1 / 8.5).
+    if (d->M <= 32 && d->kp <= 2048) {
         const unsigned grid = (d->N + 15) / 16;
         if (d->M <= 16) gemm_i8_few_kernel<T, 1><<<grid, 512, 0, st>>>(*d);
         else gemm_i8_few_kernel<T, 2><<<grid, 512, 0, st>>>(*d);
@@ -432,12 +466,16 @@ static int launch_gemm_i8_shape(const mv_gemm_i8_desc* d, hipStream_t st) {
         return MV_OK;
     }
     // The largest tile that still gives every CU a few blocks: 256 x 256 (one block per CU) from four rounds on, 128 x 64 (three per CU) from two
-    // blocks per CU, 64 x 64 below.  Measured (us, 256 x 256 / 128 x 64 / 64 x 64): 8192^3 475 / 661 / -; 26 624 x 1280 x 5120 278 / 325 / 385;
-    // 4096 x 1280 x 2560 27.6 / 25.9 / 32.3; 2048 x 1280 x 1280 23.7 / 10.3 / 10.2; 512 x 1280 x 1280 23 / 8.6 / 6.4.
+    // blocks per CU, 64 x 64 below, where K is long and tiles are few in four groups, and 32 x 32 in four groups up to two per CU.
+    // Measured (us, M x K x N; 256 / 128 x 64 / 64 / 64 in groups / 32 in groups): 8192^3 475 / 661 / - / - / -; 26 624 x 1280 x 5120 270 / 312 /
+    // 385 / - / -; 4096 x 1280 x 2560 26.8 / 24.8 / 31.5 / - / -; 2048 x 1280 x 1280 22.5 / 10.5 / 10.2 / - / -; 512 x 5120 x 1280 - / 22.9 / 19.8 /
+    // 13.7 / 16.5; 512 x 1280 x 1280 - / 8.3 / 6.7 / 7.0 / 9.1; 300 x 5120 x 1280 - / 19.1 / 14.0 / 11.9 / 10.6; 64 x 1280 x 1280 - / 8.3 / 6.5 / 6.7 / 5.2.
     const auto tiles = [&](int64_t bm, int64_t bn) { return ((d->M + bm - 1) / bm) * ((d->N + bn - 1) / bn); };
-    if (tiles(256, 256) >= 1024) return launch_gemm_i8<T, 256, 256, 128, 64, 128, 2>(d, st);
-    if (tiles(128, 64) >= 512) return launch_gemm_i8<T, 128, 64, 64, 32, 128, 2>(d, st);
-    return launch_gemm_i8<T, 64, 64, 32, 32, 128, 2>(d, st);
+    if (tiles(256, 256) >= 1024) return launch_gemm_i8<T, 256, 256, 128, 64, 128, 2, 1>(d, st);
+    if (tiles(128, 64) >= 512) return launch_gemm_i8<T, 128, 64, 64, 32, 128, 2, 1>(d, st);
+    if (tiles(32, 32) <= 512) return launch_gemm_i8<T, 32, 32, 32, 32, 128, 2, 4>(d, st);
+    if (tiles(64, 64) <= 256 && d->kp >= 2048) return launch_gemm_i8<T, 64, 64, 32, 32, 128, 2, 4>(d, st);
+    return launch_gemm_i8<T, 64, 64, 32, 32, 128, 2, 1>(d, st);
 }
 
 extern "C" int mv_gemm_i8(const mv_gemm_i8_desc* d, void* stream) {

@@ -718,7 +718,7 @@ def linear_oracle(x, codes, w_scale, bias, residual, silu):
 
 LIN = [(1, 16384, 40), (1, 16385, 40), (3, 5000, 100), (8, 2048, 64), (8, 2049, 64), (16, 1024, 48), (16, 1025, 48), (1, 1, 1), (4, 3, 5), (1, 128, 128), (1, 1280, 5120), (1, 1000, 1111), (2, 64, 7), (3, 40, 1), (5, 5120, 640), (8, 129, 33), (16, 1280, 320), (17, 1280, 320), (31, 384, 257),
        (33, 256, 96), (64, 640, 640), (65, 1000, 255), (127, 128, 256), (128, 256, 128), (129, 320, 129), (255, 2560, 320), (300, 1152, 1000),
-       (1001, 1000, 1111), (1000, 5120, 1280), (4100, 640, 512), (513, 16, 513), (2, 9000, 48)]
+       (1001, 1000, 1111), (1000, 5120, 1280), (4100, 640, 512), (513, 16, 513), (2, 9000, 48), (33, 16, 33), (40, 130, 1000), (100, 700, 130), (513, 2050, 1000), (400, 3000, 1000), (25, 2100, 90), (700, 128, 260)]
 
 
 @gpu
