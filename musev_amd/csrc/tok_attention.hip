@@ -33,15 +33,16 @@ template <> struct ExpBits<bf16_t> { static constexpr unsigned mask = 0x7f807f80
 
 template <bool B> struct Masked { static constexpr bool value = B; };
 
-template <int DC>
+// K16: 16-column steps of the head dim
+template <int K16>
 struct PackedCfg {
-    static constexpr int RS = DC <= 64 ? 64 : 128;     // elements per LDS row
+    static constexpr int RS = K16 <= 4 ? 64 : 128;     // elements per LDS row
     static constexpr int SLOTS = RS / 8;               // 16-byte slots per LDS row
     static constexpr int KT = 64;                      // keys per tile
     static constexpr int TILE = KT * RS;               // elements of a K (or V) tile
     static constexpr int PPW = TILE * 2 / 1024 / 4;    // 1-KiB pieces of it that one wave fetches
     static constexpr int LDS_BYTES = 2 * 2 * TILE * 2; // two stages of K, V
-    static constexpr int NS = KT / 32, NB = DC / 32;   // 32-key score blocks of a tile, 32-column blocks of the output
+    static constexpr int NS = KT / 32, NB = (K16 + 1) / 2;   // 32-key score blocks of a tile, 32-column blocks of the output
 };
 
 // The slot permutation of a row.  K: 16 rows x one slot must fall on 16 different slots of a 256-byte line (two rows of 128 bytes share a
@@ -49,9 +50,9 @@ struct PackedCfg {
 template <int RS> __device__ __forceinline__ int swz_k(int row) { return RS == 128 ? (row & 15) : ((row >> 1) & 7); }
 template <int RS> __device__ __forceinline__ int swz_v(int row) { return RS == 128 ? ((row & 3) << 2) : (((row >> 1) & 1) << 2); }
 
-template <typename T, int DC>
+template <typename T, int K16>
 __global__ __launch_bounds__(256, 2) void attention_packed_kernel(const mv_attn_packed_desc p) {
-    using C = PackedCfg<DC>;
+    using C = PackedCfg<K16>;
     typedef typename Vec8<T>::type V8;
     typedef __attribute__((address_space(3))) T lds_t;
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -70,11 +71,11 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(const mv_attn_
 
     // ---- Q (second operand of S^T): row in the lane, 8 columns per half wave and step; a negative scale turns its sign here ----
     const float c = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-30f);   // scores in powers of two
-    V8 qf[DC / 16];
+    V8 qf[K16];
     {
         const T* q = (const T*)p.q + (int64_t)(it.q_row + qi) * p.ldq + (int64_t)hq * p.d;
 #pragma unroll
-        for (int s = 0; s < DC / 16; ++s) {
+        for (int s = 0; s < K16; ++s) {
             const int col = 16 * s + 8 * h;
             u32x4 w = {0, 0, 0, 0};
             if (col < p.d) w = *(const u32x4*)(q + col);
@@ -119,9 +120,9 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(const mv_attn_
 
     // ---- one tile ----
     const int i16 = lane & 15;
-    int ka[C::SLOTS / 2];    // element offset of K fragment step s in a tile (row l31)
+    int ka[K16];   // element offset of K fragment step s in a tile (row l31)
 #pragma unroll
-    for (int s = 0; s < DC / 16; ++s) ka[s] = l31 * C::RS + ((2 * s + h) ^ swz_k<C::RS>(l31)) * 8;
+    for (int s = 0; s < K16; ++s) ka[s] = l31 * C::RS + ((2 * s + h) ^ swz_k<C::RS>(l31)) * 8;
     int va[C::NB];           // element offset of V^T fragment block b (keys 4 h + 0..3)
 #pragma unroll
     for (int b = 0; b < C::NB; ++b) {
@@ -139,7 +140,7 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(const mv_attn_
             for (int e = 0; e < 16; ++e) s[n][e] = 0.f;
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int k = 0; k < DC / 16; ++k)
+        for (int k = 0; k < K16; ++k)
 #pragma unroll
             for (int n = 0; n < C::NS; ++n) {
                 const V8 kf = *(const __attribute__((address_space(3))) V8*)(sk + ka[k] + n * 32 * C::RS);
@@ -346,10 +347,10 @@ extern "C" int64_t mv_attention_packed_workspace_bytes(int64_t ws_rows, int32_t 
 
 constexpr int64_t JOIN_FEW = 2048;   // packed rows up to which four waves join a row: two blocks of them per SIMD of the chip
 
-template <typename T, int DC>
+template <typename T, int K16>
 static int launch_packed(const mv_attn_packed_desc* d, hipStream_t st) {
-    static_assert(PackedCfg<DC>::LDS_BYTES <= 64 * 1024, "dynamic LDS without an attribute");
-    attention_packed_kernel<T, DC><<<(unsigned)(d->n_items * d->kv_heads), 256, PackedCfg<DC>::LDS_BYTES, st>>>(*d);
+    static_assert(PackedCfg<K16>::LDS_BYTES <= 64 * 1024, "dynamic LDS without an attribute");
+    attention_packed_kernel<T, K16><<<(unsigned)(d->n_items * d->kv_heads), 256, PackedCfg<K16>::LDS_BYTES, st>>>(*d);
     MV_CHECK_LAUNCH("mv_attention_packed");
     if (d->n_joins > 0) {
         const int64_t rows = (int64_t)d->n_joins * d->kv_heads * d->join_rows;
@@ -360,10 +361,18 @@ static int launch_packed(const mv_attn_packed_desc* d, hipStream_t st) {
     return MV_OK;
 }
 
-// head dims up to 64, 96 and 128: the columns a tile is multiplied over
 template <typename T>
 static int launch_head_dim(const mv_attn_packed_desc* d, hipStream_t st) {
-    return d->d <= 64 ? launch_packed<T, 64>(d, st) : d->d <= 96 ? launch_packed<T, 96>(d, st) : launch_packed<T, 128>(d, st);
+    switch ((d->d + 15) / 16) {
+        case 1: return launch_packed<T, 1>(d, st);
+        case 2: return launch_packed<T, 2>(d, st);
+        case 3: return launch_packed<T, 3>(d, st);
+        case 4: return launch_packed<T, 4>(d, st);
+        case 5: return launch_packed<T, 5>(d, st);
+        case 6: return launch_packed<T, 6>(d, st);
+        case 7: return launch_packed<T, 7>(d, st);
+        default: return launch_packed<T, 8>(d, st);
+    }
 }
 
 extern "C" int mv_attention_packed(const mv_attn_packed_desc* d, void* stream) {

@@ -367,6 +367,10 @@ ATTN = {
     "one_token_wide_group": ([1, 2], [700, 9000], 32, 1, 128, True),
     "few_rows_long_keys": ([3, 2], [16500, 12001], 4, 2, 64, True),
     "d8": ([33, 70], None, 2, 1, 8, True),
+    "d16": ([33, 70], [100, 71], 2, 1, 16, False),
+    "d32": ([129, 65], None, 2, 2, 32, True),
+    "d48": ([65], [190], 4, 2, 48, True),
+    "d112": ([150], None, 2, 2, 112, True),
     "d72": ([33, 150], None, 2, 2, 72, False),
     "d96": ([200], None, 2, 2, 96, True),
     "d120": ([100], [333], 2, 1, 120, True),
