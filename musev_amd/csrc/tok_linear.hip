@@ -197,13 +197,15 @@ __global__ __launch_bounds__((GemmI8Cfg<BM, BN, WM, WN, BK, NST, KS>::THREADS), 
 #pragma unroll
     for (int i = 0; i < WM / 32; ++i) as[i] = p.a_scale[min(m0 + wm + 32 * i + l31, p.M - 1)];
     // The residual is fetched beside the last two steps: as long as the sums take, its loads are hidden (26 624 x 1280 -> 5120: one block per CU,
-    // nothing else would hide them).  Only whole 16-byte loads, so that their number is known to the wait below; rows and columns past the end
-    // fetch the last ones.  Otherwise it is read where it is added.
+    // nothing else would hide them).  Every lane makes all its loads, whole ones of 16 bytes, so that at least FIRST of them are younger than the
+    // last stage's when the wait below counts: rows past the end fetch the last one, columns past the end (and the fewer than 8 that end a row,
+    // which are read where they are added) the row's last 8.
     V8 res[NRES];
     auto residual_at = [&](int x) __attribute__((always_inline)) {
-        return (const V8*)((const T*)p.residual + min(m0 + wm + 32 * (x / PASSES) + (x % PASSES) * RPP + frow, p.M - 1) * p.ldr + min(n, p.N - 8));
+        const T* r = (const T*)p.residual + min(m0 + wm + 32 * (x / PASSES) + (x % PASSES) * RPP + frow, p.M - 1) * p.ldr + min(n, p.N - 8);
+        return __builtin_bit_cast(V8, ((const typename Loose8<T>::bytes*)r)->v);
     };
-    const bool early = p.residual && kg == 0 && p.kp > KS * BK && ((p.N | p.ldr) & 7) == 0 && ((uintptr_t)p.residual & 15) == 0;
+    const bool early = p.residual && kg == 0 && p.kp > KS * BK && p.N >= 8;
 
     const int steps = p.kp / BK, turns = (steps + KS - 1) / KS;   // this group's steps: kg, kg + KS, ...; the first group has one every turn
     int into = 0, from = 0;
@@ -222,7 +224,7 @@ __global__ __launch_bounds__((GemmI8Cfg<BM, BN, WM, WN, BK, NST, KS>::THREADS), 
         if (t + 2 == turns && early) {
             asm volatile("" ::: "memory");   // (behind the last stage's loads)
 #pragma unroll
-            for (int x = 0; x < FIRST; ++x) res[x] = *residual_at(x);
+            for (int x = 0; x < FIRST; ++x) res[x] = residual_at(x);
             asm volatile("" ::: "memory");
         }
         into = into + 1 == NST ? 0 : into + 1;
@@ -245,7 +247,7 @@ __global__ __launch_bounds__((GemmI8Cfg<BM, BN, WM, WN, BK, NST, KS>::THREADS), 
     }
     if (early) {
 #pragma unroll
-        for (int x = FIRST; x < NRES; ++x) res[x] = *residual_at(x);
+        for (int x = FIRST; x < NRES; ++x) res[x] = residual_at(x);
     }
     __syncthreads();   // the stages become the groups' sums and the waves' result staging
     if constexpr (KS > 1) {
@@ -309,7 +311,7 @@ __global__ __launch_bounds__((GemmI8Cfg<BM, BN, WM, WN, BK, NST, KS>::THREADS), 
             if (p.act == MV_ACT_SILU)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = mv_silu(v[e]);
-            if (early) {
+            if (early && left >= 8) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] += (float)res[i * PASSES + x][e];
             } else if (p.residual) {

@@ -56,7 +56,7 @@ def _launch(entry: str, desc: bytes, dev: int, held: Sequence["_Held"] = ()) -> 
     for h in held:
         if stream not in h._streams:
             h._use(stream)
-    status = getattr(_lib.load(), entry)(desc, stream)
+    status = getattr(_lib._lib or _lib.load(), entry)(desc, stream)
     if status:
         check(status, entry)
 
@@ -68,7 +68,7 @@ def _matrix(t: torch.Tensor, name: str, dtype: Optional[torch.dtype] = None, dev
     (rows, cols), (ld, inner) = t.shape, t.stride()
     if inner != 1 and cols > 1:
         raise ValueError(f"{name}: expected unit inner stride, got shape {(rows, cols)} strides {(ld, inner)}")
-    if not _on_gpu(t) or (t.dtype not in _DTYPES if dtype is None else t.dtype != dtype):
+    if dev is None and not _on_gpu(t) or (t.dtype not in _DTYPES if dtype is None else t.dtype != dtype):
         raise ValueError(f"{name}: expected a CUDA {'fp16 | bf16' if dtype is None else dtype} tensor, got {t.dtype} on {t.device}")
     if dev is not None and t.get_device() != dev:
         raise ValueError(f"{name}: on {t.device}, the other tensors are on device {dev}")
