@@ -10,6 +10,8 @@ LIB=${MV_LIB_NAME:-libmusev_hip.so}
 OBJ=build
 if [ "$LIB" != "libmusev_hip.so" ]; then OBJ=build_${LIB%.so}; fi
 FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=fast ${MV_EXTRA_FLAGS:-}"
+# packed-fp32 instructions: some of their operand forms gave wrong results on the MI355X (common.h, MV_FMA_SCALAR)
+TOK_FLAGS="-Xclang -target-feature -Xclang -packed-fp32-ops"
 mkdir -p $OBJ
 pids=()
 for f in lib gemm norm attention elementwise ffn tsa xab; do
@@ -18,15 +20,14 @@ for f in lib gemm norm attention elementwise ffn tsa xab; do
     pids+=($!)
   fi
 done
-# the token-transformer kernels: no packed-fp32 instructions (some of their operand forms gave wrong results on the MI355X, see common.h)
-TOK="tok_attention tok_rotary tok_norm tok_linear"
-TOK_FLAGS="-Xclang -target-feature -Xclang -packed-fp32-ops"
+# the token-transformer kernels (tokens/), into objects of their own
+TOK="attention rotary norm linear"
 for f in $TOK; do
-  if [ ! -f $OBJ/$f.o ] || [ $f.hip -nt $OBJ/$f.o ] || [ common.h -nt $OBJ/$f.o ] || [ tok_common.h -nt $OBJ/$f.o ] || [ ../../include/musev_tokens.h -nt $OBJ/$f.o ] || [ ../../include/musev_hip.h -nt $OBJ/$f.o ]; then
-    $HIPCC $FLAGS $TOK_FLAGS -c $f.hip -o $OBJ/$f.o &
+  if [ ! -f $OBJ/tok_$f.o ] || [ tokens/$f.hip -nt $OBJ/tok_$f.o ] || [ common.h -nt $OBJ/tok_$f.o ] || [ tokens/tokens.h -nt $OBJ/tok_$f.o ] || [ ../../include/musev_tokens.h -nt $OBJ/tok_$f.o ] || [ ../../include/musev_hip.h -nt $OBJ/tok_$f.o ]; then
+    $HIPCC $FLAGS $TOK_FLAGS -c tokens/$f.hip -o $OBJ/tok_$f.o &
     pids+=($!)
   fi
 done
 for p in "${pids[@]:-}"; do [ -n "$p" ] && wait $p; done
-$HIPCC --offload-arch=gfx950 -shared -fPIC -o $LIB $OBJ/lib.o $OBJ/gemm.o $OBJ/norm.o $OBJ/attention.o $OBJ/elementwise.o $OBJ/ffn.o $OBJ/tsa.o $OBJ/xab.o $(for f in $TOK; do echo $OBJ/$f.o; done)
+$HIPCC --offload-arch=gfx950 -shared -fPIC -o $LIB $OBJ/lib.o $OBJ/gemm.o $OBJ/norm.o $OBJ/attention.o $OBJ/elementwise.o $OBJ/ffn.o $OBJ/tsa.o $OBJ/xab.o $(for f in $TOK; do echo $OBJ/tok_$f.o; done)
 echo "built $(pwd)/$LIB"

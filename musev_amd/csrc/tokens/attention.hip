@@ -1,4 +1,4 @@
-// tok_attention.hip -- packed attention (include/musev_tokens.h: mv_attention_packed).
+// tokens/attention.hip -- packed attention (include/musev_tokens.h: mv_attention_packed).
 //
 // One pass over the keys with a running maximum and sum.  A (sequence, key / value head) has q_len * group packed rows, row r = query
 // r / group, head r % group of the group: the heads that share keys share the tile that holds them, and one token of a wide group is a
@@ -13,7 +13,7 @@
 // 4 waves x 32 packed rows share 64-key tiles, two stages, one barrier per tile, two blocks per CU: 64 KB on its way per CU, enough to stream the
 // cache of a single token too, where one wave alone has rows (a form whose 4 waves walked tiles of their own for up to 32 rows was no faster:
 // 16 requests over 86 k keys 82 against 77 us).
-#include "tok_common.h"
+#include "tokens.h"
 
 extern "C" int mv_tokens_abi_version(void) { return MV_TOKENS_ABI_VERSION; }
 

@@ -1,5 +1,5 @@
-// tok_linear.hip -- the int8 projection (include/musev_tokens.h: mv_quantize_rows_i8, mv_gemm_i8).
-#include "tok_common.h"
+// tokens/linear.hip -- the int8 projection (include/musev_tokens.h: mv_quantize_rows_i8, mv_gemm_i8).
+#include "tokens.h"
 
 // ---- activations to int8, one scale per row ------------------------------------------------------------------------------------
 // code = rne(127 x / top) with top = max |x|, of the exact quotient q: x = X 2^a and top = T 2^b with integers X, T < 2^11, so a q that is no

@@ -1,5 +1,5 @@
-// tok_norm.hip -- the gated residual norm (include/musev_tokens.h: mv_gated_residual_norm).
-#include "tok_common.h"
+// tokens/norm.hip -- the gated residual norm (include/musev_tokens.h: mv_gated_residual_norm).
+#include "tokens.h"
 
 // sums over a row held by WAVES waves
 template <int WAVES>

@@ -1,5 +1,5 @@
-// tok_rotary.hip -- rotary positions with several axes (include/musev_tokens.h: mv_rotary_axes).
-#include "tok_common.h"
+// tokens/rotary.hip -- rotary positions with several axes (include/musev_tokens.h: mv_rotary_axes).
+#include "tokens.h"
 
 // The angle of a pair is position * turns full turns.  It is formed in fp64: at position 131072 an fp32 product of the two is off by
 // up to 2^-7 turns, while the fp64 product keeps its fraction of a turn to 2^-35; only that fraction goes on in fp32.

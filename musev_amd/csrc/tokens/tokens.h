@@ -1,7 +1,7 @@
-// tok_common.h -- shared helpers of the token-transformer kernels (tok_*.hip).
+// tokens.h -- shared helpers of the token-transformer kernels.
 #pragma once
-#include "common.h"
-#include "../../include/musev_tokens.h"
+#include "../common.h"
+#include "../../../include/musev_tokens.h"
 
 typedef __bf16 bf16_t;
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
