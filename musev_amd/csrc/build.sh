@@ -9,13 +9,13 @@ HIPCC=${HIPCC:-/opt/rocm/bin/hipcc}
 LIB=${MV_LIB_NAME:-libmusev_hip.so}
 OBJ=build
 if [ "$LIB" != "libmusev_hip.so" ]; then OBJ=build_${LIB%.so}; fi
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=fast ${MV_EXTRA_FLAGS:-}"
-# packed-fp32 instructions: some of their operand forms gave wrong results on the MI355X (common.h, MV_FMA_SCALAR)
-TOK_FLAGS="-Xclang -target-feature -Xclang -packed-fp32-ops"
+# no packed-fp32 instructions: some of their operand forms gave wrong results on the MI355X now and then (common.h, MV_FMA_SCALAR); hipcc makes them
+# from ordinary float code (its host pass warns that it does not know the feature)
+FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=fast -Xclang -target-feature -Xclang -packed-fp32-ops ${MV_EXTRA_FLAGS:-}"
 mkdir -p $OBJ
 pids=()
 for f in lib gemm norm attention elementwise ffn tsa xab; do
-  if [ ! -f $OBJ/$f.o ] || [ $f.hip -nt $OBJ/$f.o ] || [ common.h -nt $OBJ/$f.o ] || [ gemm_tuned.h -nt $OBJ/$f.o ] || [ ../../include/musev_hip.h -nt $OBJ/$f.o ]; then
+  if [ ! -f $OBJ/$f.o ] || [ build.sh -nt $OBJ/$f.o ] || [ $f.hip -nt $OBJ/$f.o ] || [ common.h -nt $OBJ/$f.o ] || [ gemm_tuned.h -nt $OBJ/$f.o ] || [ ../../include/musev_hip.h -nt $OBJ/$f.o ]; then
     $HIPCC $FLAGS -c $f.hip -o $OBJ/$f.o &
     pids+=($!)
   fi
@@ -23,8 +23,8 @@ done
 # the token-transformer kernels (tokens/), into objects of their own
 TOK="attention rotary norm linear"
 for f in $TOK; do
-  if [ ! -f $OBJ/tok_$f.o ] || [ tokens/$f.hip -nt $OBJ/tok_$f.o ] || [ common.h -nt $OBJ/tok_$f.o ] || [ tokens/tokens.h -nt $OBJ/tok_$f.o ] || [ ../../include/musev_tokens.h -nt $OBJ/tok_$f.o ] || [ ../../include/musev_hip.h -nt $OBJ/tok_$f.o ]; then
-    $HIPCC $FLAGS $TOK_FLAGS -c tokens/$f.hip -o $OBJ/tok_$f.o &
+  if [ ! -f $OBJ/tok_$f.o ] || [ build.sh -nt $OBJ/tok_$f.o ] || [ tokens/$f.hip -nt $OBJ/tok_$f.o ] || [ common.h -nt $OBJ/tok_$f.o ] || [ tokens/tokens.h -nt $OBJ/tok_$f.o ] || [ ../../include/musev_tokens.h -nt $OBJ/tok_$f.o ] || [ ../../include/musev_hip.h -nt $OBJ/tok_$f.o ]; then
+    $HIPCC $FLAGS -c tokens/$f.hip -o $OBJ/tok_$f.o &
     pids+=($!)
   fi
 done
