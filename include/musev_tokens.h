@@ -81,7 +81,7 @@ int mv_gated_residual_norm(const mv_gated_norm_desc* d, void* stream);
 /* ---- int8 projection -----------------------------------------------------------------------------------------------------------------
  * mv_quantize_rows_i8: scale[m] = max_k |x[m, k]| / 127, code = round-to-nearest-even(127 x / max|x|); columns K .. ldc - 1 of the codes
  * become 0; a row of zeros has scale 0; a row that holds an infinity or NaN has that scale and codes 0 (its products are NaN).
- * mv_gemm_i8: out = act(a_scale[m] * w_scale[n] * sum_k a[m, k] w[n, k] + bias[n]) + residual[m, n];  the sum is exact (int32).
+ * mv_gemm_i8: out = act(a_scale[m] * w_scale[n] * sum_k a[m, k] w[n, k] + bias[n]) + residual[m, n];  the sum is exact (int32: K <= 131071).
  * lda, ldw: multiples of 128, the columns from K on are 0.                                                                             */
 int mv_quantize_rows_i8(const void* x, int64_t ldx, int64_t rows, int32_t k, int32_t dtype, int8_t* codes, int64_t ldc, float* scale,
                         void* stream);

@@ -103,7 +103,7 @@ static void launch_quantize_width(const void* x, int64_t ldx, int64_t rows, int 
 extern "C" int mv_quantize_rows_i8(const void* x, int64_t ldx, int64_t rows, int32_t k, int32_t dtype, int8_t* codes, int64_t ldc, float* scale,
                                    void* stream) {
     MV_REQUIRE(dtype == MV_F16 || dtype == MV_BF16, "mv_quantize_rows_i8: element type %d", dtype);
-    MV_REQUIRE(rows >= 0 && rows < (1ll << 31) && k >= 1 && k <= 131072, "mv_quantize_rows_i8: %ld rows of %d (1 .. 131072)", (long)rows, k);
+    MV_REQUIRE(rows >= 0 && rows < (1ll << 31) && k >= 1 && k <= 131071, "mv_quantize_rows_i8: %ld rows of %d (1 .. 131071)", (long)rows, k);
     MV_REQUIRE(ldc % 128 == 0 && ldc >= k && ldc < k + 128, "mv_quantize_rows_i8: code rows of %ld for k = %d (k rounded up to 128)", (long)ldc, k);
     if (rows == 0) return MV_OK;
     MV_REQUIRE(x && codes && scale && ((uintptr_t)codes & 15) == 0, "mv_quantize_rows_i8: null or unaligned pointer");
@@ -497,7 +497,7 @@ extern "C" int mv_gemm_i8(const mv_gemm_i8_desc* d, void* stream) {
 
 extern "C" int mv_linear_i8(const mv_linear_i8_desc* d, void* stream) {
     MV_REQUIRE(d, "mv_linear_i8: null descriptor");
-    MV_REQUIRE(d->M >= 0 && d->K >= 1 && d->kp >= d->K && d->kp < d->K + 128 && d->kp % 128 == 0, "mv_linear_i8: M %ld, K %d, kp %ld", (long)d->M, d->K, (long)d->kp);
+    MV_REQUIRE(d->M >= 0 && d->K >= 1 && d->K <= 131071 && d->kp >= d->K && d->kp < d->K + 128 && d->kp % 128 == 0, "mv_linear_i8: M %ld, K %d (1 .. 131071: the sums fit 32 bits), kp %ld", (long)d->M, d->K, (long)d->kp);
     if (d->M == 0) return MV_OK;
     if (one_launch(d->M, d->kp)) {
         MV_REQUIRE(d->dtype == MV_F16 || d->dtype == MV_BF16, "mv_linear_i8: element type %d", d->dtype);

@@ -440,11 +440,14 @@ def gated_residual_norm(x: torch.Tensor, f: torch.Tensor, *, kind: str = "layer"
 
 
 # ---- int8 projection ------------------------------------------------------------------------------------------------------------------
+_I8_MAX_K = 131071   # K * 128 * 128 < 2^31: the sum of any int8 products fits 32 bits
+
+
 class Int8Rows(_Held):
     """int8 rows with one scale each: row m stands for ``codes[m, :k] * scale[m]``.  ``codes`` is padded with zeros to a multiple of 128 columns."""
 
     def __init__(self, codes: torch.Tensor, scale: torch.Tensor, k: int):
-        if codes.dtype != torch.int8 or codes.ndim != 2 or not codes.is_contiguous() or codes.shape[1] != -(-k // 128) * 128 or \
+        if not 1 <= k <= _I8_MAX_K or codes.dtype != torch.int8 or codes.ndim != 2 or not codes.is_contiguous() or codes.shape[1] != -(-k // 128) * 128 or \
                 scale.dtype != torch.float32 or scale.shape != codes.shape[:1] or not scale.is_contiguous() or scale.device != codes.device:
             raise ValueError(f"Int8Rows: codes must be contiguous int8 [rows, {k} rounded up to 128] and scale contiguous fp32 [rows] beside them")
         self.codes, self.scale, self.k, self.rows, self.kp = codes, scale, k, codes.shape[0], codes.shape[1]
@@ -455,8 +458,8 @@ class Int8Rows(_Held):
 def pack_weight_i8(codes: torch.Tensor, scale: torch.Tensor) -> Int8Rows:
     """:class:`Int8Rows` from int8 ``codes`` [N, K] and fp32 ``scale`` [N] (a checkpoint's weight: one scale per output channel), laid out for
     :func:`gemm_i8` once."""
-    if codes.dim() != 2 or codes.dtype != torch.int8 or not _on_gpu(codes) or not 1 <= codes.shape[1] <= 131072:
-        raise ValueError("pack_weight_i8: codes must be a CUDA int8 [N, K] tensor, K <= 131072")
+    if codes.dim() != 2 or codes.dtype != torch.int8 or not _on_gpu(codes) or not 1 <= codes.shape[1] <= _I8_MAX_K:
+        raise ValueError(f"pack_weight_i8: codes must be a CUDA int8 [N, K] tensor, K <= {_I8_MAX_K}")
     if scale.dtype != torch.float32 or scale.shape != (codes.shape[0],) or scale.device != codes.device:
         raise ValueError(f"pack_weight_i8: scale must be fp32 [{codes.shape[0]}] on {codes.device}")
     n, k = codes.shape
@@ -469,8 +472,8 @@ def quantize_rows_i8(x: torch.Tensor) -> Int8Rows:
     """Each row of ``x`` [M, K] (fp16 | bf16) as int8 codes and one scale: scale = max|x| / 127, code = 127 x / max|x| rounded to nearest, ties
     to even.  A row of zeros has scale 0; a row that holds an infinity or NaN keeps that as its scale (its products are NaN)."""
     m, k, ld = _matrix(x, "x")
-    if not 1 <= k <= 131072:
-        raise ValueError(f"quantize_rows_i8: {k} columns (1 .. 131072)")
+    if not 1 <= k <= _I8_MAX_K:
+        raise ValueError(f"quantize_rows_i8: {k} columns (1 .. {_I8_MAX_K})")
     kp = -(-k // 128) * 128
     codes = torch.empty((m, kp), dtype=torch.int8, device=x.device)
     scale = torch.empty((m,), dtype=torch.float32, device=x.device)

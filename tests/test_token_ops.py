@@ -118,7 +118,7 @@ def test_entry_points_refuse_without_a_gpu():
     ln.M, ln.workspace = 17, 0
     refused(lib.mv_linear_i8(C.byref(ln), None), b"workspace")
     refused(lib.mv_quantize_rows_i8(16, 64, 4, 64, 0, 16, 64, 16, None), b"code rows")
-    refused(lib.mv_quantize_rows_i8(16, 64, 4, 0, 0, 16, 128, 16, None), b"131072")
+    refused(lib.mv_quantize_rows_i8(16, 64, 4, 0, 0, 16, 128, 16, None), b"131071")
 
 
 def _cover(items, joins, ws_rows, ql, kl, group, causal):
@@ -300,6 +300,8 @@ def test_refusals_of_the_int8_projection(on_cpu):
     sq = ops.pack_weight_i8(torch.ones(40, 40, dtype=torch.int8), torch.ones(40))
     with pytest.raises(ValueError, match="overlaps"):
         ops.linear_i8(x, sq, out=x)
+    with pytest.raises(ValueError, match="131071"):
+        ops.pack_weight_i8(torch.zeros(1, 131072, dtype=torch.int8), torch.ones(1))
     for codes, scale, match in ((w.codes.int(), w.scale, "codes"), (w.codes, w.scale[:3], "scale"), (w.codes, w.scale.double(), "scale")):
         with pytest.raises(ValueError, match=match):
             ops.pack_weight_i8(codes, scale)
@@ -472,6 +474,38 @@ def test_attention_leaves_rows_behind_the_last_sequence_and_other_columns():
     assert res is out
     within(out[:145], *attention_oracle(q, k, v, ql, ql, heads, heads, d, True))
     assert bool((wide[145:] == 7).all()) and bool((wide[:, :8] == 7).all()) and bool((wide[:, 8 + heads * d:] == 7).all())
+
+
+@gpu
+def test_attention_of_no_rows_at_all():
+    from musev_amd import ops
+    for dt in DTYPES:
+        e = torch.empty(0, 128, dtype=dt, device=DEV)
+        assert ops.attention_packed(ops.attention_plan([0, 0], heads=2, d=64), e, e, e).shape == (0, 128)
+        k = rnd((9, 128), 1, dt)
+        assert ops.attention_packed(ops.attention_plan([0, 0], [4, 5], heads=2, d=64), e, k, k).shape == (0, 128)
+        q = rnd((7, 128), 2, dt)
+        got = ops.attention_packed(ops.attention_plan([3, 4], [0, 0], heads=2, d=64), q, e, e)
+        torch.cuda.synchronize()
+        assert bool((got == 0).all())
+
+
+@gpu
+def test_attention_far_into_a_large_matrix():
+    """key rows whose byte offsets pass 2^32, and rows 8 MB apart"""
+    from musev_amd import ops
+    dt, d = torch.float16, 64
+    ld = 1 << 20
+    big = torch.zeros(3000 * ld + 512, dtype=dt, device=DEV)     # 6 GB
+    k = big[:3000 * ld].view(3000, ld)[:, 8:8 + d]
+    v = big[:3000 * ld].view(3000, ld)[:, 128:128 + d]
+    k.copy_(rnd((3000, d), 3, dt))
+    v.copy_(rnd((3000, d), 4, dt))
+    q = rnd((131, d), 5, dt)
+    ql, kl = [1, 130], [100, 2900]
+    got = ops.attention_packed(ops.attention_plan(ql, kl, heads=1, d=d), q, k, v)
+    torch.cuda.synchronize()
+    within(got, *attention_oracle(q, k.contiguous(), v.contiguous(), ql, kl, 1, 1, d, True))
 
 
 # ---- rotary positions ---------------------------------------------------------------------------------------------------------------
@@ -847,8 +881,12 @@ def test_two_captured_graphs_and_eager_calls_agree():
     long_q, long_k, long_v = attention_inputs([1, 2], [9000, 7001], 8, 2, 128, dt, 17)
     plan = b1.ops.attention_plan([1, 2], [9000, 7001], heads=8, kv_heads=2, d=128)   # (joined partial sums: a workspace per graph)
 
+    deep = b1.ops.pack_weight_i8(torch.randint(-127, 128, (640, 3000), generator=torch.Generator().manual_seed(4), dtype=torch.int32).to(torch.int8).to(DEV),
+                                 torch.full((640,), 0.001, device=DEV))
+    rows = rnd((300, 3000), 18, dt)   # (K in groups of waves: more LDS than a launch has by default)
+
     def work(b, x):
-        return (*b(x), b.ops.attention_packed(plan, long_q, long_k, long_v))
+        return (*b(x), b.ops.attention_packed(plan, long_q, long_k, long_v), b.ops.linear_i8(rows, deep))
     want = [[t.clone() for t in work(b, x)] for b, x in zip((b1, b2), xs)]
     torch.cuda.synchronize()
     graphs, outs, ins = [], [], [x.clone() for x in xs]
