@@ -55,7 +55,7 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(const mv_attn_
     using C = PackedCfg<K16>;
     typedef typename Vec8<T>::type V8;
     typedef __attribute__((address_space(3))) T lds_t;
-    extern __shared__ __attribute__((aligned(16))) char smem[];
+    extern __shared__ __attribute__((aligned(256))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const PackedItem it = ((const PackedItem*)p.items)[blockIdx.x / p.kv_heads];
@@ -120,32 +120,46 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(const mv_attn_
 
     // ---- one tile ----
     const int i16 = lane & 15;
-    int ka[K16];   // element offset of K fragment step s in a tile (row l31)
-#pragma unroll
-    for (int s = 0; s < K16; ++s) ka[s] = l31 * C::RS + ((2 * s + h) ^ swz_k<C::RS>(l31)) * 8;
-    int va[C::NB];           // element offset of V^T fragment block b (keys 4 h + 0..3)
-#pragma unroll
-    for (int b = 0; b < C::NB; ++b) {
-        const int row = 4 * h + (i16 >> 2), slot = 4 * b + 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
-        va[b] = row * C::RS + (slot ^ swz_v<C::RS>(row)) * 8 + (i16 & 1) * 4;
-    }
+    // A fragment's LDS address is one per lane and operand, its step or block an XOR (slots are permuted by XOR, rows are whole lines) and its
+    // rows an immediate offset.  K fragment step k: row l31, slot 2 k + h; V^T fragment block b: keys 4 h + 0..3, columns 32 b.
+    const unsigned ka = (unsigned)(l31 * C::RS + (h ^ swz_k<C::RS>(l31)) * 8) * 2;
+    const int vrow = 4 * h + (i16 >> 2), vslot = 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
+    const unsigned va = (unsigned)(vrow * C::RS + (vslot ^ swz_v<C::RS>(vrow)) * 8 + (i16 & 1) * 4) * 2;
     auto compute = [&](int key, int stage, auto tag) __attribute__((always_inline)) {
         constexpr bool masked = decltype(tag)::value;   // some row may not see all of the tile
-        const lds_t* sk = ring + stage * 2 * C::TILE;
-        const lds_t* sv = sk + C::TILE;
+        // At two waves per SIMD (head dims from 65 on) fragments are read AHEAD matrix instructions before they are used and the order is pinned:
+        // left to itself the compiler reads each just before its use and the matrix pipe waits out the LDS latency (d = 128, a causal prompt of 16384:
+        // 1.07 -> 1.02 ms).  With more waves the others cover it and the compiler's own order is as good (d = 64, 8192 tokens: 168 against 171 us).
+        constexpr bool PINNED = K16 > 4;
+        const lds_t* sv = ring + stage * 2 * C::TILE + C::TILE;
+        const unsigned kb = (unsigned)(uintptr_t)(ring + stage * 2 * C::TILE) + ka, vb = (unsigned)(uintptr_t)sv + va;
+        constexpr int NK = K16 * C::NS, NV = 2 * C::NS * C::NB, AHEAD = PINNED ? 3 : 1;
+        auto k_frag = [&](int f) __attribute__((always_inline)) {
+            return *(const __attribute__((address_space(3))) V8*)(uintptr_t)((kb ^ (f / C::NS << 5)) + f % C::NS * 32 * C::RS * 2);
+        };
+        auto v_frag = [&](int f) __attribute__((always_inline)) {
+            const unsigned at = (vb ^ (f % C::NB << 6)) + f / C::NB * 16 * C::RS * 2;
+            const short4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(uintptr_t)at);
+            const short4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(uintptr_t)(at + 8 * C::RS * 2));
+            typedef short short8v __attribute__((ext_vector_type(8)));
+            return __builtin_bit_cast(V8, short8v{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
+        };
         float16v s[C::NS];
 #pragma unroll
         for (int n = 0; n < C::NS; ++n)
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[n][e] = 0.f;
+        V8 kf[NK], vf[NV];
+#pragma unroll
+        for (int f = 0; f < AHEAD && f < NK; ++f) kf[f] = k_frag(f);
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int k = 0; k < K16; ++k)
-#pragma unroll
-            for (int n = 0; n < C::NS; ++n) {
-                const V8 kf = *(const __attribute__((address_space(3))) V8*)(sk + ka[k] + n * 32 * C::RS);
-                s[n] = mfma_32x32x16(kf, qf[k], s[n]);
-            }
+        for (int f = 0; f < NK; ++f) {
+            if constexpr (PINNED) __builtin_amdgcn_sched_barrier(0);
+            s[f % C::NS] = mfma_32x32x16(kf[f], qf[f / C::NS], s[f % C::NS]);
+            if (f + AHEAD < NK) kf[f + AHEAD] = k_frag(f + AHEAD);
+        }
+        if constexpr (PINNED) __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_setprio(0);
         if constexpr (masked) {
             const int left = lim - key - 4 * h;
@@ -174,6 +188,10 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(const mv_attn_
         }
         const float mc = m * c;
         float t0 = 0.f, t1 = 0.f;
+        if constexpr (!masked) {   // (beside the exponentials)
+#pragma unroll
+            for (int f = 0; f < AHEAD && f < NV; ++f) vf[f] = v_frag(f);
+        }
         V8 pf[2 * C::NS];
 #pragma unroll
         for (int n = 0; n < C::NS; ++n)
@@ -216,18 +234,18 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(const mv_attn_
                 return;
             }
         }
+        if constexpr (masked) {
+#pragma unroll
+            for (int f = 0; f < AHEAD && f < NV; ++f) vf[f] = v_frag(f);
+        }
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int k = 0; k < 2 * C::NS; ++k)
-#pragma unroll
-            for (int b = 0; b < C::NB; ++b) {
-                const lds_t* a = sv + va[b] + 16 * k * C::RS;
-                const short4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)a);
-                const short4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(a + 8 * C::RS));
-                typedef short short8v __attribute__((ext_vector_type(8)));
-                const short8v xy = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-                acc[b] = mfma_32x32x16(__builtin_bit_cast(V8, xy), pf[k], acc[b]);
-            }
+        for (int f = 0; f < NV; ++f) {
+            if constexpr (PINNED) __builtin_amdgcn_sched_barrier(0);
+            acc[f % C::NB] = mfma_32x32x16(vf[f], pf[f / C::NB], acc[f % C::NB]);
+            if (f + AHEAD < NV) vf[f + AHEAD] = v_frag(f + AHEAD);
+        }
+        if constexpr (PINNED) __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_setprio(0);
     };
 
