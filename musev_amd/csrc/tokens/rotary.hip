@@ -105,9 +105,12 @@ extern "C" int mv_rotary_axes(const mv_rotary_desc* d, void* stream) {
     a.per_head = make_div(a.rot_items + (tail + 7) / 8);
     a.per_token = make_div((unsigned)heads * a.per_head.d);
     a.pairs = make_div(d->pairs);
-    MV_REQUIRE(a.per_token.d < 32768, "mv_rotary_axes: %u work items per token (below 32768)", a.per_token.d);   // (div_of's range with 4 tokens)
-    // several tokens per block where there are enough to fill the chip with blocks, one otherwise
-    a.tokens_per_block = d->tokens >= 4096 ? 4 : 1;
+    MV_REQUIRE(a.per_token.d < 32768, "mv_rotary_axes: %u work items per token (below 32768)", a.per_token.d);   // (div_of's range)
+    // As many tokens per block (up to 8) as give its 256 threads two work items each, but at least 1024 blocks.  Measured (us, 1 / 2 / 4 / 8 tokens):
+    // 53 248 tokens of 512 items 147 / 153 / 161 / 165; 26 624 of 160 46.9 / 41.8 / 42.3 / 44.9; 16 384 of 16 10.7 / 6.9 / 5.2 / 4.4; 512 of 320 4.5 /
+    // 5.0 / 6.5 / 10.2.
+    a.tokens_per_block = 1;
+    while (a.tokens_per_block < 8 && a.tokens_per_block * a.per_token.d < 512 && d->tokens >= 1024 * 2 * a.tokens_per_block) a.tokens_per_block *= 2;
     // non-temporal results from 64 MB on: 26 624 tokens x 20 heads x 128 (136 MB) 47.4 -> 42.4 us, 13 312 x 16 x 80 (34 MB) 15.5 -> 20.8
     a.large = d->tokens * heads * d->d * 2 > (64ll << 20);
     const int64_t grid = (d->tokens + a.tokens_per_block - 1) / a.tokens_per_block;
