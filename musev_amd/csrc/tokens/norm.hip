@@ -145,14 +145,16 @@ static void launch_norm(const mv_gated_norm_desc* d, hipStream_t st) {
     gated_norm_kernel<T, NV, WAVES><<<(unsigned)((d->rows + R - 1) / R), 256, 0, st>>>(*d);
 }
 
-// up to 2048 columns a wave holds a row; wider rows take the block's four waves
+// A wave holds a row of up to 1536 columns where there are rows enough to fill the chip; the block's four waves share it otherwise.  Measured (us,
+// rms, both norms, one / four waves per row): 1 x 1280 6.3 / 3.9; 1024 x 1280 7.9 / 5.6; 2048 x 640 6.5 / 6.8; 4099 x 1001 11.3 / 13.1; 16 000 x 1280
+// 37 / 41; 16 000 x 2048 55 / 47.
 template <typename T>
 static void launch_norm_width(const mv_gated_norm_desc* d, hipStream_t st) {
     const int c = d->c;
     if (c <= 512) launch_norm<T, 1, 1>(d, st);
+    else if (c > 1536 ? c <= 2048 : d->rows <= 2048) launch_norm<T, 1, 4>(d, st);
     else if (c <= 1024) launch_norm<T, 2, 1>(d, st);
     else if (c <= 1536) launch_norm<T, 3, 1>(d, st);
-    else if (c <= 2048) launch_norm<T, 4, 1>(d, st);
     else if (c <= 4096) launch_norm<T, 2, 4>(d, st);
     else if (c <= 8192) launch_norm<T, 4, 4>(d, st);
     else launch_norm<T, 8, 4>(d, st);
