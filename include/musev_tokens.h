@@ -97,7 +97,7 @@ typedef struct mv_gemm_i8_desc {
 } mv_gemm_i8_desc;
 int mv_gemm_i8(const mv_gemm_i8_desc* d, void* stream);
 /* both in one call: x [M, K] of the element type; workspace: M * kp bytes of codes and M fp32 scales, 16-byte aligned;
- * not used (null) where M <= 16 and M * kp <= 16384: one launch quantises and multiplies */
+ * not used (null) where M <= 4 and M * kp <= 16384, or M <= 16 and M * kp <= 8192: one launch quantises and multiplies */
 typedef struct mv_linear_i8_desc {
     const void* x;
     const int8_t* w;

@@ -26,10 +26,17 @@ __device__ __forceinline__ int row_code(float x, const RowScale& r) {
 
 // |x| as bits: ordered like the values, NaN above infinity
 __device__ __forceinline__ unsigned abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ unsigned lanes16_max(unsigned v) {
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, false));    // lanes 1 0 3 2 of a quad
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false));    // lanes 2 3 0 1
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, false));   // mirrored within 8
+    return max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, false));   // mirrored within 16
+}
 template <int WAVES>
 __device__ __forceinline__ unsigned row_top(unsigned v, unsigned* red) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o, 64));
+    v = lanes16_max(v);
+    v = max(v, (unsigned)__shfl_xor((int)v, 16, 64));
+    v = max(v, (unsigned)__shfl_xor((int)v, 32, 64));
     if constexpr (WAVES > 1) {
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
         __syncthreads();
@@ -370,11 +377,12 @@ __global__ __launch_bounds__(512) void gemm_i8_few_kernel(const mv_gemm_i8_desc 
     }
 }
 
-// Quantisation and product in one launch, for so few activations that every block can quantise them for itself: M <= 16 rows and at most
-// ONE_LAUNCH codes.  All 512 threads read x (each keeps its elements in registers between the row's maximum and the codes), the codes go to LDS
+// Quantisation and product in one launch, for so few activations that every block can quantise them for itself: up to 16384 codes of up to 4 rows,
+// 8192 of up to 16.  Measured (us of GPU time, one launch / two; a second launch also costs the host 4): 1 x 1280 -> 5120 4.9 / 6.4; 4 x 4096 -> 1280
+// 7.6 / 10.8; 8 x 1024 -> 1280 5.0 / 5.8; 16 x 512 -> 5120 6.8 / 5.5; 16 x 1024 -> 5120 10.2 / 6.8.  All 512 threads read x (each keeps its elements in registers between the row's maximum and the codes), the codes go to LDS
 // and the weights stream as above, their first two units already on their way meanwhile.
 constexpr int ONE_LAUNCH = 16384;
-static bool one_launch(int64_t m, int64_t kp) { return m <= 16 && m * kp <= ONE_LAUNCH; }
+static bool one_launch(int64_t m, int64_t kp) { return m <= 16 && m * kp <= (m <= 4 ? ONE_LAUNCH : ONE_LAUNCH / 2); }
 
 template <typename T>
 __global__ __launch_bounds__(512) void linear_i8_few_kernel(const mv_linear_i8_desc p) {
@@ -402,13 +410,12 @@ __global__ __launch_bounds__(512) void linear_i8_few_kernel(const mv_linear_i8_d
         const int ch = tid + 512 * j, m = ch / per_row, col = (ch - m * per_row) * 8;
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
-        if (ch < total && col < p.K) {
-            load8((const T*)p.x + m * p.ldx + col, p.K - col, v[j]);
-            unsigned top = 0;
+        if (ch < total && col < p.K) load8((const T*)p.x + m * p.ldx + col, p.K - col, v[j]);
+        unsigned top = 0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) top = max(top, abs_bits(v[j][e]));
-            atomicMax(&tops[m], top);   // (a maximum does not depend on the order)
-        }
+        for (int e = 0; e < 8; ++e) top = max(top, abs_bits(v[j][e]));
+        top = lanes16_max(top);   // (16 lanes are of one row: kp is a multiple of 128)
+        if (l15 == 0 && ch < total) atomicMax(&tops[m], top);   // (a maximum does not depend on the order)
     }
     __syncthreads();
 #pragma unroll

@@ -468,6 +468,9 @@ def pack_weight_i8(codes: torch.Tensor, scale: torch.Tensor) -> Int8Rows:
     return Int8Rows(packed, scale.clone(memory_format=torch.contiguous_format), k)
 
 
+_ONE_LAUNCH = 16384   # codes of up to 4 rows (half as many of up to 16) that mv_linear_i8 takes in one launch, without a workspace
+
+
 def quantize_rows_i8(x: torch.Tensor) -> Int8Rows:
     """Each row of ``x`` [M, K] (fp16 | bf16) as int8 codes and one scale: scale = max|x| / 127, code = 127 x / max|x| rounded to nearest, ties
     to even.  A row of zeros has scale 0; a row that holds an infinity or NaN keeps that as its scale (its products are NaN)."""
@@ -539,7 +542,7 @@ def linear_i8(x: torch.Tensor, w: Int8Rows, *, bias: Optional[torch.Tensor] = No
     if given:
         _no_overlap(out, "linear_i8: out", (("x", x),))
     # mv_linear_i8's workspace: the rows' codes, then their scales; none where it quantises and multiplies in one launch
-    ws = None if m <= 16 and m * w.kp <= 16384 else torch.empty(m * (w.kp + 4), dtype=torch.uint8, device=x.device)
+    ws = None if m <= 16 and m * w.kp <= (_ONE_LAUNCH if m <= 4 else _ONE_LAUNCH // 2) else torch.empty(m * (w.kp + 4), dtype=torch.uint8, device=x.device)
     _launch("mv_linear_i8", _pack_linear(x.data_ptr(), w._codes, w._scale, pb, pr, po, ws.data_ptr() if ws is not None else 0, m, w.rows, k, w.kp, ldx, w.kp, ldr, ldo, act,
                                          _DTYPES[dtype]), x.get_device(), (w,))
     return out
