@@ -1,7 +1,7 @@
 """Token-transformer operators over the C ABI of include/musev_tokens.h: packed attention, rotary positions with several axes, the gated
 residual norm and the int8 projection.  They are part of :mod:`musev_amd.ops` (``from musev_amd import ops; ops.attention_packed(...)``)
 and follow its manner: 2-D row matrices with unit inner stride, no CPU path, launches on the current stream of the tensors' device.
-fp16 and bf16; forward only, like the rest of the framework.
+fp16 and bf16; forward only, like the rest of the framework: a tensor that requires gradients is refused while gradients are recorded.
 
 Each call reads its tensors on the stream it is made on: a tensor made on another stream has to be finished there first.  Nothing is kept
 between calls; what a call needs besides its arguments is allocated for that call (inside a graph capture: from the capture's pool), so
@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import operator
 import struct
 from typing import Callable, List, Optional, Sequence, Tuple, Union
 
@@ -61,6 +62,11 @@ def _launch(entry: str, desc: bytes, dev: int, held: Sequence["_Held"] = ()) -> 
         check(status, entry)
 
 
+def _no_gradients(name: str) -> None:
+    if torch.is_grad_enabled():
+        raise ValueError(f"{name}: requires gradients, and this operator has none to give: call it under torch.no_grad() or detach the tensor")
+
+
 def _matrix(t: torch.Tensor, name: str, dtype: Optional[torch.dtype] = None, dev: Optional[int] = None) -> Tuple[int, int, int]:
     """(rows, columns, row stride) of a 2-D tensor with unit inner stride on the GPU; a single row has no stride of its own: its width stands in"""
     if not isinstance(t, torch.Tensor) or t.ndim != 2:
@@ -72,6 +78,8 @@ def _matrix(t: torch.Tensor, name: str, dtype: Optional[torch.dtype] = None, dev
         raise ValueError(f"{name}: expected a CUDA {'fp16 | bf16' if dtype is None else dtype} tensor, got {t.dtype} on {t.device}")
     if dev is not None and t.get_device() != dev:
         raise ValueError(f"{name}: on {t.device}, the other tensors are on device {dev}")
+    if t.requires_grad:
+        _no_gradients(name)
     if rows <= 1:
         return rows, cols, cols
     if ld < cols or ld > _I32_MAX:
@@ -150,7 +158,7 @@ def _lens(v, name: str) -> List[int]:
         if v.is_cuda:
             raise ValueError(f"{name}: lengths are host integers (reading them from the GPU would wait for it)")
         v = v.tolist()
-    v = [int(x) for x in v]
+    v = [operator.index(x) for x in v]
     if not v or min(v) < 0 or sum(v) > _I32_MAX:
         raise ValueError(f"{name}: expected at least one length, none negative, at most 2^31 - 1 rows in all")
     return v
@@ -351,6 +359,8 @@ def _affine(t: Optional[torch.Tensor], name: str, c: int, dtype: torch.dtype, de
         return 0
     if t.dtype != dtype or t.get_device() != dev or not t.is_contiguous() or t.numel() != c:
         raise ValueError(f"{name}: expected a contiguous {dtype} tensor of {c} elements on device {dev}")
+    if t.requires_grad:
+        _no_gradients(name)
     return t.data_ptr()
 
 
@@ -500,9 +510,7 @@ def _i8_result(what: str, m: int, w: Int8Rows, like: torch.Tensor, dtype, bias, 
         raise ValueError(f"{what}: a weight without rows")
     pb = pr = ldr = 0
     if bias is not None:
-        if bias.dtype != dtype or bias.get_device() != dev or not bias.is_contiguous() or bias.numel() != n:
-            raise ValueError(f"{what}: bias must be a contiguous {dtype} tensor of {n} elements on {like.device}")
-        pb = bias.data_ptr()
+        pb = _affine(bias, f"{what}: bias", n, dtype, dev)
     if residual is not None:
         rows, cols, ldr = _matrix(residual, "residual", dtype, dev)
         if rows != m or cols != n:

@@ -203,6 +203,15 @@ def test_tensors_off_the_gpu_are_refused():
             call()
 
 
+def test_plan_takes_integers_only():
+    import numpy as np
+    from musev_amd import ops
+    ok = dict(heads=2, d=64, device="cpu")
+    assert ops.attention_plan(np.array([3, 4]), torch.tensor([5, 6]), **ok).kv_lens == (5, 6)
+    with pytest.raises(TypeError):
+        ops.attention_plan([3.5], **ok)
+
+
 @pytest.fixture
 def on_cpu(monkeypatch):
     """argument checks alone: CPU tensors pass for device memory and no launch may follow"""
@@ -238,6 +247,23 @@ def test_refusals_of_attention(on_cpu):
                             ((big[:, 4:68], kv, kv), {}, "16"), ((q, kv, kv), {"out": torch.zeros(8, 300, dtype=torch.float16)[:, 8:72]}, "16"), ((q, torch.zeros(8, 36, dtype=torch.float16)[:, :32], kv), {}, "16")):
         with pytest.raises(ValueError, match=match):
             ops.attention_packed(plan, *args, **kw)
+
+
+def test_tensors_that_require_gradients_are_refused(on_cpu):
+    from musev_amd import ops
+    x = torch.zeros(6, 64, dtype=torch.float16)
+    p = torch.zeros(64, dtype=torch.float16, requires_grad=True)
+    r = torch.zeros(6, 64, dtype=torch.float16, requires_grad=True)
+    plan, table = ops.attention_plan([6], heads=1, d=64, device="cpu"), ops.rotary_table([64], device="cpu")
+    w = ops.Int8Rows(torch.zeros(64, 128, dtype=torch.int8), torch.ones(64), 64)
+    pos = torch.zeros(6, 1)
+    for call in (lambda: ops.attention_packed(plan, x, r, x), lambda: ops.rotary_axes(r, None, pos, table, heads=1, d=64),
+                 lambda: ops.gated_residual_norm(x, r), lambda: ops.gated_residual_norm(x, x, pre=(p, None, 1e-6)), lambda: ops.linear_i8(r, w),
+                 lambda: ops.linear_i8(x, w, bias=p)):
+        with pytest.raises(ValueError, match="gradients"):
+            call()
+        with torch.no_grad(), pytest.raises(on_cpu):
+            call()
 
 
 def test_refusals_of_rotary(on_cpu):
@@ -810,6 +836,38 @@ def test_linear_i8_extreme_codes_zero_and_nonfinite_rows(m):
         rows[2:4] = False
         assert bool(torch.isnan(got[2:4]).all())
     within(got[rows], want[rows], half_step(dt) * want[rows].abs() + 2.0 ** -20 * want[rows])
+
+
+@gpu
+def test_no_rows():
+    from musev_amd import ops
+    w = ops.pack_weight_i8(torch.ones(8, 40, dtype=torch.int8, device=DEV), torch.ones(8, device=DEV))
+    for dt in DTYPES:
+        x = torch.empty(0, 40, dtype=dt, device=DEV)
+        assert ops.linear_i8(x, w).shape == (0, 8) and ops.quantize_rows_i8(x).codes.shape == (0, 128)
+        assert ops.gemm_i8(ops.quantize_rows_i8(x), w, dtype=dt).shape == (0, 8)
+        assert ops.rotary_axes(x, None, torch.empty(0, 1, device=DEV), ops.rotary_table([40]), heads=1, d=40)[0].shape == (0, 40)
+
+
+@gpu
+@pytest.mark.parametrize("m", [1, 20, 200])
+def test_linear_of_columns_of_a_wide_matrix(m):
+    """x a column slice with an odd offset, the result another matrix's slice, two results side by side"""
+    from musev_amd import ops
+    dt, k, n = torch.bfloat16, 300, 133
+    big = rnd((m, k + 9), 5, dt)
+    x = big[:, 3:3 + k]
+    g = torch.Generator().manual_seed(6)
+    codes = torch.randint(-127, 128, (n, k), generator=g, dtype=torch.int32).to(torch.int8).to(DEV)
+    ws = torch.full((n,), 0.01, device=DEV)
+    w = ops.pack_weight_i8(codes.t().contiguous().t(), ws)     # (any strides)
+    wide = torch.zeros(m, 2 * n, dtype=dt, device=DEV)
+    ops.linear_i8(x, w, out=wide[:, :n])
+    ops.linear_i8(x, w, out=wide[:, n:], residual=wide[:, :n])
+    torch.cuda.synchronize()
+    want, bound = linear_oracle(x.contiguous(), codes, ws, None, None, False)
+    within(wide[:, :n], want, bound)
+    within(wide[:, n:], *linear_oracle(x.contiguous(), codes, ws, None, wide[:, :n], False))
 
 
 # ---- together, on other streams, in graphs ----------------------------------------------------------------------------------------------
