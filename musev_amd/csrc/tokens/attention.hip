@@ -129,7 +129,7 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(const mv_attn_
         constexpr bool masked = decltype(tag)::value;   // some row may not see all of the tile
         // At two waves per SIMD (head dims from 65 on) fragments are read AHEAD matrix instructions before they are used and the order is pinned:
         // left to itself the compiler reads each just before its use and the matrix pipe waits out the LDS latency (d = 128, a causal prompt of 16384:
-        // 1.07 -> 1.02 ms).  With more waves the others cover it and the compiler's own order is as good (d = 64, 8192 tokens: 168 against 171 us).
+        // 1.04 -> 1.00 ms).  With more waves the others cover it and the compiler's own order is as good (d = 64, 8192 tokens: 166 against 171 us).
         constexpr bool PINNED = K16 > 4;
         const lds_t* sv = ring + stage * 2 * C::TILE + C::TILE;
         const unsigned kb = (unsigned)(uintptr_t)(ring + stage * 2 * C::TILE) + ka, vb = (unsigned)(uintptr_t)sv + va;

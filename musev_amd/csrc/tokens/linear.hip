@@ -123,30 +123,32 @@ extern "C" int mv_quantize_rows_i8(const void* x, int64_t ldx, int64_t rows, int
 typedef int int4v __attribute__((ext_vector_type(4)));
 typedef int int16v __attribute__((ext_vector_type(16)));
 
-// Tiles through LDS: BM rows of activations x BN rows of weights, BK bytes of K per step, NST stages of which NST - 1 are in flight, every
-// wave WM x WN of the result in v_mfma_i32_32x32x32_i8 blocks (weights as the first operand: a lane holds 4 consecutive outputs of one
-// row).  LDS rows are BK bytes = SLOTS slots of 16; 256 / BK rows share a 256-byte line of banks, so the slots of a row are permuted by the
-// line's number and a fragment read (16 rows, one slot) touches every bank once.  The permutation is applied to the column each lane
-// fetches (global -> LDS directly).
+// Tiles through LDS: BM rows of activations x BN rows of weights, 128 bytes of K per step, two stages (one computed on, one on its way; three
+// or four stages of 64 or 128 bytes were no faster), every wave WM x WN of the result in v_mfma_i32_32x32x32_i8 blocks (weights as the first
+// operand: a lane holds 4 consecutive outputs of one row).  LDS rows are 128 bytes = 8 slots of 16 and two rows share a 256-byte line of banks, so
+// the slots of a row are permuted by the line's number and a fragment read (16 rows, one slot) touches every bank once.  The permutation is
+// applied to the column each lane fetches (global -> LDS directly).
 // KS groups of waves share a block's tile and take the steps of K in turn, each with stages of its own: where a product has fewer tiles than
 // there are CUs and a long K, the latency of its steps is what it costs.  The groups' sums meet in LDS.
-template <int BM, int BN, int WM, int WN, int BK, int NST, int KS>
+constexpr int BK = 128;
+
+template <int BM, int BN, int WM, int WN, int KS>
 struct GemmI8Cfg {
     static constexpr int WAVES = (BM / WM) * (BN / WN), THREADS = 64 * WAVES * KS;
     static constexpr int SLOTS = BK / 16, PROWS = 1024 / BK;            // slots of a row; rows of a 1-KiB piece
     static constexpr int STAGE = (BM + BN) * BK;
     static constexpr int PA = BM / PROWS / WAVES, PW = BN / PROWS / WAVES;   // pieces a wave fetches of each tile
-    static constexpr int SROW = WN + 4;                                 // ints per row of the result staging
+    static constexpr int SROW = WN + 4;                                 // floats per row of the result staging
     static constexpr int STAGING = WAVES * 32 * SROW * 4, SUMS = WM * WN * 4;   // bytes; of a wave's sums
     static constexpr int AFTER = STAGING + (KS - 1) * WAVES * SUMS;
-    static constexpr int LDS = KS * NST * STAGE > AFTER ? KS * NST * STAGE : AFTER;
+    static constexpr int LDS = KS * 2 * STAGE > AFTER ? KS * 2 * STAGE : AFTER;
     static_assert(BM % (PROWS * WAVES) == 0 && BN % (PROWS * WAVES) == 0, "every wave fetches whole pieces");
     static __device__ __forceinline__ int swz(int row) { return (row / (256 / BK)) % SLOTS; }
 };
 
-template <typename T, int BM, int BN, int WM, int WN, int BK, int NST, int KS>
-__global__ __launch_bounds__((GemmI8Cfg<BM, BN, WM, WN, BK, NST, KS>::THREADS), 2) void gemm_i8_kernel(const mv_gemm_i8_desc p, const int tiles_m, const int tiles_n) {
-    using C = GemmI8Cfg<BM, BN, WM, WN, BK, NST, KS>;
+template <typename T, int BM, int BN, int WM, int WN, int KS>
+__global__ __launch_bounds__((GemmI8Cfg<BM, BN, WM, WN, KS>::THREADS), 2) void gemm_i8_kernel(const mv_gemm_i8_desc p, const int tiles_m, const int tiles_n) {
+    using C = GemmI8Cfg<BM, BN, WM, WN, KS>;
     typedef __attribute__((address_space(3))) char lds_c;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     lds_c* const lds = (lds_c*)smem;
@@ -175,7 +177,7 @@ __global__ __launch_bounds__((GemmI8Cfg<BM, BN, WM, WN, BK, NST, KS>::THREADS), 
         ow[j] = (unsigned)(row * p.ldw + ((pslot ^ C::swz(row)) << 4));
     }
     auto issue = [&](int k, int stage) __attribute__((always_inline)) {
-        lds_c* dst = lds + (kg * NST + stage) * C::STAGE;
+        lds_c* dst = lds + (kg * 2 + stage) * C::STAGE;
 #pragma unroll
         for (int j = 0; j < C::PA; ++j)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void*)(dst + (wave * C::PA + j) * 1024), 16, (int)oa[j], k, 0, 0);
@@ -215,41 +217,45 @@ __global__ __launch_bounds__((GemmI8Cfg<BM, BN, WM, WN, BK, NST, KS>::THREADS), 
     const bool early = p.residual && kg == 0 && p.kp > KS * BK && p.N >= 8;
 
     const int steps = p.kp / BK, turns = (steps + KS - 1) / KS;   // this group's steps: kg, kg + KS, ...; the first group has one every turn
-    int into = 0, from = 0;
-#pragma unroll
-    for (int s = 0; s < NST - 1; ++s)
-        if (s * KS + kg < steps) issue((s * KS + kg) * BK, into++);
+    if (kg < steps) issue(kg * BK, 0);
 #pragma unroll 1
     for (int t = 0; t < turns; ++t) {
-        // this wave's share of the step has landed ... (younger steps may be on their way)
+        // this wave's share of the step has landed ...
         if (t + 1 == turns && early) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(FIRST) : "memory");   // (the residual's loads are the youngest)
-        else if (NST > 2 && (t + NST - 2) * KS + kg < steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * (C::PA + C::PW)) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();                      // ... and everyone's; everyone has left the stage of the step before
         asm volatile("" ::: "memory");
-        if ((t + NST - 1) * KS + kg < steps) issue(((t + NST - 1) * KS + kg) * BK, into);
+        if ((t + 1) * KS + kg < steps) issue(((t + 1) * KS + kg) * BK, (t + 1) & 1);
         if (t + 2 == turns && early) {
             asm volatile("" ::: "memory");   // (behind the last stage's loads)
 #pragma unroll
             for (int x = 0; x < FIRST; ++x) res[x] = residual_at(x);
             asm volatile("" ::: "memory");
         }
-        into = into + 1 == NST ? 0 : into + 1;
         if (KS > 1 && t * KS + kg >= steps) break;   // (the last turn: this group has no step left, nor a barrier)
-        const lds_c* sa = lds + (kg * NST + from) * C::STAGE + wm * BK;
-        const lds_c* sw = lds + (kg * NST + from) * C::STAGE + BM * BK + wn * BK;
-        from = from + 1 == NST ? 0 : from + 1;
+        const lds_c* sa = lds + (kg * 2 + (t & 1)) * C::STAGE + wm * BK;
+        const lds_c* sw = lds + (kg * 2 + (t & 1)) * C::STAGE + BM * BK + wn * BK;
+        // the next quarter's fragments (small tiles: the whole step's) are read before this quarter's matrix instructions, in pinned order: left to
+        // itself the compiler reads them just before their use and the matrix pipe waits out the LDS latency
+        int4v fa[4][WM / 32], fw[4][WN / 32];
+        auto read = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
-        for (int s = 0; s < BK / 32; ++s) {
-            int4v fa[WM / 32], fw[WN / 32];
+            for (int i = 0; i < WM / 32; ++i) fa[s][i] = *(const __attribute__((address_space(3))) int4v*)(sa + i * 32 * BK + fo[s]);
 #pragma unroll
-            for (int i = 0; i < WM / 32; ++i) fa[i] = *(const __attribute__((address_space(3))) int4v*)(sa + i * 32 * BK + fo[s]);
+            for (int j = 0; j < WN / 32; ++j) fw[s][j] = *(const __attribute__((address_space(3))) int4v*)(sw + j * 32 * BK + fo[s]);
+        };
+        constexpr int AHEAD = WM * WN > 64 * 32 ? 1 : 3;
 #pragma unroll
-            for (int j = 0; j < WN / 32; ++j) fw[j] = *(const __attribute__((address_space(3))) int4v*)(sw + j * 32 * BK + fo[s]);
+        for (int s = 0; s < AHEAD; ++s) read(s);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            if (s + AHEAD < 4) read(s + AHEAD);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < WM / 32; ++i)
 #pragma unroll
-                for (int j = 0; j < WN / 32; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[j], fa[i], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < WN / 32; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[s][j], fa[s][i], acc[i][j], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
     if (early) {
@@ -445,10 +451,10 @@ __global__ __launch_bounds__(512) void linear_i8_few_kernel(const mv_linear_i8_d
     ((T*)p.out)[m * p.ldo + n] = (T)r;
 }
 
-template <typename T, int BM, int BN, int WM, int WN, int BK, int NST, int KS>
+template <typename T, int BM, int BN, int WM, int WN, int KS>
 static int launch_gemm_i8(const mv_gemm_i8_desc* d, hipStream_t st) {
-    using C = GemmI8Cfg<BM, BN, WM, WN, BK, NST, KS>;
-    const auto kernel = gemm_i8_kernel<T, BM, BN, WM, WN, BK, NST, KS>;
+    using C = GemmI8Cfg<BM, BN, WM, WN, KS>;
+    const auto kernel = gemm_i8_kernel<T, BM, BN, WM, WN, KS>;
     const int64_t tm = (d->M + BM - 1) / BM, tn = (d->N + BN - 1) / BN;
     MV_REQUIRE(tm * tn < (1ll << 31), "mv_gemm_i8: %ld x %ld tiles", (long)tm, (long)tn);
     if (C::LDS > 64 * 1024) {
@@ -480,11 +486,11 @@ static int launch_gemm_i8_shape(const mv_gemm_i8_desc* d, hipStream_t st) {
     // 385 / - / -; 4096 x 1280 x 2560 26.8 / 24.8 / 31.5 / - / -; 2048 x 1280 x 1280 22.5 / 10.5 / 10.2 / - / -; 512 x 5120 x 1280 - / 22.9 / 19.8 /
     // 13.7 / 16.5; 512 x 1280 x 1280 - / 8.3 / 6.7 / 7.0 / 9.1; 300 x 5120 x 1280 - / 19.1 / 14.0 / 11.9 / 10.6; 64 x 1280 x 1280 - / 8.3 / 6.5 / 6.7 / 5.2.
     const auto tiles = [&](int64_t bm, int64_t bn) { return ((d->M + bm - 1) / bm) * ((d->N + bn - 1) / bn); };
-    if (tiles(256, 256) >= 1024) return launch_gemm_i8<T, 256, 256, 128, 64, 128, 2, 1>(d, st);
-    if (tiles(128, 64) >= 512) return launch_gemm_i8<T, 128, 64, 64, 32, 128, 2, 1>(d, st);
-    if (tiles(32, 32) <= 512) return launch_gemm_i8<T, 32, 32, 32, 32, 128, 2, 4>(d, st);
-    if (tiles(64, 64) <= 256 && d->kp >= 2048) return launch_gemm_i8<T, 64, 64, 32, 32, 128, 2, 4>(d, st);
-    return launch_gemm_i8<T, 64, 64, 32, 32, 128, 2, 1>(d, st);
+    if (tiles(256, 256) >= 1024) return launch_gemm_i8<T, 256, 256, 128, 64, 1>(d, st);
+    if (tiles(128, 64) >= 512) return launch_gemm_i8<T, 128, 64, 64, 32, 1>(d, st);
+    if (tiles(32, 32) <= 512) return launch_gemm_i8<T, 32, 32, 32, 32, 4>(d, st);
+    if (tiles(64, 64) <= 256 && d->kp >= 2048) return launch_gemm_i8<T, 64, 64, 32, 32, 4>(d, st);
+    return launch_gemm_i8<T, 64, 64, 32, 32, 1>(d, st);
 }
 
 extern "C" int mv_gemm_i8(const mv_gemm_i8_desc* d, void* stream) {
