@@ -471,8 +471,8 @@ static int launch_gemm_i8(const mv_gemm_i8_desc* d, hipStream_t st) {
 
 template <typename T>
 static int launch_gemm_i8_shape(const mv_gemm_i8_desc* d, hipStream_t st) {
-    // Up to 32 rows of a short K: the weight stream (us, stream / 32 x 32 tiles: 16 x 1280 x 5120 4.5 / 5.0; 20 x 640 x 640 3.2 / 4.7; from K =
-    // 2048 on its waves' turns add up, 32 x 5120 x 5120 16.1 / 8.5).
+    // Up to 32 rows of a short K: the weight stream (us, stream / 32 x 32 tiles: 16 x 1280 x 5120 4.5 / 4.9; 20 x 640 x 640 3.1 / 4.6; 32 x 2048 x 2048
+    // 5.0 / 5.5; beyond, its waves' turns add up: 32 x 5120 x 5120 16.4 / 8.2).
     if (d->M <= 32 && d->kp <= 2048) {
         const unsigned grid = (d->N + 15) / 16;
         if (d->M <= 16) gemm_i8_few_kernel<T, 1><<<grid, 512, 0, st>>>(*d);
@@ -482,9 +482,10 @@ static int launch_gemm_i8_shape(const mv_gemm_i8_desc* d, hipStream_t st) {
     }
     // The largest tile that still gives every CU a few blocks: 256 x 256 (one block per CU) from four rounds on, 128 x 64 (three per CU) from two
     // blocks per CU, 64 x 64 below, where K is long and tiles are few in four groups, and 32 x 32 in four groups up to two per CU.
-    // Measured (us, M x K x N; 256 / 128 x 64 / 64 / 64 in groups / 32 in groups): 8192^3 475 / 661 / - / - / -; 26 624 x 1280 x 5120 270 / 312 /
-    // 385 / - / -; 4096 x 1280 x 2560 26.8 / 24.8 / 31.5 / - / -; 2048 x 1280 x 1280 22.5 / 10.5 / 10.2 / - / -; 512 x 5120 x 1280 - / 22.9 / 19.8 /
-    // 13.7 / 16.5; 512 x 1280 x 1280 - / 8.3 / 6.7 / 7.0 / 9.1; 300 x 5120 x 1280 - / 19.1 / 14.0 / 11.9 / 10.6; 64 x 1280 x 1280 - / 8.3 / 6.5 / 6.7 / 5.2.
+    // Measured (us, M x K x N; 256 / 128 x 64 / 64 / 64 in groups / 32 in groups): 8192^3 472 / 655 / 799 / - / -; 26 624 x 1280 x 5120 249 / 315 /
+    // 380 / 792 / -; 4096 x 1280 x 2560 27.2 / 25.1 / 32.8 / 62 / -; 2048 x 1280 x 1280 22.9 / 10.3 / 10.8 / 18.4 / 22.6; 512 x 5120 x 1280 60 / 23.0 /
+    // 19.8 / 13.9 / 16.3; 512 x 1280 x 1280 22.5 / 8.4 / 6.6 / 7.1 / 9.1; 300 x 5120 x 1280 61 / 19.3 / 14.0 / 11.8 / 10.8; 64 x 1280 x 1280 20 / 8.2 /
+    // 6.4 / 6.8 / 5.1.
     const auto tiles = [&](int64_t bm, int64_t bn) { return ((d->M + bm - 1) / bm) * ((d->N + bn - 1) / bn); };
     if (tiles(256, 256) >= 1024) return launch_gemm_i8<T, 256, 256, 128, 64, 1>(d, st);
     if (tiles(128, 64) >= 512) return launch_gemm_i8<T, 128, 64, 64, 32, 1>(d, st);
