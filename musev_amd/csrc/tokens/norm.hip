@@ -20,7 +20,7 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
 // block.  Both norms' statistics are formed in two passes over the registers (mean, then squared deviations), in fp32.  Bound by memory:
 // x and f in, s and h out.
 template <typename T, int NV, int WAVES>
-__global__ __launch_bounds__(256) void gated_norm_kernel(const mv_gated_norm_desc p) {
+__global__ __launch_bounds__(256) void gated_norm_kernel(const mv_gated_norm_desc p, const bool cold) {
     __shared__ float red[4];
     constexpr int LANES = 64 * WAVES;
     const int lane = threadIdx.x % LANES, c = p.c;
@@ -43,8 +43,8 @@ __global__ __launch_bounds__(256) void gated_norm_kernel(const mv_gated_norm_des
     for (int j = 0; j < NV; ++j) {
         const int col = (j * LANES + lane) * 8;
         if (col < c) {
-            load8(f + col, c - col, y[j]);
-            load8(x + col, c - col, s[j]);
+            load8_from(f + col, c - col, y[j], cold);
+            load8_from(x + col, c - col, s[j], cold);
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[j][e] = s[j][e] = 0.f;
@@ -142,7 +142,9 @@ __global__ __launch_bounds__(256) void gated_norm_kernel(const mv_gated_norm_des
 template <typename T, int NV, int WAVES>
 static void launch_norm(const mv_gated_norm_desc* d, hipStream_t st) {
     constexpr int R = 4 / WAVES;
-    gated_norm_kernel<T, NV, WAVES><<<(unsigned)((d->rows + R - 1) / R), 256, 0, st>>>(*d);
+    // (53 248 x 1280, 273 MB of inputs: 123 -> 113 us where other work ran in between; 26 624 x 1280, half of that and still in the cache: 57 -> 65)
+    const bool cold = d->rows * d->c * 4 > COLD_BYTES;
+    gated_norm_kernel<T, NV, WAVES><<<(unsigned)((d->rows + R - 1) / R), 256, 0, st>>>(*d, cold);
 }
 
 // A wave holds a row of up to 1536 columns where there are rows enough to fill the chip; the block's four waves share it otherwise.  Measured (us,

@@ -19,7 +19,7 @@ struct RotaryArgs {
     mv_rotary_desc p;
     Div per_token, per_head, pairs;   // work items of a token, of a head
     int rot_items, tokens_per_block;  // items of a head that turn (the others copy what passes through)
-    bool large;                       // results past the caches
+    bool large, cold;                 // results, inputs past the caches
 };
 
 // A block owns a few tokens: their sines and cosines go to LDS once, shared by all heads, then every thread takes work items of 8 elements
@@ -62,8 +62,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
         if constexpr (HALVES) {
             const int pr = (int)e * 8, n = p.pairs - pr;
             float u[8], w[8];
-            load8(in + pr, n, u);
-            load8(in + p.pairs + pr, n, w);
+            load8_from(in + pr, n, u, a.cold);
+            load8_from(in + p.pairs + pr, n, w, a.cold);
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
                 const float2 sc = tr[min(pr + x, p.pairs - 1)];
@@ -76,7 +76,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a) {
         } else {
             const int pr = (int)e * 4, n = 2 * (p.pairs - pr);
             float u[8];
-            load8(in + 2 * pr, n, u);
+            load8_from(in + 2 * pr, n, u, a.cold);
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const float2 sc = tr[min(pr + x, p.pairs - 1)];
@@ -113,6 +113,7 @@ extern "C" int mv_rotary_axes(const mv_rotary_desc* d, void* stream) {
     while (a.tokens_per_block < 8 && a.tokens_per_block * a.per_token.d < 512 && d->tokens >= 1024 * 2 * a.tokens_per_block) a.tokens_per_block *= 2;
     // non-temporal results from 64 MB on: 26 624 tokens x 20 heads x 128 (136 MB) 47.4 -> 42.4 us, 13 312 x 16 x 80 (34 MB) 15.5 -> 20.8
     a.large = d->tokens * heads * d->d * 2 > (64ll << 20);
+    a.cold = d->tokens * heads * d->d * 2 > COLD_BYTES;   // (53 248 x 32 heads x 128: 146 -> 143 us)
     const int64_t grid = (d->tokens + a.tokens_per_block - 1) / a.tokens_per_block;
     MV_REQUIRE(grid < (1ll << 31), "mv_rotary_axes: %ld tokens", (long)d->tokens);
     const size_t lds = (size_t)a.tokens_per_block * d->pairs * sizeof(float2);

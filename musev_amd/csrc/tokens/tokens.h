@@ -48,7 +48,18 @@ __device__ __forceinline__ void store8(T* p, int n, const float* in) {
             if (e < n) p[e] = v[e];
 }
 
-// the same for a result that the caches need not keep for this kernel (non-temporal: 13 312 x 1280 x 4 streams of the gated norm 130 -> 112 us)
+// load8 past the caches: for inputs that they cannot hold (`cold`, uniform)
+template <typename T>
+__device__ __forceinline__ void load8_from(const T* p, int n, float* out, bool cold) {
+    if (cold && n >= 8) {
+        const typename Vec8<T>::type v = __builtin_bit_cast(typename Vec8<T>::type, __builtin_nontemporal_load((const typename Loose8<T>::anywhere*)p));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) out[e] = (float)v[e];
+    } else load8(p, n, out);
+}
+constexpr int64_t COLD_BYTES = 256ll << 20;   // the last-level cache
+
+// store8 of a result that the caches need not keep for this kernel (non-temporal: 13 312 x 1280 x 4 streams of the gated norm 130 -> 112 us)
 template <typename T>
 __device__ __forceinline__ void store8_stream(T* p, int n, const float* in) {
     typedef typename Vec8<T>::type V;
