@@ -146,7 +146,7 @@ struct GemmI8Cfg {
     static __device__ __forceinline__ int swz(int row) { return (row / (256 / BK)) % SLOTS; }
 };
 
-template <typename T, int BM, int BN, int WM, int WN, int KS>
+template <typename T, int BM, int BN, int WM, int WN, int KS, bool COLD>
 __global__ __launch_bounds__((GemmI8Cfg<BM, BN, WM, WN, KS>::THREADS), 2) void gemm_i8_kernel(const mv_gemm_i8_desc p, const int tiles_m, const int tiles_n) {
     using C = GemmI8Cfg<BM, BN, WM, WN, KS>;
     typedef __attribute__((address_space(3))) char lds_c;
@@ -212,6 +212,8 @@ __global__ __launch_bounds__((GemmI8Cfg<BM, BN, WM, WN, KS>::THREADS), 2) void g
     V8 res[NRES];
     auto residual_at = [&](int x) __attribute__((always_inline)) {
         const T* r = (const T*)p.residual + min(m0 + wm + 32 * (x / PASSES) + (x % PASSES) * RPP + frow, p.M - 1) * p.ldr + min(n, p.N - 8);
+        if constexpr (COLD)   // (a residual that the last-level cache cannot hold)
+            return __builtin_bit_cast(V8, __builtin_nontemporal_load((const typename Loose8<T>::anywhere*)r));
         return __builtin_bit_cast(V8, ((const typename Loose8<T>::bytes*)r)->v);
     };
     const bool early = p.residual && kg == 0 && p.kp > KS * BK && p.N >= 8;
@@ -451,10 +453,10 @@ __global__ __launch_bounds__(512) void linear_i8_few_kernel(const mv_linear_i8_d
     ((T*)p.out)[m * p.ldo + n] = (T)r;
 }
 
-template <typename T, int BM, int BN, int WM, int WN, int KS>
+template <typename T, int BM, int BN, int WM, int WN, int KS, bool COLD = false>
 static int launch_gemm_i8(const mv_gemm_i8_desc* d, hipStream_t st) {
     using C = GemmI8Cfg<BM, BN, WM, WN, KS>;
-    const auto kernel = gemm_i8_kernel<T, BM, BN, WM, WN, KS>;
+    const auto kernel = gemm_i8_kernel<T, BM, BN, WM, WN, KS, COLD>;
     const int64_t tm = (d->M + BM - 1) / BM, tn = (d->N + BN - 1) / BN;
     MV_REQUIRE(tm * tn < (1ll << 31), "mv_gemm_i8: %ld x %ld tiles", (long)tm, (long)tn);
     if (C::LDS > 64 * 1024) {
@@ -487,7 +489,10 @@ static int launch_gemm_i8_shape(const mv_gemm_i8_desc* d, hipStream_t st) {
     // 19.8 / 13.9 / 16.3; 512 x 1280 x 1280 22.5 / 8.4 / 6.6 / 7.1 / 9.1; 300 x 5120 x 1280 61 / 19.3 / 14.0 / 11.8 / 10.8; 64 x 1280 x 1280 20 / 8.2 /
     // 6.4 / 6.8 / 5.1.
     const auto tiles = [&](int64_t bm, int64_t bn) { return ((d->M + bm - 1) / bm) * ((d->N + bn - 1) / bn); };
-    if (tiles(256, 256) >= 1024) return launch_gemm_i8<T, 256, 256, 128, 64, 1>(d, st);
+    // A residual past the last-level cache is read non-temporally (272 MB, 26 624 x 1280 -> 5120 with the quantisation: 280 -> 272 us; 136 MB, 6656 x 1280
+    // -> 10240 and still in the cache: 129.5 -> 132).
+    if (tiles(256, 256) >= 1024)
+        return d->residual && d->M * d->N * 2 > COLD_BYTES ? launch_gemm_i8<T, 256, 256, 128, 64, 1, true>(d, st) : launch_gemm_i8<T, 256, 256, 128, 64, 1>(d, st);
     if (tiles(128, 64) >= 512) return launch_gemm_i8<T, 128, 64, 64, 32, 1>(d, st);
     if (tiles(32, 32) <= 512) return launch_gemm_i8<T, 32, 32, 32, 32, 4>(d, st);
     if (tiles(64, 64) <= 256 && d->kp >= 2048) return launch_gemm_i8<T, 64, 64, 32, 32, 4>(d, st);

@@ -815,6 +815,25 @@ def test_linear_i8(mkn, dt):
 
 
 @gpu
+@pytest.mark.parametrize("m,k,n,dt", [(8200, 300, 8197, torch.float16), (26624, 200, 5121, torch.bfloat16)], ids=["ragged", "residual_past_the_cache"])
+def test_linear_i8_large(m, k, n, dt):
+    """the largest tiles, ragged on every side"""
+    from musev_amd import ops
+    x = rnd((m, k), 1, dt)
+    g = torch.Generator().manual_seed(2)
+    codes = torch.randint(-127, 128, (n, k), generator=g, dtype=torch.int32).to(torch.int8).to(DEV)
+    ws = ((0.5 + torch.rand(n, generator=g)) / (73 * math.sqrt(k))).to(DEV)
+    bias, w = rnd((n,), 3, dt), ops.pack_weight_i8(codes, ws)
+    res = torch.randn((m, n + 3), generator=torch.Generator(DEV).manual_seed(4), device=DEV).to(dt)[:, 1:1 + n]
+    for r, act in ((None, ops.MV_ACT_SILU), (res, 0)):
+        got = ops.linear_i8(x, w, bias=bias, residual=r, act=act)
+        torch.cuda.synchronize()
+        for a in range(0, m, 4096):
+            want, bound = linear_oracle(x[a:a + 4096], codes, ws, bias, None if r is None else r[a:a + 4096], act == ops.MV_ACT_SILU)
+            within(got[a:a + 4096], want, bound, what=(m, k, n, a))
+
+
+@gpu
 @pytest.mark.parametrize("m", [1, 40, 300])
 def test_linear_i8_extreme_codes_zero_and_nonfinite_rows(m):
     """the largest possible sum (K = 131072 would reach 2^31) stays exact; a row that is not finite gives NaN, the others do not notice"""
