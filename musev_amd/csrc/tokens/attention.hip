@@ -88,7 +88,7 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(const mv_attn_
     for (int b = 0; b < C::NB; ++b)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[b][e] = 0.f;
-    float m = -1.0e30f, l = 0.f;    // reference of the exponents (score units; m * c stays finite), sum of this lane's own keys
+    float m = -3.0e38f / fmaxf(c, 1.0f), l = 0.f;    // reference of the exponents (score units; m * c stays finite), sum of this lane's own keys
 
     // ---- global -> LDS ----
     lds_t* ring = (lds_t*)((__attribute__((address_space(3))) char*)smem);
@@ -174,8 +174,11 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(const mv_attn_
         for (int n = 0; n < C::NS; ++n)
 #pragma unroll
             for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[n][e]);
-        // the reference moves only when a score passes it by more than 2^6: P stays below 64 and the accumulators are rarely rescaled
-        if (__any((mx - m) * c > 6.0f)) {
+        // The reference moves only when a score passes it by more than 2^6: P stays below 64 and the accumulators are rarely rescaled.
+        // The exponent s c - m c is formed in one step with m c rounded: half a step of that is a factor common to the row, which the sum takes out
+        // again.  Of references beyond 2^12 it could pass the type's range, so there the difference is formed first.
+        float mc = m * c;
+        if (__any((mx - m) * c > 6.0f || fabsf(mc) > 0x1p12f)) {
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
             const float mn = fmaxf(m, mx);
             const float a = __builtin_amdgcn_exp2f((m - mn) * c);
@@ -185,8 +188,15 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(const mv_attn_
             for (int b = 0; b < C::NB; ++b)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[b][e] *= a;
+            mc = m * c;
+            if (__any(fabsf(mc) > 0x1p12f)) {
+#pragma unroll
+                for (int n = 0; n < C::NS; ++n)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[n][e] -= m;
+                mc = 0.f;
+            }
         }
-        const float mc = m * c;
         float t0 = 0.f, t1 = 0.f;
         if constexpr (!masked) {   // (beside the exponentials)
 #pragma unroll
@@ -255,7 +265,7 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(const mv_attn_
     const int whole = max(0, first_lim - it.key_begin) / C::KT;
     auto walk = [&](int t, auto tag) __attribute__((always_inline)) {
         const int key = it.key_begin + t * C::KT;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // this wave's share of tile t has landed ...
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // this wave's share of tile t has landed, its reads of tile t - 1 are over ...
         __builtin_amdgcn_s_barrier();                        // ... and everyone's; everyone has left tile t - 1 and its stage
         asm volatile("" ::: "memory");
         if (t + 1 < tiles) issue(key + C::KT, (t + 1) & 1);

@@ -453,6 +453,23 @@ def test_attention_of_peaked_and_of_growing_scores(dt):
 
 
 @gpu
+@pytest.mark.parametrize("dt,big,step", [(torch.bfloat16, 2.0 ** 55, 2.0 ** 50), (torch.float16, 2.0 ** 15, 2.0 ** 4)], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lens", [([200], [200]), ([1, 3], [5000, 70])], ids=["prompt", "split"])
+def test_attention_of_scores_far_below_zero(lens, d, dt, big, step):
+    """the best score a query sees is -d big step, the others lower by at least as much: its output is that key's value, exactly"""
+    from musev_amd import ops
+    ql, kl = lens
+    q = torch.full((sum(ql), d), big, device=DEV).to(dt)
+    rank = torch.cat([torch.arange(n) % 200 + 1 + (torch.arange(n) > 0) for n in kl])
+    k = (rank[:, None].float() * -step).expand(-1, d).contiguous().to(DEV).to(dt)   # (multiples of a power of two up to 201: exact)
+    v = rnd((sum(kl), d), 3, dt)
+    got = ops.attention_packed(ops.attention_plan(ql, kl, heads=1, d=d, scale=1.0), q, k, v)
+    first = torch.tensor([sum(kl[:i]) for i, n in enumerate(ql) for _ in range(n)], device=DEV)
+    assert torch.equal(got, v[first])
+
+
+@gpu
 @pytest.mark.parametrize("one", [False, True], ids=["prompt", "one_token"])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")], ids=["nan", "inf", "-inf"])
 def test_what_is_not_seen_does_not_reach_the_output(bad, one):
