@@ -64,7 +64,8 @@ int mv_rotary_axes(const mv_rotary_desc* d, void* stream);
  *   y = post ? N(f) * post_gamma + post_beta : f          N: rms (x / sqrt(mean x^2 + eps)) or layer ((x - mean) / sqrt(var + eps))
  *   s = alpha * x + gate[g] * y                            g: group_index[row], or row / rows_per_group; gate null: 1
  *   h = (N(s) * pre_gamma + pre_beta) * (1 + scale[g]) + shift[g]   (only with norm_out)
- * stream_out = s, norm_out = h; every statistic and s itself in fp32, each output rounded once.  A row whose group_index lies outside
+ * stream_out = s, norm_out = h; every statistic and s itself in fp32 (rows whose squares sum within its range: values up to about 1e16 in size),
+ * each output rounded once.  A row whose group_index lies outside
  * [0, groups) is filled with NaN.  stream_out may be x or f, norm_out may be f or x.                                                  */
 typedef struct mv_gated_norm_desc {
     const void *x, *f;
@@ -81,7 +82,8 @@ int mv_gated_residual_norm(const mv_gated_norm_desc* d, void* stream);
 /* ---- int8 projection -----------------------------------------------------------------------------------------------------------------
  * mv_quantize_rows_i8: scale[m] = max_k |x[m, k]| / 127, code = round-to-nearest-even(127 x / max|x|); columns K .. ldc - 1 of the codes
  * become 0; a row of zeros has scale 0; a row that holds an infinity or NaN has that scale and codes 0 (its products are NaN).
- * mv_gemm_i8: out = act(a_scale[m] * w_scale[n] * sum_k a[m, k] w[n, k] + bias[n]) + residual[m, n];  the sum is exact (int32: K <= 131071).
+ * mv_gemm_i8: out = act(a_scale[m] * w_scale[n] * sum_k a[m, k] w[n, k] + bias[n]) + residual[m, n];  the sum is exact (int32: K <= 131071),
+ * what follows is fp32 from left to right (sum * a_scale first).
  * lda, ldw: multiples of 128, the columns from K on are 0.                                                                             */
 int mv_quantize_rows_i8(const void* x, int64_t ldx, int64_t rows, int32_t k, int32_t dtype, int8_t* codes, int64_t ldc, float* scale,
                         void* stream);

@@ -374,8 +374,9 @@ def gated_residual_norm(x: torch.Tensor, f: torch.Tensor, *, kind: str = "layer"
         h = (N(s) * gamma + beta) * (1 + scale[g]) + shift[g]   with ``pre = (gamma, beta, eps)``; h reads s before its rounding
 
     N: ``kind`` "rms" or "layer"; a gamma or beta may be ``None``.  ``gate`` / ``scale`` / ``shift``: [groups, C] matrices, g the row's group --
-    ``group_index`` (int32 per row: packed sequences) or row // ``rows_per_group``; with one group neither is needed.  A row whose
-    group_index is no group is filled with NaN.  Returns (s, h), h ``None`` without ``pre``.  ``out`` may be ``x`` or ``f`` itself, ``norm_out`` too."""
+    ``group_index`` (int32 per row: packed sequences) or row // ``rows_per_group``; with one group neither is needed.  Statistics are
+    fp32: values up to about 1e16 in size.  A row whose group_index is no group is filled with NaN.  Returns (s, h), h ``None`` without
+    ``pre``.  ``out`` may be ``x`` or ``f`` itself, ``norm_out`` too."""
     rows, c, ldx = _matrix(x, "x")
     dtype, dev = x.dtype, x.get_device()
     frows, fc, ldf = _matrix(f, "f", dtype, dev)
