@@ -490,9 +490,27 @@ static int launch_gemm_i8_shape(const mv_gemm_i8_desc* d, hipStream_t st) {
     // 6.4 / 6.8 / 5.1.
     const auto tiles = [&](int64_t bm, int64_t bn) { return ((d->M + bm - 1) / bm) * ((d->N + bn - 1) / bn); };
     // A residual past the last-level cache is read non-temporally (272 MB, 26 624 x 1280 -> 5120 with the quantisation: 280 -> 272 us; 136 MB, 6656 x 1280
-    // -> 10240 and still in the cache: 129.5 -> 132).
-    if (tiles(256, 256) >= 1024)
-        return d->residual && d->M * d->N * 2 > COLD_BYTES ? launch_gemm_i8<T, 256, 256, 128, 64, 1, true>(d, st) : launch_gemm_i8<T, 256, 256, 128, 64, 1>(d, st);
+    // -> 10240 and still in the cache: 129.5 -> 132).  Rounds of one 256 x 256 tile per CU: where the last would hold at most a quarter of a round, the rows
+    // of those tiles go to the smaller tiles, which spread them over the chip (us, together / apart; tiles left over in brackets: 6656 x 1280 x 10240
+    // 127.8 / 114.7 [40]; 8448 x 4096 x 8192 297.8 / 274.0 [32]; 13 824 x 1280 x 5120 125.3 / 119.5 [60]; 26 624 x 1280 x 5120 240.7 / 240.6 [40]; but
+    // 9216 x 2048 x 8192 176.2 / 183.0 [128]; 28 160 x 1280 x 5120 242.7 / 247.4 [160]).
+    if (const int64_t all = tiles(256, 256); all >= 1024) {
+        constexpr int64_t CUS = 256;
+        const int64_t cols = (d->N + 255) / 256, whole = all / CUS * CUS / cols, left = all - whole * cols;
+        mv_gemm_i8_desc head = *d, tail = *d;
+        const bool split = left > 0 && left <= CUS / 4;
+        if (split) {
+            head.M = whole * 256;
+            tail.M -= head.M;
+            tail.a += head.M * d->lda;
+            tail.a_scale += head.M;
+            if (d->residual) tail.residual = (const T*)d->residual + head.M * d->ldr;
+            tail.out = (T*)d->out + head.M * d->ldo;
+        }
+        const int rc = d->residual && d->M * d->N * 2 > COLD_BYTES ? launch_gemm_i8<T, 256, 256, 128, 64, 1, true>(&head, st)
+                                                                   : launch_gemm_i8<T, 256, 256, 128, 64, 1>(&head, st);
+        return rc == MV_OK && split ? launch_gemm_i8_shape<T>(&tail, st) : rc;
+    }
     if (tiles(128, 64) >= 512) return launch_gemm_i8<T, 128, 64, 64, 32, 1>(d, st);
     if (tiles(32, 32) <= 512) return launch_gemm_i8<T, 32, 32, 32, 32, 4>(d, st);
     if (tiles(64, 64) <= 256 && d->kp >= 2048) return launch_gemm_i8<T, 64, 64, 32, 32, 4>(d, st);

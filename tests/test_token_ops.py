@@ -851,6 +851,25 @@ def test_linear_i8_large(m, k, n, dt):
 
 
 @gpu
+@pytest.mark.parametrize("m,k,n,dt", [(8200, 300, 8190, torch.float16), (8300, 140, 8190, torch.bfloat16)])
+def test_linear_i8_rows_left_over_by_whole_rounds(m, k, n, dt):
+    """the rows behind the last whole round of the largest tiles, added to a residual in place; columns beside the result stay as they were"""
+    from musev_amd import ops
+    x = rnd((m, k), 1, dt)
+    codes = torch.randint(-127, 128, (n, k), generator=torch.Generator().manual_seed(2), dtype=torch.int32).to(torch.int8).to(DEV)
+    ws = ((0.5 + torch.rand(n, generator=torch.Generator().manual_seed(3))) / (73 * math.sqrt(k))).to(DEV)
+    bias, w = rnd((n,), 3, dt), ops.pack_weight_i8(codes, ws)
+    wide = torch.randn((m, n + 4), generator=torch.Generator(DEV).manual_seed(4), device=DEV).to(dt)
+    before = wide.clone()
+    got = ops.linear_i8(x, w, bias=bias, residual=wide[:, 1:1 + n], out=wide[:, 1:1 + n])
+    torch.cuda.synchronize()
+    assert torch.equal(wide[:, :1], before[:, :1]) and torch.equal(wide[:, 1 + n:], before[:, 1 + n:])
+    for a in range(0, m, 4096):
+        want, bound = linear_oracle(x[a:a + 4096], codes, ws, bias, before[a:a + 4096, 1:1 + n], False)
+        within(got[a:a + 4096], want, bound, what=(m, k, n, a))
+
+
+@gpu
 @pytest.mark.parametrize("m", [1, 40, 300])
 def test_linear_i8_extreme_codes_zero_and_nonfinite_rows(m):
     """the largest possible sum (K = 131072 would reach 2^31) stays exact; a row that is not finite gives NaN, the others do not notice"""
