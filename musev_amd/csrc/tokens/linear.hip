@@ -482,7 +482,7 @@ static int launch_gemm_i8_shape(const mv_gemm_i8_desc* d, hipStream_t st) {
         MV_CHECK_LAUNCH("mv_gemm_i8");
         return MV_OK;
     }
-    // The largest tile that still gives every CU a few blocks: 256 x 256 (one block per CU) from four rounds on, 128 x 64 (three per CU) from two
+    // The largest tile that fills the chip: 256 x 256 (one block per CU) from three quarters of a round on, 128 x 64 (three per CU) from two
     // blocks per CU, 64 x 64 below, where K is long and tiles are few in four groups, and 32 x 32 in four groups up to two per CU.
     // Measured (us, M x K x N; 256 / 128 x 64 / 64 / 64 in groups / 32 in groups): 8192^3 472 / 655 / 799 / - / -; 26 624 x 1280 x 5120 249 / 315 /
     // 380 / 792 / -; 4096 x 1280 x 2560 27.2 / 25.1 / 32.8 / 62 / -; 2048 x 1280 x 1280 22.9 / 10.3 / 10.8 / 18.4 / 22.6; 512 x 5120 x 1280 60 / 23.0 /
@@ -490,15 +490,17 @@ static int launch_gemm_i8_shape(const mv_gemm_i8_desc* d, hipStream_t st) {
     // 6.4 / 6.8 / 5.1.
     const auto tiles = [&](int64_t bm, int64_t bn) { return ((d->M + bm - 1) / bm) * ((d->N + bn - 1) / bn); };
     // A residual past the last-level cache is read non-temporally (272 MB, 26 624 x 1280 -> 5120 with the quantisation: 280 -> 272 us; 136 MB, 6656 x 1280
-    // -> 10240 and still in the cache: 129.5 -> 132).  Rounds of one 256 x 256 tile per CU: where the last would hold at most a quarter of a round, the rows
-    // of those tiles go to the smaller tiles, which spread them over the chip (us, together / apart; tiles left over in brackets: 6656 x 1280 x 10240
-    // 127.8 / 114.7 [40]; 8448 x 4096 x 8192 297.8 / 274.0 [32]; 13 824 x 1280 x 5120 125.3 / 119.5 [60]; 26 624 x 1280 x 5120 240.7 / 240.6 [40]; but
-    // 9216 x 2048 x 8192 176.2 / 183.0 [128]; 28 160 x 1280 x 5120 242.7 / 247.4 [160]).
-    if (const int64_t all = tiles(256, 256); all >= 1024) {
+    // -> 10240 and still in the cache: 129.5 -> 132).  The 256 x 256 tiles run in rounds of one per CU: where the last round would hold at most 3 / 8 of
+    // one, the rows of its tiles go to the smaller tiles, which spread them over the chip.  Measured with a residual (us; 128 x 64 alone / 256 alone /
+    // 256 and the rest apart), K = 1280, N = 4096: 160 tiles 23.6 / 25.3 / -; 208 31.2 / 26.4 / -; 272 38.4 / 48.2 / 37.3; 352 47.3 / 49.2 / 44.8; 384 51.4 /
+    // 50.4 / 50.1; 416 56.5 / 52.2 / 53.5; 608 82.3 / 75.9 / 73.4; 640 86.3 / 77.1 / 79.6; 784 104.9 / 99.8 / 90.4.  K = 4096: 160 54.7 / 52.4 / -; 272 95.8 /
+    // 109.2 / 76.8; 352 119.5 / 111.0 / 99.2; 384 130.6 / 113.3 / 114.5.  K = 640: 160 16.9 / 18.1 / -; 272 26.4 / 34.1 / 26.8; 384 34.2 / 35.8 / 36.1; 784
+    // 67.8 / 69.1 / 62.7.
+    if (const int64_t all = tiles(256, 256); all >= 192) {
         constexpr int64_t CUS = 256;
         const int64_t cols = (d->N + 255) / 256, whole = all / CUS * CUS / cols, left = all - whole * cols;
         mv_gemm_i8_desc head = *d, tail = *d;
-        const bool split = left > 0 && left <= CUS / 4;
+        const bool split = whole > 0 && left > 0 && left <= 3 * CUS / 8;
         if (split) {
             head.M = whole * 256;
             tail.M -= head.M;
