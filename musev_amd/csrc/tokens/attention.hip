@@ -281,13 +281,16 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(const mv_attn_
     if (row0 + l31 >= rows) return;
     if (it.ws_row >= 0) {
         float* ws = (float*)p.workspace;
-        const int64_t at = (int64_t)kvh * p.ws_rows + it.ws_row + wave * 32 + l31;
+        // a part's sums as [4 columns][row][4]: what a half wave stores, and what the join reads, is contiguous
+        const int part_rows = min(128, rows - it.m0);
+        const int64_t first = (int64_t)kvh * p.ws_rows + it.ws_row, at = first + wave * 32 + l31;
 #pragma unroll
         for (int b = 0; b < C::NB; ++b)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const int col = 32 * b + 8 * g + 4 * h;
-                if (col < p.d) *(float4v*)(ws + at * p.d + col) = float4v{acc[b][4 * g], acc[b][4 * g + 1], acc[b][4 * g + 2], acc[b][4 * g + 3]};
+                const int quad = 8 * b + 2 * g + h;
+                if (quad * 4 < p.d)
+                    *(float4v*)(ws + first * p.d + (quad * part_rows + wave * 32 + l31) * 4) = float4v{acc[b][4 * g], acc[b][4 * g + 1], acc[b][4 * g + 2], acc[b][4 * g + 3]};
             }
         if (h == 0) {
             float* wml = ws + (int64_t)p.kv_heads * p.ws_rows * p.d + at * 2;
@@ -311,61 +314,86 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(const mv_attn_
         }
 }
 
-// Joins the parts of rows whose keys were split over several items.  WPR waves per packed row take its parts in turn, four loads of each on their
-// way at once: the parts were just written by other XCDs, and what the join of a few rows costs is those loads' latency (one token of 8 k keys, 8
-// key / value heads: 13.8 us with four waves per row, 21.9 with one).  With many rows the other rows hide it and one wave per row is right (a
-// prompt of 1024, 16 heads: 21 against 31 us).
-template <typename T, int WPR>
-__global__ __launch_bounds__(256) void attention_join_kernel(const mv_attn_packed_desc p) {
-    __shared__ float2v other[3][64];
-    const int lane = threadIdx.x & 63, wave = WPR == 1 ? 0 : threadIdx.x >> 6, group = p.heads / p.kv_heads;
-    const int at_row = WPR == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
-    const int join = at_row / (p.kv_heads * p.join_rows), rest = at_row - join * (p.kv_heads * p.join_rows);
-    if (join >= p.n_joins) return;
-    const int kvh = rest / p.join_rows, row = rest - kvh * p.join_rows;
+// Joins the parts of rows whose keys were split over several items: a thread takes four columns of a row.  G threads share its parts, in turn and four
+// at a time: the parts were just written by other XCDs, and what the join of many parts costs is those loads' latency.  Attention and join (us, G = 1 /
+// 8): 64 parts, one token over 8192 keys, 8 key / value heads 17.6 / 12.0; 52 parts, 2 x 4 tokens over 16 500 keys 22.5 / 18.0; 32 parts, 2 x 128
+// tokens over 8192 29.8 / 28.9; 16 parts, 4 x 128 over 8192 39.9 / 39.4; 16 parts, one token over 2048 9.15 / 9.35; up to 9 parts of chunks 23.4 / 27.7.
+template <typename T, int G>
+__global__ __launch_bounds__(256) void attention_join_kernel(const mv_attn_packed_desc p, const int blocks) {
+    constexpr int OWN = 256 / G;   // (row, four columns) of a block
+    __shared__ float4v other_o[G > 1 ? G - 1 : 1][OWN];
+    __shared__ float2v other_ml[G > 1 ? G - 1 : 1][OWN];
+    const int join = blockIdx.x / (p.kv_heads * blocks), rest = blockIdx.x - join * (p.kv_heads * blocks);
+    const int kvh = rest / blocks, own = threadIdx.x % OWN, part0 = threadIdx.x / OWN, group = p.heads / p.kv_heads;
     const PackedJoin jn = ((const PackedJoin*)p.joins)[join];
-    if (row >= jn.rows) return;   // (joins differ in their rows; with WPR = 4 the whole block)
-    const int rr = jn.m0 + row, i = rr / group, head = kvh * group + (rr - i * group);
+    const int x = (rest - kvh * blocks) * OWN + own;
+    const int quad = x / jn.rows, row = x - quad * jn.rows;
+    const bool valid = quad * 4 < p.d;   // (joins differ in their rows)
     const float* ws = (const float*)p.workspace;
-    const int64_t at = (int64_t)kvh * p.ws_rows + jn.ws_row + row;
-    const float* ml = ws + (int64_t)p.kv_heads * p.ws_rows * p.d;
-    const int col = min(lane * 2, p.d - 2);
-    float mm = -3.0e38f, ll = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int s0 = 0; s0 < jn.parts; s0 += 64) {
-        const int n = min(64, jn.parts - s0);
-        float2v w = {-3.0e38f, 0.f};   // lane s: part s's reference and sum
-        if (lane < n) w = *(const float2v*)(ml + (at + (int64_t)(s0 + lane) * jn.rows) * 2);
-        const float mn = fmaxf(mm, wave_max(w.x)), old = __builtin_amdgcn_exp2f(mm - mn);
-        const float a = w.y != 0.f ? __builtin_amdgcn_exp2f(w.x - mn) : 0.f;   // (a part that saw no key adds nothing)
-        mm = mn;
-        ll = ll * old + wave_sum(a * w.y);
-        o0 *= old;
-        o1 *= old;
-        for (int s = wave; s < n; s += 4 * WPR) {
-            float2v v[4];
-            float as[4];
+    const int64_t first = (int64_t)kvh * p.ws_rows + jn.ws_row;
+    const float* ml = ws + (int64_t)p.kv_heads * p.ws_rows * p.d + (first + row) * 2;
+    const float* sums = ws + first * p.d + (int64_t)x * 4;
+    float mm = -3.0e38f, ll = 0.f;
+    float4v o = {0.f, 0.f, 0.f, 0.f};
+    if (valid)
+        for (int s = part0; s < jn.parts; s += 4 * G) {
+            float2v w[4];
+            float4v v[4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int sx = min(s + WPR * x, n - 1);
-                v[x] = *(const float2v*)(ws + (at + (int64_t)(s0 + sx) * jn.rows) * p.d + col);
-                as[x] = s + WPR * x < n ? __shfl(a, sx, 64) : 0.f;
+            for (int u = 0; u < 4; ++u) {
+                const int64_t at = (int64_t)min(s + G * u, jn.parts - 1) * jn.rows;
+                w[u] = *(const float2v*)(ml + at * 2);
+                v[u] = *(const float4v*)(sums + at * p.d);
             }
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-                if (as[x] != 0.f) o0 = __builtin_fmaf(as[x], v[x].x, o0), o1 = __builtin_fmaf(as[x], v[x].y, o1);
+            for (int u = 0; u < 4; ++u)
+                if (s + G * u >= jn.parts) w[u] = float2v{-3.0e38f, 0.f};
+            const float mn = fmaxf(fmaxf(mm, fmaxf(w[0].x, w[1].x)), fmaxf(w[2].x, w[3].x)), old = __builtin_amdgcn_exp2f(mm - mn);
+            mm = mn;
+            ll *= old;
+            o *= old;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const float a = w[u].y != 0.f ? __builtin_amdgcn_exp2f(w[u].x - mn) : 0.f;   // (a part that saw no key adds nothing)
+                ll = __builtin_fmaf(a, w[u].y, ll);
+                if (a == 0.f) continue;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(a, v[u][e], o[e]);
+            }
+        }
+    if constexpr (G > 1) {
+        if (part0 > 0) {
+            other_o[part0 - 1][own] = o;
+            other_ml[part0 - 1][own] = float2v{mm, ll};
+        }
+        __syncthreads();
+        if (part0 > 0) return;
+        float mn = mm;
+#pragma unroll
+        for (int u = 0; u < G - 1; ++u) mn = fmaxf(mn, other_ml[u][own].x);
+        const float a0 = ll != 0.f ? __builtin_amdgcn_exp2f(mm - mn) : 0.f;
+        ll *= a0;
+        if (a0 != 1.f)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = a0 != 0.f ? o[e] * a0 : 0.f;
+#pragma unroll
+        for (int u = 0; u < G - 1; ++u) {
+            const float2v w = other_ml[u][own];
+            const float a = w.y != 0.f ? __builtin_amdgcn_exp2f(w.x - mn) : 0.f;
+            ll = __builtin_fmaf(a, w.y, ll);
+            if (a == 0.f) continue;
+            const float4v v = other_o[u][own];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(a, v[e], o[e]);
         }
     }
-    if constexpr (WPR > 1) {
-        if (wave > 0) other[wave - 1][lane] = float2v{o0, o1};
-        __syncthreads();
-        if (wave > 0) return;
-#pragma unroll
-        for (int x = 0; x < 3; ++x) o0 += other[x][lane].x, o1 += other[x][lane].y;
-    }
-    if (lane * 2 >= p.d) return;
+    if (!valid) return;
+    const int rr = jn.m0 + row, i = rr / group, head = kvh * group + (rr - i * group);
     const int see = p.causal ? i + jn.kv_len - jn.q_len + 1 : jn.kv_len;
-    T w2[2] = {see > 0 ? (T)(o0 / ll) : (T)0.f, see > 0 ? (T)(o1 / ll) : (T)0.f};
-    *(unsigned*)((T*)p.out + (int64_t)(jn.q_row + i) * p.ldo + (int64_t)head * p.d + col) = *(const unsigned*)w2;
+    T w4[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w4[e] = see > 0 ? (T)(o[e] / ll) : (T)0.f;
+    *(uint2*)((T*)p.out + (int64_t)(jn.q_row + i) * p.ldo + (int64_t)head * p.d + quad * 4) = *(const uint2*)w4;
 }
 
 extern "C" int64_t mv_attention_packed_workspace_bytes(int64_t ws_rows, int32_t kv_heads, int32_t d) {
@@ -373,7 +401,11 @@ extern "C" int64_t mv_attention_packed_workspace_bytes(int64_t ws_rows, int32_t 
     return ws_rows * kv_heads * (d + 2) * 4;
 }
 
-constexpr int64_t JOIN_FEW = 2048;   // packed rows up to which four waves join a row: two blocks of them per SIMD of the chip
+template <typename T, int G>
+static void launch_join(const mv_attn_packed_desc* d, hipStream_t st) {
+    const int blocks = (d->join_rows * (d->d / 4) + 256 / G - 1) / (256 / G);
+    attention_join_kernel<T, G><<<(unsigned)(d->n_joins * d->kv_heads * blocks), 256, 0, st>>>(*d, blocks);
+}
 
 template <typename T, int K16>
 static int launch_packed(const mv_attn_packed_desc* d, hipStream_t st) {
@@ -381,9 +413,8 @@ static int launch_packed(const mv_attn_packed_desc* d, hipStream_t st) {
     attention_packed_kernel<T, K16><<<(unsigned)(d->n_items * d->kv_heads), 256, PackedCfg<K16>::LDS_BYTES, st>>>(*d);
     MV_CHECK_LAUNCH("mv_attention_packed");
     if (d->n_joins > 0) {
-        const int64_t rows = (int64_t)d->n_joins * d->kv_heads * d->join_rows;
-        if (rows <= JOIN_FEW) attention_join_kernel<T, 4><<<(unsigned)rows, 256, 0, st>>>(*d);
-        else attention_join_kernel<T, 1><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(*d);
+        if (d->ws_rows > 16ll * d->n_joins * d->join_rows) launch_join<T, 8>(d, st);   // (parts of a join, in the mean)
+        else launch_join<T, 1>(d, st);
         MV_CHECK_LAUNCH("mv_attention_packed (join)");
     }
     return MV_OK;
