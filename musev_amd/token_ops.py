@@ -10,6 +10,7 @@ concurrent calls and several captured graphs never share it.  A graph refers to 
 from __future__ import annotations
 
 import ctypes as C
+import heapq
 import math
 import operator
 import struct
@@ -168,12 +169,13 @@ TILE_ROWS = 128   # packed rows per item
 # Keys of an item that is worth a split: an item's parts each write and the join reads back (d + 2) fp32 per row.
 MIN_PART = 128
 BLOCKS = 512      # two blocks on each of the 256 CUs
+LATE_PART = 1024  # keys of a part of a block that would run late
 
 
 def _plan_items(ql: Sequence[int], kl: Sequence[int], group: int, kv_heads: int, causal: bool):
     """(items, joins, workspace rows): see include/musev_tokens.h.  An item's keys end with what its last query sees.  Where the items alone would
-    leave CUs idle, or one item would outlast the others, its keys are split into parts of about 1 / BLOCKS of all the work; the longest items
-    come first."""
+    leave CUs idle, or one item would outlast the others, its keys are split into parts of about 1 / BLOCKS of all the work (`_late_parts`: or
+    where a last round would hold few of them); the longest items come first."""
     tiles, q_row, k_row = [], 0, 0
     for q, kv in zip(ql, kl):
         for m0 in range(0, q * group, TILE_ROWS):
@@ -183,8 +185,10 @@ def _plan_items(ql: Sequence[int], kl: Sequence[int], group: int, kv_heads: int,
     items, joins, ws = [], [], 0
     part = max(MIN_PART, -(-sum(t[5] for t in tiles) * kv_heads // BLOCKS))
     part = -(-part // 64) * 64
-    for q_row, q, k_row, kv, m0, end in tiles:
-        n = max(1, (end + part // 2) // part)
+    parts = [max(1, (t[5] + part // 2) // part) for t in tiles]
+    if max(parts, default=1) == 1 and BLOCKS < len(tiles) * kv_heads <= 8 * BLOCKS:
+        parts = _late_parts([t[5] for t in tiles], kv_heads)
+    for (q_row, q, k_row, kv, m0, end), n in zip(tiles, parts):
         if n == 1:
             items.append((q_row, q, k_row, kv, m0, 0, end, -1))
             continue
@@ -197,6 +201,36 @@ def _plan_items(ql: Sequence[int], kl: Sequence[int], group: int, kv_heads: int,
         ws += n * rows
     items.sort(key=lambda i: i[5] - i[6])
     return items, joins, ws
+
+
+def _late_parts(ends: Sequence[int], kv_heads: int) -> List[int]:
+    """Parts of every tile (`ends`: its keys) where there are a few rounds of blocks: blocks that would outlast the mean are split to end with the
+    others, where they are few and long enough to pay for the join of their parts.  Measured (us, whole / split, late blocks x their keys): 12 heads
+    over 6000 keys 272 / 227 [60 x 6000], 6 over 13 312 590 / 514 [114], 8 over 13 312 573 / 516 [320]; but 8 over 4 x 3000 149 / 162 [256 x 3000], 8 over
+    3 x 4500 262 / 272 [352 x 4500], 8 over 6 x 1500 46.6 / 47.0 [64 x 1500]."""
+    parts = [1] * len(ends)
+    if max(ends) < 2 * LATE_PART:
+        return parts
+    order = sorted(range(len(ends)), key=lambda i: -ends[i])
+    mean = sum(ends) * kv_heads // BLOCKS
+
+    def rooms(split):
+        """(tile, keys that fit in before the mean where its last block starts) in order; tiles for which ``split`` holds are cut to that size"""
+        busy = [0] * BLOCKS
+        for i in order:
+            start = busy[0]
+            if split(i):
+                start = heapq.nsmallest(kv_heads, busy)[-1]
+                parts[i] = -(-ends[i] // max(LATE_PART, mean - start))
+            for _ in range(kv_heads * parts[i]):
+                start = busy[0]
+                heapq.heapreplace(busy, start + ends[i] // parts[i])
+            yield i, mean - start
+
+    late = {i for i, room in rooms(lambda i: False) if ends[i] > room + LATE_PART}
+    for _ in rooms(lambda i: i in late and ends[i] >= 32 * kv_heads * len(late)):
+        pass
+    return parts
 
 
 def attention_plan(q_lens: Sequence[int], kv_lens: Optional[Sequence[int]] = None, *, heads: int, kv_heads: Optional[int] = None, d: int,

@@ -175,6 +175,29 @@ def test_plan_covers_every_visible_key_once(seed):
         assert plan._workspace == _lib.load().mv_attention_packed_workspace_bytes(d.ws_rows, kvh, 64)
 
 
+LATE = {   # lengths, heads per key / value head, key / value heads, causal -> tiles that are split
+    "few_late": ([6000], [6000], 1, 12, False, 5),
+    "many_late": ([13312], [13312], 1, 8, False, 40),
+    "two_lengths": ([13312, 5121], [13312, 5121], 1, 16, False, 8),
+    "one_key_head": ([1100], [9000], 64, 1, False, 38),
+    "late_but_short": ([3000] * 4, [3000] * 4, 1, 8, False, 0),
+    "balanced": ([16384], [16384], 4, 4, True, 0),
+    "too_many_rounds": ([70000], [3000], 1, 8, False, 0),
+    "heads_beyond_the_blocks": ([200], [2100], 1, 600, False, 0),
+}
+
+
+@pytest.mark.parametrize("name", list(LATE))
+def test_plan_splits_the_blocks_that_would_run_late(name):
+    """the parts cover every key once; the longest items come first"""
+    from musev_amd import token_ops as to
+    ql, kl, group, kvh, causal, split = LATE[name]
+    items, joins, ws = to._plan_items(ql, kl, group, kvh, causal)
+    assert len(joins) == split
+    _cover(items, joins, ws, ql, kl, group, causal)
+    assert all(a[6] - a[5] >= b[6] - b[5] for a, b in zip(items, items[1:]))
+
+
 def test_plan_refusals():
     from musev_amd import ops
     ok = dict(heads=4, kv_heads=2, d=64, device="cpu")
@@ -436,6 +459,20 @@ def test_attention_of_drawn_lengths(seed, dt):
     got = ops.attention_packed(ops.attention_plan(ql, kl, heads=heads, kv_heads=kvh, d=d, causal=causal), q, k, v)
     torch.cuda.synchronize()
     within(got, *attention_oracle(q, k, v, ql, kl, heads, kvh, d, causal), what=(ql, kl, heads, kvh, d, causal))
+
+
+@gpu
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_of_blocks_that_would_run_late(causal):
+    """a little more than a round of blocks: the last tiles' keys are split"""
+    from musev_amd import ops
+    ql, kl, heads, kvh, d = [2176, 3], [4100, 900], 32, 4, 32
+    q, k, v = attention_inputs(ql, kl, heads, kvh, d, torch.float16, 21)
+    plan = ops.attention_plan(ql, kl, heads=heads, kv_heads=kvh, d=d, causal=causal)
+    assert plan.n_joins > 0 or causal
+    got = ops.attention_packed(plan, q, k, v)
+    torch.cuda.synchronize()
+    within(got, *attention_oracle(q, k, v, ql, kl, heads, kvh, d, causal), what=causal)
 
 
 @gpu
