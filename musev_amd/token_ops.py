@@ -228,8 +228,10 @@ def _late_parts(ends: Sequence[int], kv_heads: int) -> List[int]:
             yield i, mean - start
 
     late = {i for i, room in rooms(lambda i: False) if ends[i] > room + LATE_PART}
-    for _ in rooms(lambda i: i in late and ends[i] >= 32 * kv_heads * len(late)):
-        pass
+    late = {i for i in late if ends[i] >= 32 * kv_heads * len(late)}
+    if late:
+        for _ in rooms(lambda i: i in late):
+            pass
     return parts
 
 
