@@ -450,6 +450,9 @@ def gated_residual_norm(x: torch.Tensor, f: torch.Tensor, *, kind: str = "layer"
         per = min(per, _I32_MAX)
     elif groups > 1:
         raise ValueError(f"gated_residual_norm: {groups} groups need rows_per_group or group_index")
+    for nm, a in (("post", post), ("pre", pre)):
+        if a is not None and not 0.0 <= a[2] < math.inf:
+            raise ValueError(f"gated_residual_norm: {nm} eps {a[2]} (a finite number, not negative)")
     given = out is not None or norm_out is not None
     if out is None:
         out, lds = x.new_empty((rows, c)), c

@@ -326,6 +326,15 @@ def test_refusals_of_the_gated_norm(on_cpu):
         ops.gated_residual_norm(wide, wide)
 
 
+@pytest.mark.parametrize("eps", [-1e-6, float("nan"), float("inf")])
+@pytest.mark.parametrize("which", ["pre", "post"])
+def test_the_gated_norm_refuses_an_eps_that_is_none(on_cpu, which, eps):
+    from musev_amd import ops
+    x, f = torch.zeros(6, 40, dtype=torch.float16), torch.zeros(6, 40, dtype=torch.float16)
+    with pytest.raises(ValueError, match="eps"):
+        ops.gated_residual_norm(x, f, **{which: (None, None, eps)})
+
+
 def test_refusals_of_the_int8_projection(on_cpu):
     from musev_amd import ops
     w = ops.pack_weight_i8(torch.ones(24, 40, dtype=torch.int8), torch.ones(24))
@@ -487,6 +496,19 @@ def test_attention_of_peaked_and_of_growing_scores(dt):
         got = ops.attention_packed(ops.attention_plan(ql, heads=heads, kv_heads=kvh, d=d, scale=scale), q, k, v)
         torch.cuda.synchronize()
         within(got, *attention_oracle(q, k, v, ql, ql, heads, kvh, d, True, scale), what=scale)
+
+
+@gpu
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS)
+@pytest.mark.parametrize("scale", [0.0, 1e-30])
+def test_attention_of_a_vanishing_scale(scale, dt):
+    """every key a query sees weighs the same; keys split over many parts and not"""
+    from musev_amd import ops
+    ql, kl = [130, 1, 0, 2], [130, 3000, 7, 64]
+    q, k, v = attention_inputs(ql, kl, 4, 2, 64, dt, 31)
+    got = ops.attention_packed(ops.attention_plan(ql, kl, heads=4, kv_heads=2, d=64, scale=scale), q, k, v)
+    torch.cuda.synchronize()
+    within(got, *attention_oracle(q, k, v, ql, kl, 4, 2, 64, True, scale), what=scale)
 
 
 @gpu
