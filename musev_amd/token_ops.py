@@ -72,7 +72,8 @@ def _matrix(t: torch.Tensor, name: str, dtype: Optional[torch.dtype] = None, dev
     """(rows, columns, row stride) of a 2-D tensor with unit inner stride on the GPU; a single row has no stride of its own: its width stands in"""
     if not isinstance(t, torch.Tensor) or t.ndim != 2:
         raise ValueError(f"{name}: expected a 2-D tensor, got {tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__}")
-    (rows, cols), (ld, inner) = t.shape, t.stride()
+    rows, cols = t.shape
+    ld, inner = t.stride()
     if inner != 1 and cols > 1:
         raise ValueError(f"{name}: expected unit inner stride, got shape {(rows, cols)} strides {(ld, inner)}")
     if dev is None and not _on_gpu(t) or (t.dtype not in _DTYPES if dtype is None else t.dtype != dtype):
@@ -360,13 +361,13 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
     if table._dev != dev:
         raise ValueError(f"rotary_axes: table on {table.device}, tensors on {q.device}")
     if out_q is None:
-        oq, ldoq = q.new_empty((n, heads * d)), heads * d
+        oq, ldoq = torch.empty_like(q), heads * d   # (a matrix with gaps between its rows gets one without)
     else:
         oq, ldoq = out_q, _rotary_out("q", q, out_q, (("q", q), ("k", k), ("positions", positions)), dtype, dev)
     ok = None
     if k is not None:
         if out_k is None:
-            ok, ldok = q.new_empty((n, kv_heads * d)), kv_heads * d
+            ok, ldok = torch.empty_like(k), kv_heads * d
         else:
             ok, ldok = out_k, _rotary_out("k", k, out_k, (("q", q), ("k", k), ("positions", positions)), dtype, dev)
             if out_q is not None:
@@ -455,7 +456,7 @@ def gated_residual_norm(x: torch.Tensor, f: torch.Tensor, *, kind: str = "layer"
             raise ValueError(f"gated_residual_norm: {nm} eps {a[2]} (a finite number, not negative)")
     given = out is not None or norm_out is not None
     if out is None:
-        out, lds = x.new_empty((rows, c)), c
+        out, lds = torch.empty_like(x), c
     else:
         lds = _matrix(out, "out", dtype, dev)[2]
         if out.shape != x.shape:
@@ -465,7 +466,7 @@ def gated_residual_norm(x: torch.Tensor, f: torch.Tensor, *, kind: str = "layer"
     if pre is not None:
         pre_gamma, pre_beta, pre_eps = _affine(pre[0], "pre gamma", c, dtype, dev), _affine(pre[1], "pre beta", c, dtype, dev), pre[2]
         if norm_out is None:
-            norm_out, ldh = x.new_empty((rows, c)), c
+            norm_out, ldh = torch.empty_like(x), c
         else:
             ldh = _matrix(norm_out, "norm_out", dtype, dev)[2]
             if norm_out.shape != x.shape:
