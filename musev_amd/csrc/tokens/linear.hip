@@ -482,25 +482,24 @@ static int launch_gemm_i8_shape(const mv_gemm_i8_desc* d, hipStream_t st) {
         MV_CHECK_LAUNCH("mv_gemm_i8");
         return MV_OK;
     }
-    // The largest tile that fills the chip: 256 x 256 (one block per CU) from three quarters of a round on, 128 x 64 (three per CU) from two
-    // blocks per CU, 64 x 64 below, where K is long and tiles are few in four groups, and 32 x 32 in four groups up to two per CU.
+    // The largest tile that fills the chip: 256 x 256 (one block per CU) from three quarters of a round on, 128 x 128 where one round holds them, 128 x 64
+    // (three per CU) from two blocks per CU, 64 x 64 below, where K is long and tiles are few in four groups, and 32 x 32 in four groups up to two per CU.
     // Measured (us, M x K x N; 256 / 128 x 64 / 64 / 64 in groups / 32 in groups): 8192^3 472 / 655 / 799 / - / -; 26 624 x 1280 x 5120 249 / 315 /
     // 380 / 792 / -; 4096 x 1280 x 2560 27.2 / 25.1 / 32.8 / 62 / -; 2048 x 1280 x 1280 22.9 / 10.3 / 10.8 / 18.4 / 22.6; 512 x 5120 x 1280 60 / 23.0 /
     // 19.8 / 13.9 / 16.3; 512 x 1280 x 1280 22.5 / 8.4 / 6.6 / 7.1 / 9.1; 300 x 5120 x 1280 61 / 19.3 / 14.0 / 11.8 / 10.8; 64 x 1280 x 1280 20 / 8.2 /
     // 6.4 / 6.8 / 5.1.
     const auto tiles = [&](int64_t bm, int64_t bn) { return ((d->M + bm - 1) / bm) * ((d->N + bn - 1) / bn); };
     // A residual past the last-level cache is read non-temporally (272 MB, 26 624 x 1280 -> 5120 with the quantisation: 280 -> 272 us; 136 MB, 6656 x 1280
-    // -> 10240 and still in the cache: 129.5 -> 132).  The 256 x 256 tiles run in rounds of one per CU: where the last round would hold at most 3 / 8 of
+    // -> 10240 and still in the cache: 129.5 -> 132).  The 256 x 256 tiles run in rounds of one per CU: where the last round would hold at most half of
     // one, the rows of its tiles go to the smaller tiles, which spread them over the chip.  Measured with a residual (us; 128 x 64 alone / 256 alone /
-    // 256 and the rest apart), K = 1280, N = 4096: 160 tiles 23.6 / 25.3 / -; 208 31.2 / 26.4 / -; 272 38.4 / 48.2 / 37.3; 352 47.3 / 49.2 / 44.8; 384 51.4 /
-    // 50.4 / 50.1; 416 56.5 / 52.2 / 53.5; 608 82.3 / 75.9 / 73.4; 640 86.3 / 77.1 / 79.6; 784 104.9 / 99.8 / 90.4.  K = 4096: 160 54.7 / 52.4 / -; 272 95.8 /
-    // 109.2 / 76.8; 352 119.5 / 111.0 / 99.2; 384 130.6 / 113.3 / 114.5.  K = 640: 160 16.9 / 18.1 / -; 272 26.4 / 34.1 / 26.8; 384 34.2 / 35.8 / 36.1; 784
-    // 67.8 / 69.1 / 62.7.
+    // 256 and the rest apart), K = 1280, N = 4096: 160 tiles 23.6 / 25.3 / -; 208 31.2 / 26.4 / -; 272 38.4 / 48.2 / 37.3; 352 47.3 / 48.9 / 41.4; 384 51.4 /
+    // 48.9 / 43.3; 416 56.5 / 50.5 / 51.4; 640 86.3 / 76.6 / 71.5; 672 89.8 / 75.1 / 80.6.  K = 4096: 160 54.7 / 52.4 / -; 272 95.8 / 109.2 / 76.8; 384 130.6 /
+    // 112.6 / 103.1; 400 - / 115.9 / 121.2.  K = 640: 160 16.9 / 18.1 / -; 272 26.4 / 34.1 / 26.8; 384 34.2 / 36.3 / 33.2; 416 37.4 / 36.5 / 37.3.
     if (const int64_t all = tiles(256, 256); all >= 192) {
         constexpr int64_t CUS = 256;
         const int64_t cols = (d->N + 255) / 256, whole = all / CUS * CUS / cols, left = all - whole * cols;
         mv_gemm_i8_desc head = *d, tail = *d;
-        const bool split = whole > 0 && left > 0 && left <= 3 * CUS / 8;
+        const bool split = whole > 0 && left > 0 && left <= CUS / 2;
         if (split) {
             head.M = whole * 256;
             tail.M -= head.M;
@@ -513,6 +512,10 @@ static int launch_gemm_i8_shape(const mv_gemm_i8_desc* d, hipStream_t st) {
                                                                    : launch_gemm_i8<T, 256, 256, 128, 64, 1>(&head, st);
         return rc == MV_OK && split ? launch_gemm_i8_shape<T>(&tail, st) : rc;
     }
+    // 128 x 128 tiles (two blocks per CU) where one round holds them all and they fill more than half of it.  Measured with a residual, N = 4096 (us; the
+    // rules below / 128 x 128): K = 1280, 288 tiles 14.5 / 14.3, 448 19.9 / 15.2, 512 21.1 / 16.1, 544 22.2 / 24.3; K = 4096, 288 31.2 / 28.5, 384 35.0 / 31.8,
+    // 512 52.2 / 38.1, 544 52.3 / 56.3; K = 640, 288 10.3 / 10.6, 384 10.7 / 10.7, 448 13.7 / 11.1; 256 tiles of K = 2048 14.6 / 15.0.
+    if (const int64_t t = tiles(128, 128); t <= 512 && (t > 384 || (t > 256 && d->kp >= 1280))) return launch_gemm_i8<T, 128, 128, 64, 32, 1>(d, st);
     if (tiles(128, 64) >= 512) return launch_gemm_i8<T, 128, 64, 64, 32, 1>(d, st);
     if (tiles(32, 32) <= 512) return launch_gemm_i8<T, 32, 32, 32, 32, 4>(d, st);
     if (tiles(64, 64) <= 256 && d->kp >= 2048) return launch_gemm_i8<T, 64, 64, 32, 32, 4>(d, st);

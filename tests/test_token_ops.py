@@ -910,6 +910,25 @@ def test_linear_i8_large(m, k, n, dt):
 
 
 @gpu
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS)
+@pytest.mark.parametrize("m,k,n", [(1900, 100, 3989), (2048, 1300, 2100), (5848, 260, 4000)], ids=["one_round", "long_k", "left_over"])
+def test_linear_i8_one_round_of_middle_tiles(m, k, n, dt):
+    """tiles of 128 x 128, ragged, alone and for the rows that the largest tiles leave"""
+    from musev_amd import ops
+    x = rnd((m, k), 1, dt)
+    codes = torch.randint(-127, 128, (n, k), generator=torch.Generator().manual_seed(2), dtype=torch.int32).to(torch.int8).to(DEV)
+    ws = ((0.5 + torch.rand(n, generator=torch.Generator().manual_seed(3))) / (73 * math.sqrt(k))).to(DEV)
+    bias, w = rnd((n,), 3, dt), ops.pack_weight_i8(codes, ws)
+    res = torch.randn((m, n + 3), generator=torch.Generator(DEV).manual_seed(4), device=DEV).to(dt)[:, 1:1 + n]
+    for r, act in ((None, ops.MV_ACT_SILU), (res, 0)):
+        got = ops.linear_i8(x, w, bias=bias, residual=r, act=act)
+        torch.cuda.synchronize()
+        for a in range(0, m, 4096):
+            want, bound = linear_oracle(x[a:a + 4096], codes, ws, bias, None if r is None else r[a:a + 4096], act == ops.MV_ACT_SILU)
+            within(got[a:a + 4096], want, bound, what=(m, k, n, a))
+
+
+@gpu
 @pytest.mark.parametrize("m,k,n,dt", [(8200, 300, 8190, torch.float16), (8300, 140, 8190, torch.bfloat16)])
 def test_linear_i8_rows_left_over_by_whole_rounds(m, k, n, dt):
     """the rows behind the last whole round of the largest tiles, added to a residual in place; columns beside the result stay as they were"""
