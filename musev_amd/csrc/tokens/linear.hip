@@ -483,7 +483,7 @@ static int launch_gemm_i8_shape(const mv_gemm_i8_desc* d, hipStream_t st) {
         return MV_OK;
     }
     // The largest tile that fills the chip: 256 x 256 (one block per CU) from three quarters of a round on, 128 x 128 where one round holds them, 128 x 64
-    // (three per CU) from two blocks per CU, 64 x 64 below, where K is long and tiles are few in four groups, and 32 x 32 in four groups up to two per CU.
+    // (three per CU) from two blocks per CU, 64 x 64 below, where K is long and tiles are few in two or four groups, and 32 x 32 in four groups up to two per CU.
     // Measured (us, M x K x N; 256 / 128 x 64 / 64 / 64 in groups / 32 in groups): 8192^3 472 / 655 / 799 / - / -; 26 624 x 1280 x 5120 249 / 315 /
     // 380 / 792 / -; 4096 x 1280 x 2560 27.2 / 25.1 / 32.8 / 62 / -; 2048 x 1280 x 1280 22.9 / 10.3 / 10.8 / 18.4 / 22.6; 512 x 5120 x 1280 60 / 23.0 /
     // 19.8 / 13.9 / 16.3; 512 x 1280 x 1280 22.5 / 8.4 / 6.6 / 7.1 / 9.1; 300 x 5120 x 1280 61 / 19.3 / 14.0 / 11.8 / 10.8; 64 x 1280 x 1280 20 / 8.2 /
@@ -518,7 +518,10 @@ static int launch_gemm_i8_shape(const mv_gemm_i8_desc* d, hipStream_t st) {
     if (const int64_t t = tiles(128, 128); t <= 512 && (t > 384 || (t > 256 && d->kp >= 1280))) return launch_gemm_i8<T, 128, 128, 64, 32, 1>(d, st);
     if (tiles(128, 64) >= 512) return launch_gemm_i8<T, 128, 64, 64, 32, 1>(d, st);
     if (tiles(32, 32) <= 512) return launch_gemm_i8<T, 32, 32, 32, 32, 4>(d, st);
+    // 64 x 64 in groups (us, N = 1280; one / two / four): K = 2048, 240 tiles 7.8 / 7.7 / 7.7, 300 8.6 / 10.0 / 13.5; K = 2560, 260 10.1 / 10.6 / 14.8, 400
+    // 13.1 / 11.9 / 16.7; K = 4096, 240 17.7 / 13.9 / 12.1, 260 17.0 / 13.6 / 20.0, 500 19.1 / 18.3 / 23.1, 520 19.7 / 27.6 / 31.2.
     if (tiles(64, 64) <= 256 && d->kp >= 2048) return launch_gemm_i8<T, 64, 64, 32, 32, 4>(d, st);
+    if (tiles(64, 64) <= 512 && d->kp >= 2560) return launch_gemm_i8<T, 64, 64, 32, 32, 2>(d, st);
     return launch_gemm_i8<T, 64, 64, 32, 32, 1>(d, st);
 }
 

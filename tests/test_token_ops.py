@@ -911,6 +911,22 @@ def test_linear_i8_large(m, k, n, dt):
 
 @gpu
 @pytest.mark.parametrize("dt", DTYPES, ids=IDS)
+@pytest.mark.parametrize("k", [2600, 2817, 4096])
+def test_linear_i8_long_k_in_two_groups(k, dt):
+    """an even and an odd number of steps of K shared by two groups of waves"""
+    from musev_amd import ops
+    m, n = 701, 1501
+    x = rnd((m, k), 1, dt)
+    codes = torch.randint(-127, 128, (n, k), generator=torch.Generator().manual_seed(2), dtype=torch.int32).to(torch.int8).to(DEV)
+    ws = ((0.5 + torch.rand(n, generator=torch.Generator().manual_seed(3))) / (73 * math.sqrt(k))).to(DEV)
+    res, w = rnd((m, n), 4, dt), ops.pack_weight_i8(codes, ws)
+    got = ops.linear_i8(x, w, residual=res)
+    torch.cuda.synchronize()
+    within(got, *linear_oracle(x, codes, ws, None, res, False), what=k)
+
+
+@gpu
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS)
 @pytest.mark.parametrize("m,k,n", [(1900, 100, 3989), (2048, 1300, 2100), (5848, 260, 4000)], ids=["one_round", "long_k", "left_over"])
 def test_linear_i8_one_round_of_middle_tiles(m, k, n, dt):
     """tiles of 128 x 128, ragged, alone and for the rows that the largest tiles leave"""
