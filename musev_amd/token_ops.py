@@ -9,6 +9,7 @@ concurrent calls and several captured graphs never share it.  A graph refers to 
 """
 from __future__ import annotations
 
+import collections
 import ctypes as C
 import heapq
 import math
@@ -167,16 +168,16 @@ def _lens(v, name: str) -> List[int]:
 
 
 TILE_ROWS = 128   # packed rows per item
-# Keys of an item that is worth a split: an item's parts each write and the join reads back (d + 2) fp32 per row.
+# The least keys of a part: an item's parts each write and the join reads back (d + 2) fp32 per row.
 MIN_PART = 128
 BLOCKS = 512      # two blocks on each of the 256 CUs
 LATE_PART = 1024  # keys of a part of a block that would run late
 
 
-def _plan_items(ql: Sequence[int], kl: Sequence[int], group: int, kv_heads: int, causal: bool):
+def _plan_items(ql: Sequence[int], kl: Sequence[int], group: int, kv_heads: int, causal: bool, d: int = 128):
     """(items, joins, workspace rows): see include/musev_tokens.h.  An item's keys end with what its last query sees.  Where the items alone would
-    leave CUs idle, or one item would outlast the others, its keys are split into parts of about 1 / BLOCKS of all the work (`_late_parts`: or
-    where a last round would hold few of them); the longest items come first."""
+    leave CUs idle, or one item would outlast the others, its keys are split into parts of 1 / BLOCKS of all the work or more (`_cheapest_parts`;
+    `_late_parts`: or where a last round would hold few of them); the longest items come first."""
     tiles, q_row, k_row = [], 0, 0
     for q, kv in zip(ql, kl):
         for m0 in range(0, q * group, TILE_ROWS):
@@ -187,6 +188,8 @@ def _plan_items(ql: Sequence[int], kl: Sequence[int], group: int, kv_heads: int,
     part = max(MIN_PART, -(-sum(t[5] for t in tiles) * kv_heads // BLOCKS))
     part = -(-part // 64) * 64
     parts = [max(1, (t[5] + part // 2) // part) for t in tiles]
+    if max(parts, default=1) > 1:
+        parts = _cheapest_parts([(min(TILE_ROWS, t[1] * group - t[4]), t[5]) for t in tiles], part, kv_heads, d)
     if max(parts, default=1) == 1 and BLOCKS < len(tiles) * kv_heads <= 8 * BLOCKS:
         parts = _late_parts([t[5] for t in tiles], kv_heads)
     for (q_row, q, k_row, kv, m0, end), n in zip(tiles, parts):
@@ -202,6 +205,28 @@ def _plan_items(ql: Sequence[int], kl: Sequence[int], group: int, kv_heads: int,
         ws += n * rows
     items.sort(key=lambda i: i[5] - i[6])
     return items, joins, ws
+
+
+def _cheapest_parts(tiles: Sequence[Tuple[int, int]], part: int, kv_heads: int, d: int) -> List[int]:
+    """Parts of every tile (its rows, its keys), of ``part`` keys or a multiple of that, whichever costs least: the longest part's tiles of 64 keys
+    1.22 us each (at head dim 128), the join 2.7 us and 0.64 us for each MB of sums that parts hand over -- fitted to 24 sets of lengths at five sizes
+    of parts, within 10 %.  Measured (us, parts of 1 / BLOCKS / cheapest): 587 tokens of 32 / 4 heads x 104 24.2 / 16.7; 3 x 700 of 8 / 2 x 64 20.0 / 14.8;
+    4 x 300 of 8 x 64 12.9 / 9.7; 128 tokens over 8192 keys of 8 x 128 24.8 / 22.9; 1500 of 4 / 1 x 128 23.1 / 20.1; one token per request: the same."""
+    counts = collections.Counter(tiles)
+    per_tile = 1.22 * (0.35 + 0.65 * -(-d // 16) / 8)
+    least = sum(end * n for (_, end), n in counts.items()) * kv_heads // BLOCKS   # (keys of a block if all were busy to the end)
+    best, choice = math.inf, part
+    for f in (1.0, 1.5, 2.0, 3.0, 4.0, 6.0, 8.0, math.inf):
+        size, longest, shared = f * part, least, 0
+        for (rows, end), n in counts.items():
+            k = max(1, int(end / size + 0.5))
+            longest = max(longest, -(-end // k))
+            if k > 1:
+                shared += rows * k * n
+        cost = per_tile * -(-longest // 64) + (2.7 + 0.64e-6 * 4 * shared * kv_heads * (d + 2) if shared else 0.0)
+        if cost < 0.97 * best:
+            best, choice = cost, size
+    return [max(1, int(end / choice + 0.5)) for _, end in tiles]
 
 
 def _late_parts(ends: Sequence[int], kv_heads: int) -> List[int]:
@@ -259,7 +284,7 @@ def attention_plan(q_lens: Sequence[int], kv_lens: Optional[Sequence[int]] = Non
     dev = torch.device(device)
     if dev.type == "cuda" and dev.index is None:
         dev = torch.device("cuda", torch.cuda.current_device())
-    items, joins, ws_rows = _plan_items(ql, kl, heads // kv_heads, kv_heads, bool(causal))
+    items, joins, ws_rows = _plan_items(ql, kl, heads // kv_heads, kv_heads, bool(causal), d)
     table = torch.tensor((items + joins) or [(0,) * 8], dtype=torch.int32).to(dev)   # (one upload)
     n = len(items)
     return AttentionPlan(ql, kl, heads, kv_heads, d, bool(causal), scale, table[:n], table[n:n + len(joins)], max((j[6] for j in joins), default=0), ws_rows)

@@ -175,6 +175,17 @@ def test_plan_covers_every_visible_key_once(seed):
         assert plan._workspace == _lib.load().mv_attention_packed_workspace_bytes(d.ws_rows, kvh, 64)
 
 
+@pytest.mark.parametrize("ql,kl,group,kvh,d,split", [([300] * 4, [300] * 4, 1, 8, 64, False), ([700] * 3, [700] * 3, 4, 2, 64, False), ([1], [8192], 4, 8, 128, True),
+                                                     ([128], [8192], 1, 8, 128, True), ([1500], [1500], 4, 1, 128, True), ([16] * 8, [2000] * 8, 4, 2, 128, True),
+                                                     ([1], [100], 1, 1, 64, False), ([0, 3], [50, 0], 1, 1, 64, False)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_plan_splits_where_the_parts_pay(ql, kl, group, kvh, d, split, causal):
+    from musev_amd import token_ops as to
+    items, joins, ws = to._plan_items(ql, kl, group, kvh, causal, d)
+    assert bool(joins) == split
+    _cover(items, joins, ws, ql, kl, group, causal)
+
+
 LATE = {   # lengths, heads per key / value head, key / value heads, causal -> tiles that are split
     "few_late": ([6000], [6000], 1, 12, False, 5),
     "many_late": ([13312], [13312], 1, 8, False, 40),
