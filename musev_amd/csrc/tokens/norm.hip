@@ -1,31 +1,34 @@
 // tokens/norm.hip -- the gated residual norm (include/musev_tokens.h: mv_gated_residual_norm).
 #include "tokens.h"
 
-// sums over a row held by WAVES waves
-template <int WAVES>
+// sums over a row held by 16 or 32 lanes, a wave or four waves
+template <int LANES>
 __device__ __forceinline__ float row_sum(float v, float* red) {
-    v = wave_sum_fast(v);
-    if constexpr (WAVES > 1) {
+    if constexpr (LANES == 16) v = lanes16_sum(v);
+    else if constexpr (LANES == 32) {
+        v = lanes16_sum(v);
+        v += __shfl_xor(v, 16, 64);
+    } else v = wave_sum_fast(v);
+    if constexpr (LANES > 64) {
         __syncthreads();   // (the previous sum's readers are through)
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
         __syncthreads();
         v = red[0];
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) v += red[w];
+        for (int w = 1; w < LANES / 64; ++w) v += red[w];
     }
     return v;
 }
 
-// A row stays in registers from its one read to its one write: NV chunks of 8 columns per lane, WAVES waves per row, 4 / WAVES rows per
+// A row stays in registers from its one read to its one write: NV chunks of 8 columns per lane, LANES lanes per row, 256 / LANES rows per
 // block.  Both norms' statistics are formed in two passes over the registers (mean, then squared deviations), in fp32.  Bound by memory:
 // x and f in, s and h out.
-template <typename T, int NV, int WAVES>
+template <typename T, int NV, int LANES>
 __global__ __launch_bounds__(256) void gated_norm_kernel(const mv_gated_norm_desc p, const bool cold) {
     __shared__ float red[4];
-    constexpr int LANES = 64 * WAVES;
     const int lane = threadIdx.x % LANES, c = p.c;
-    const int64_t row = (int64_t)blockIdx.x * (4 / WAVES) + threadIdx.x / LANES;
-    if (row >= p.rows) return;   // (a whole wave; with WAVES = 4 the grid is exact)
+    const int64_t row = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    if (row >= p.rows) return;   // (all lanes of a row; with four waves per row the grid is exact)
     T* so = (T*)p.stream_out + row * p.lds;
     T* ho = (T*)p.norm_out + row * p.ldh;
     const int64_t g = p.group_index ? (int64_t)p.group_index[row] : p.rows_per_group > 0 ? (int64_t)((unsigned)row / (unsigned)p.rows_per_group) : 0;
@@ -60,7 +63,7 @@ __global__ __launch_bounds__(256) void gated_norm_kernel(const mv_gated_norm_des
             for (int j = 0; j < NV; ++j)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) t += v[j][e];
-            mean = row_sum<WAVES>(t, red) * inv_c;
+            mean = row_sum<LANES>(t, red) * inv_c;
         }
         float t = 0.f;
 #pragma unroll
@@ -72,7 +75,7 @@ __global__ __launch_bounds__(256) void gated_norm_kernel(const mv_gated_norm_des
                 t = __builtin_fmaf(d, d, t);
             }
         }
-        rstd = 1.0f / sqrtf(row_sum<WAVES>(t, red) * inv_c + eps);
+        rstd = 1.0f / sqrtf(row_sum<LANES>(t, red) * inv_c + eps);
     };
     float mean, rstd;
     if (p.post) statistics(y, p.post_eps, mean, rstd);
@@ -139,27 +142,33 @@ __global__ __launch_bounds__(256) void gated_norm_kernel(const mv_gated_norm_des
     }
 }
 
-template <typename T, int NV, int WAVES>
+template <typename T, int NV, int LANES>
 static void launch_norm(const mv_gated_norm_desc* d, hipStream_t st) {
-    constexpr int R = 4 / WAVES;
+    constexpr int R = 256 / LANES;
     // (53 248 x 1280, 273 MB of inputs: 123 -> 113 us where other work ran in between; 26 624 x 1280, half of that and still in the cache: 57 -> 65)
     const bool cold = d->rows * d->c * 4 > COLD_BYTES;
-    gated_norm_kernel<T, NV, WAVES><<<(unsigned)((d->rows + R - 1) / R), 256, 0, st>>>(*d, cold);
+    gated_norm_kernel<T, NV, LANES><<<(unsigned)((d->rows + R - 1) / R), 256, 0, st>>>(*d, cold);
 }
 
 // A wave holds a row of up to 1536 columns where there are rows enough to fill the chip; the block's four waves share it otherwise.  Measured (us,
 // rms, both norms, one / four waves per row): 1 x 1280 6.3 / 3.9; 1024 x 1280 7.9 / 5.6; 2048 x 640 6.5 / 6.8; 4099 x 1001 11.3 / 13.1; 16 000 x 1280
-// 37 / 41; 16 000 x 2048 55 / 47.
+// 37 / 41; 16 000 x 2048 55 / 47.  Narrow rows share a wave (layer, indexed groups; a wave per row / shared): 37 590 x 44 40.4 / 14.7; 50 000 x 128 32.6 /
+// 11.8; 1 x 128 3.7 / 3.6; 20 000 x 200 16.2 / 9.7; 200 x 256 4.3 / 4.2; with several chunks per lane only where rows are many: 20 000 x 320 17.5 / 13.8,
+// 100 000 x 512 80 / 70, but 2000 x 320 5.2 / 7.7, 4000 x 512 6.5 / 7.3.
 template <typename T>
 static void launch_norm_width(const mv_gated_norm_desc* d, hipStream_t st) {
     const int c = d->c;
-    if (c <= 512) launch_norm<T, 1, 1>(d, st);
-    else if (c > 1536 ? c <= 2048 : d->rows <= 2048) launch_norm<T, 1, 4>(d, st);
-    else if (c <= 1024) launch_norm<T, 2, 1>(d, st);
-    else if (c <= 1536) launch_norm<T, 3, 1>(d, st);
-    else if (c <= 4096) launch_norm<T, 2, 4>(d, st);
-    else if (c <= 8192) launch_norm<T, 4, 4>(d, st);
-    else launch_norm<T, 8, 4>(d, st);
+    if (c <= 128) launch_norm<T, 1, 16>(d, st);
+    else if (c <= 256) launch_norm<T, 1, 32>(d, st);
+    else if (c <= 384 && d->rows > 16384) launch_norm<T, 3, 16>(d, st);
+    else if (c <= 512 && d->rows > 16384) launch_norm<T, 2, 32>(d, st);
+    else if (c <= 512) launch_norm<T, 1, 64>(d, st);
+    else if (c > 1536 ? c <= 2048 : d->rows <= 2048) launch_norm<T, 1, 256>(d, st);
+    else if (c <= 1024) launch_norm<T, 2, 64>(d, st);
+    else if (c <= 1536) launch_norm<T, 3, 64>(d, st);
+    else if (c <= 4096) launch_norm<T, 2, 256>(d, st);
+    else if (c <= 8192) launch_norm<T, 4, 256>(d, st);
+    else launch_norm<T, 8, 256>(d, st);
 }
 
 extern "C" int mv_gated_residual_norm(const mv_gated_norm_desc* d, void* stream) {

@@ -71,16 +71,20 @@ __device__ __forceinline__ void store8_stream(T* p, int n, const float* in) {
     } else store8(p, n, in);
 }
 
-// sum over a wave: within 16 lanes by cross-lane moves of the VALU, then two exchanges
+// sums over 16 lanes (cross-lane moves of the VALU) and over a wave (two exchanges more)
 template <int CTRL>
 __device__ __forceinline__ float lane_move(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
 }
-__device__ __forceinline__ float wave_sum_fast(float v) {
+__device__ __forceinline__ float lanes16_sum(float v) {
     v += lane_move<0xB1>(v);    // lanes 1 0 3 2 of a quad
     v += lane_move<0x4E>(v);    // lanes 2 3 0 1
     v += lane_move<0x141>(v);   // mirrored within 8
     v += lane_move<0x140>(v);   // mirrored within 16
+    return v;
+}
+__device__ __forceinline__ float wave_sum_fast(float v) {
+    v = lanes16_sum(v);
     v += __shfl_xor(v, 16, 64);
     v += __shfl_xor(v, 32, 64);
     return v;

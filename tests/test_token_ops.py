@@ -778,6 +778,26 @@ def test_gated_norm(c, kind, dt):
 
 
 @gpu
+@pytest.mark.parametrize("kind,dt", [("layer", torch.float16), ("rms", torch.bfloat16)], ids=["layer-fp16", "rms-bf16"])
+@pytest.mark.parametrize("rows", [35, 16389])
+@pytest.mark.parametrize("c", [3, 100, 128, 129, 250, 256, 257, 384, 385, 511, 512])
+def test_gated_norm_of_rows_that_share_a_wave(c, rows, kind, dt):
+    """narrow rows side by side in a wave, some of no group (NaN) between those that have one; in place"""
+    from musev_amd import ops
+    x, f = rnd((rows, c), 41, dt), rnd((rows, c), 42, dt, 0.7)
+    gate, scale, shift = (rnd((5, c), 43 + i, dt, 0.5) for i in range(3))
+    post, pre = (rnd((c,), 50, dt, 0.3) + 1, rnd((c,), 51, dt, 0.3), 1e-5), (rnd((c,), 52, dt, 0.3) + 1, None, 1e-6)
+    idx = torch.randint(-1, 6, (rows,), generator=torch.Generator().manual_seed(3), dtype=torch.int32).to(DEV)
+    has = (idx >= 0) & (idx < 5)
+    want = norm_oracle(x, f, kind, 0.75, post, pre, gate, scale, shift, idx.long().clamp(0, 4))
+    s, h = ops.gated_residual_norm(x, f, kind=kind, alpha=0.75, post=post, pre=pre, gate=gate, scale=scale, shift=shift, group_index=idx, out=x, norm_out=f)
+    torch.cuda.synchronize()
+    for got, (w, b) in zip((s, h), want):
+        assert bool(got[~has].isnan().all())
+        within(got[has], w[has], b[has], what=(c, rows, kind))
+
+
+@gpu
 @pytest.mark.parametrize("c", [40, 320, 1001, 4100])
 def test_gated_norm_in_place_strided_and_unaligned(c):
     from musev_amd import ops
