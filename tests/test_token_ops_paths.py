@@ -1,0 +1,116 @@
+"""More of the token-transformer operators (musev_amd.token_ops): the forms that only large, split or unusual calls reach, and the refusals
+beside them.  Oracles and bounds are those of test_token_ops; a bound of its own is derived where it stands."""
+import math
+
+import pytest
+import torch
+
+from test_token_ops import DEV, DTYPES, IDS, attention_inputs, attention_oracle, gpu, norm_oracle, rnd, rotary_oracle, within
+
+
+def randn(shape, seed, dt, scale=1.0):
+    """rnd() made on the GPU: large inputs"""
+    return (torch.randn(shape, generator=torch.Generator(DEV).manual_seed(seed), device=DEV) * scale).to(dt)
+
+
+# ---- packed attention: parts of split keys ------------------------------------------------------------------------------------------
+SPLIT = {   # q_lens, kv_lens, heads, kv_heads: a join of many parts (shared by eight threads) and of few
+    "many_parts": ([1, 3], [8192, 4000], 8, 2),
+    "few_parts": ([40, 130], [1500, 1100], 4, 2),
+}
+
+
+def split_plan(name, d, causal=True, scale=None):
+    from musev_amd import ops
+    ql, kl, heads, kvh = SPLIT[name]
+    plan = ops.attention_plan(ql, kl, heads=heads, kv_heads=kvh, d=d, causal=causal, scale=scale)
+    assert plan.n_joins > 0 and (plan.ws_rows > 16 * plan.n_joins * plan.join_rows) == (name == "many_parts")
+    return plan
+
+
+@gpu
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS)
+@pytest.mark.parametrize("d", [64, 80, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")], ids=["nan", "inf", "-inf"])
+@pytest.mark.parametrize("name", list(SPLIT))
+def test_what_is_not_seen_does_not_reach_the_output_of_split_keys(name, bad, d, dt):
+    """the last key of a sequence (only its last query sees it) and the rows behind the last sequence hold values that are not finite"""
+    from musev_amd import ops
+    ql, kl, heads, kvh = SPLIT[name]
+    plan = split_plan(name, d)
+    q, k, v = attention_inputs(ql, kl, heads, kvh, d, dt, 9)
+    pad = torch.full((70, kvh * d), bad, dtype=dt, device=DEV)
+    clean, bound = attention_oracle(q, k, v, ql, kl, heads, kvh, d, True)
+    last = sum(kl) - 1
+    k2, v2 = torch.cat([k, pad]), torch.cat([v, pad])
+    k2[last], v2[last] = bad, bad
+    got = ops.attention_packed(plan, q, k2, v2)
+    torch.cuda.synchronize()
+    within(got[:-1], clean[:-1], bound[:-1])
+    v2 = torch.cat([v, pad])       # V alone: a visible value shows in its own column only
+    v2[last, d + 5] = bad          # (of the second key / value head)
+    got = ops.attention_packed(plan, q, torch.cat([k, pad]), v2)
+    torch.cuda.synchronize()
+    rest = torch.ones_like(got, dtype=torch.bool)
+    rest.view(-1, heads, d)[-1, heads // 2:, 5] = False
+    seen = got[~rest]
+    assert bool((torch.isnan(seen) if math.isnan(bad) else seen == bad).all())
+    within(got[rest], clean[rest], bound[rest])
+
+
+# ---- rotary positions: several tokens per block, results and inputs past the caches ----------------------------------------------
+MANY = {   # tokens, heads, kv_heads, d, sections
+    "four_tokens_per_block": (4097, 1, 1, 16, [16]),
+    "eight_tokens_per_block": (20003, 2, 1, 24, [8, 14]),
+    "two_tokens_per_block": (2049, 6, 3, 40, [8, 8, 16]),
+    "results_past_the_caches": (20001, 10, 3, 128, [32, 48, 48]),
+    "inputs_past_the_last_cache": (20001, 45, 8, 128, [32, 48, 44]),
+}
+
+
+@gpu
+@pytest.mark.parametrize("pairing", ["adjacent", "halves"])
+@pytest.mark.parametrize("name", list(MANY))
+def test_rotary_of_many_tokens(name, pairing):
+    """aligned and one element off it, apart and in place; the last block holds fewer tokens than the others"""
+    from musev_amd import ops
+    n, heads, kvh, d, sec = MANY[name]
+    dt = torch.float16 if pairing == "halves" else torch.bfloat16
+    pos = torch.randint(0, 4096, (n, len(sec)), generator=torch.Generator(DEV).manual_seed(1), dtype=torch.int32, device=DEV)
+    table = ops.rotary_table(sec)
+    wide = randn((n, (heads + kvh) * d + 3), 2, dt)
+    for off in (0, 1):
+        src = wide[:, off:off + (heads + kvh) * d]
+        q, k = src[:, :heads * d], src[:, heads * d:]
+        keep = wide.clone()
+        oq, ok = ops.rotary_axes(q, k, pos, table, heads=heads, kv_heads=kvh, d=d, pairing=pairing)
+        torch.cuda.synchronize()
+        for got, x, h in ((oq, q, heads), (ok, k, kvh)):
+            for a in range(0, n, 4096):
+                within(got[a:a + 4096], *rotary_oracle(x[a:a + 4096], pos[a:a + 4096], sec, 10000.0, False, h, d, pairing), what=(name, off, a))
+        ops.rotary_axes(q, k, pos, table, heads=heads, kv_heads=kvh, d=d, pairing=pairing, out_q=q, out_k=k)
+        torch.cuda.synchronize()
+        assert torch.equal(q, oq) and torch.equal(k, ok)
+        cols = slice(off + (heads + kvh) * d, None)
+        assert torch.equal(wide[:, :off], keep[:, :off]) and torch.equal(wide[:, cols], keep[:, cols])
+        wide = keep
+
+
+# ---- gated residual norm: inputs past the last-level cache --------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("c,off,dt", [(1001, 3, torch.float16), (1280, 0, torch.bfloat16), (44, 1, torch.float16), (4100, 2, torch.bfloat16)])
+def test_gated_norm_of_inputs_past_the_last_cache(c, off, dt):
+    """in place, odd widths and columns off their alignment, a row per wave and rows that share one"""
+    from musev_amd import ops
+    rows = (256 << 20) // (4 * c) + 61
+    x, f = (randn((rows, c + 5), s, dt)[:, off:off + c] for s in (1, 2))
+    gate, scale, shift = (rnd((7, c), 43 + i, dt, 0.5) for i in range(3))
+    pre, per = (rnd((c,), 52, dt, 0.3) + 1, None, 1e-6), -(-rows // 7)
+    x0, f0 = x.clone(), f.clone()
+    s, h = ops.gated_residual_norm(x, f, alpha=0.75, pre=pre, gate=gate, scale=scale, shift=shift, rows_per_group=per, out=x, norm_out=f)
+    torch.cuda.synchronize()
+    for a in range(0, rows, 200_000_000 // (8 * c)):
+        e = min(rows, a + 200_000_000 // (8 * c))
+        ws, wh = norm_oracle(x0[a:e], f0[a:e], "layer", 0.75, None, pre, gate, scale, shift, torch.arange(a, e, device=DEV) // per)
+        within(s[a:e], *ws, what=("s", c, a))
+        within(h[a:e], *wh, what=("h", c, a))
