@@ -347,16 +347,16 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const mv_attn_packe
             }
 #pragma unroll
             for (int u = 0; u < 4; ++u)
-                if (s + G * u >= jn.parts) w[u] = float2v{-3.0e38f, 0.f};
+                if (s + G * u >= jn.parts) w[u] = float2v{-3.0e38f, 0.f}, v[u] = float4v{0.f, 0.f, 0.f, 0.f};
             const float mn = fmaxf(fmaxf(mm, fmaxf(w[0].x, w[1].x)), fmaxf(w[2].x, w[3].x)), old = __builtin_amdgcn_exp2f(mm - mn);
             mm = mn;
             ll *= old;
             o *= old;
+            // (a part that saw no key holds zeros; one whose weight vanishes counts all the same: 0 x infinity is NaN, as it is where keys are not split)
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const float a = w[u].y != 0.f ? __builtin_amdgcn_exp2f(w[u].x - mn) : 0.f;   // (a part that saw no key adds nothing)
+                const float a = __builtin_amdgcn_exp2f(w[u].x - mn);
                 ll = __builtin_fmaf(a, w[u].y, ll);
-                if (a == 0.f) continue;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(a, v[u][e], o[e]);
             }
@@ -371,17 +371,14 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const mv_attn_packe
         float mn = mm;
 #pragma unroll
         for (int u = 0; u < G - 1; ++u) mn = fmaxf(mn, other_ml[u][own].x);
-        const float a0 = ll != 0.f ? __builtin_amdgcn_exp2f(mm - mn) : 0.f;
+        const float a0 = __builtin_amdgcn_exp2f(mm - mn);
         ll *= a0;
-        if (a0 != 1.f)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = a0 != 0.f ? o[e] * a0 : 0.f;
+        o *= a0;
 #pragma unroll
         for (int u = 0; u < G - 1; ++u) {
             const float2v w = other_ml[u][own];
-            const float a = w.y != 0.f ? __builtin_amdgcn_exp2f(w.x - mn) : 0.f;
+            const float a = __builtin_amdgcn_exp2f(w.x - mn);
             ll = __builtin_fmaf(a, w.y, ll);
-            if (a == 0.f) continue;
             const float4v v = other_o[u][own];
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(a, v[e], o[e]);

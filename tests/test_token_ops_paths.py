@@ -58,6 +58,35 @@ def test_what_is_not_seen_does_not_reach_the_output_of_split_keys(name, bad, d, 
     within(got[rest], clean[rest], bound[rest])
 
 
+@gpu
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")], ids=["nan", "inf", "-inf"])
+@pytest.mark.parametrize("name", list(SPLIT))
+def test_a_visible_value_that_is_not_finite_shows_however_little_it_weighs(name, bad, dt, monkeypatch):
+    """one key outweighs all others by e^512: the others' weights vanish, and 0 x infinity is NaN -- with the keys split into parts as without"""
+    from musev_amd import ops, token_ops
+    ql, kl, heads, kvh = SPLIT[name]
+    d = 64
+    q = torch.ones(sum(ql), heads * d, dtype=dt, device=DEV)
+    k = torch.zeros(sum(kl), kvh * d, dtype=dt, device=DEV)
+    v = rnd((sum(kl), kvh * d), 3, dt)
+    k[600], k[kl[0] + 600] = 8, 8
+    v[10, 5], v[kl[0] + 10, 5] = bad, bad
+    plans = [split_plan(name, d, scale=1.0)]
+    monkeypatch.setattr(token_ops, "MIN_PART", 1 << 20)
+    plans.append(ops.attention_plan(ql, kl, heads=heads, kv_heads=kvh, d=d, scale=1.0))
+    assert plans[1].n_joins == 0
+    for plan in plans:
+        got = ops.attention_packed(plan, q, k, v).view(-1, heads, d)
+        torch.cuda.synchronize()
+        hit = torch.zeros_like(got, dtype=torch.bool)
+        hit[:, :heads // kvh, 5] = True
+        assert not bool(torch.isfinite(got[hit]).any()), plan.n_joins
+        want = torch.cat([v[600].view(kvh, 1, d).expand(kvh, heads // kvh, d).reshape(1, heads, d).expand(ql[0], -1, -1),
+                          v[kl[0] + 600].view(kvh, 1, d).expand(kvh, heads // kvh, d).reshape(1, heads, d).expand(ql[1], -1, -1)])
+        assert torch.equal(got[~hit], want[~hit]), plan.n_joins
+
+
 # ---- rotary positions: several tokens per block, results and inputs past the caches ----------------------------------------------
 MANY = {   # tokens, heads, kv_heads, d, sections
     "four_tokens_per_block": (4097, 1, 1, 16, [16]),
