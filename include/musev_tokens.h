@@ -27,7 +27,7 @@ int mv_tokens_abi_version(void);
  * A (sequence, key / value head) has q_len * group packed rows: row r is query r / group, head r % group of the group.
  * `items` (device, 8 int32 each), made by musev_amd.token_ops.attention_plan, 128 packed rows each:
  *   {first query row, q_len, first key row, kv_len, first packed row, key begin, key end, first workspace row or -1}
- * An item with a workspace row writes its unnormalised sums and the rows' references / sums there; `joins` (device, 8 int32 each:
+ * An item with a workspace row writes its unnormalised sums and the rows' references (in scores) and sums of weights there; `joins` (device, 8 int32 each:
  *   {first query row, q_len, kv_len, first packed row, first workspace row, parts, rows per part, 0}) says which parts make up which rows.
  * Rows must be 16-byte aligned.                                                                                                        */
 typedef struct mv_attn_packed_desc {

@@ -31,6 +31,9 @@ template <typename T> struct ExpBits;   // both elements of a dword: exponent ma
 template <> struct ExpBits<half_t> { static constexpr unsigned mask = 0x7c007c00u, one = 0x04000400u; };
 template <> struct ExpBits<bf16_t> { static constexpr unsigned mask = 0x7f807f80u, one = 0x00800080u; };
 
+// a score's factor to powers of two
+__device__ __forceinline__ float score_factor(float scale) { return fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-30f); }
+
 template <bool B> struct Masked { static constexpr bool value = B; };
 
 // K16: 16-column steps of the head dim
@@ -70,7 +73,7 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(const mv_attn_
     const int lim_hi = __builtin_amdgcn_readlane(lim, 31);
 
     // ---- Q (second operand of S^T): row in the lane, 8 columns per half wave and step; a negative scale turns its sign here ----
-    const float c = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-30f);   // scores in powers of two
+    const float c = score_factor(p.scale);
     V8 qf[K16];
     {
         const T* q = (const T*)p.q + (int64_t)(it.q_row + qi) * p.ldq + (int64_t)hq * p.d;
@@ -294,7 +297,7 @@ __global__ __launch_bounds__(256, 2) void attention_packed_kernel(const mv_attn_
             }
         if (h == 0) {
             float* wml = ws + (int64_t)p.kv_heads * p.ws_rows * p.d + at * 2;
-            wml[0] = m * c;
+            wml[0] = m;
             wml[1] = l;
         }
         return;
@@ -333,6 +336,15 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const mv_attn_packe
     const int64_t first = (int64_t)kvh * p.ws_rows + jn.ws_row;
     const float* ml = ws + (int64_t)p.kv_heads * p.ws_rows * p.d + (first + row) * 2;
     const float* sums = ws + first * p.d + (int64_t)x * 4;
+    // Weight of sums formed with reference m beside those with `top`: 2 to the difference of the references in the exponent.  Those are what the sums were
+    // formed with: m c rounded, of references up to 2^12; m c itself beyond, where its rounding would be part of the weight (at 2^21 by up to 9 %), so the
+    // difference is formed first.
+    const float c = score_factor(p.scale);
+    auto weight = [&](float m, float top) __attribute__((always_inline)) {
+#pragma clang fp contract(off)
+        const float mc = m * c, tc = top * c;
+        return __builtin_amdgcn_exp2f(fabsf(tc) > 0x1p12f ? (m - top) * c : mc - tc);
+    };
     float mm = -3.0e38f, ll = 0.f;
     float4v o = {0.f, 0.f, 0.f, 0.f};
     if (valid)
@@ -348,14 +360,14 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const mv_attn_packe
 #pragma unroll
             for (int u = 0; u < 4; ++u)
                 if (s + G * u >= jn.parts) w[u] = float2v{-3.0e38f, 0.f}, v[u] = float4v{0.f, 0.f, 0.f, 0.f};
-            const float mn = fmaxf(fmaxf(mm, fmaxf(w[0].x, w[1].x)), fmaxf(w[2].x, w[3].x)), old = __builtin_amdgcn_exp2f(mm - mn);
+            const float mn = fmaxf(fmaxf(mm, fmaxf(w[0].x, w[1].x)), fmaxf(w[2].x, w[3].x)), old = weight(mm, mn);
             mm = mn;
             ll *= old;
             o *= old;
             // (a part that saw no key holds zeros; one whose weight vanishes counts all the same: 0 x infinity is NaN, as it is where keys are not split)
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const float a = __builtin_amdgcn_exp2f(w[u].x - mn);
+                const float a = weight(w[u].x, mn);
                 ll = __builtin_fmaf(a, w[u].y, ll);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(a, v[u][e], o[e]);
@@ -371,13 +383,13 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const mv_attn_packe
         float mn = mm;
 #pragma unroll
         for (int u = 0; u < G - 1; ++u) mn = fmaxf(mn, other_ml[u][own].x);
-        const float a0 = __builtin_amdgcn_exp2f(mm - mn);
+        const float a0 = weight(mm, mn);
         ll *= a0;
         o *= a0;
 #pragma unroll
         for (int u = 0; u < G - 1; ++u) {
             const float2v w = other_ml[u][own];
-            const float a = __builtin_amdgcn_exp2f(w.x - mn);
+            const float a = weight(w.x, mn);
             ll = __builtin_fmaf(a, w.y, ll);
             const float4v v = other_o[u][own];
 #pragma unroll

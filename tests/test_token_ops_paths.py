@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_token_ops import DEV, DTYPES, IDS, attention_inputs, attention_oracle, gpu, norm_oracle, rnd, rotary_oracle, within
+from test_token_ops import DEV, DTYPES, IDS, attention_inputs, attention_oracle, gpu, half_step, norm_oracle, rnd, rotary_oracle, subnormal, within
 
 
 def randn(shape, seed, dt, scale=1.0):
@@ -85,6 +85,37 @@ def test_a_visible_value_that_is_not_finite_shows_however_little_it_weighs(name,
         want = torch.cat([v[600].view(kvh, 1, d).expand(kvh, heads // kvh, d).reshape(1, heads, d).expand(ql[0], -1, -1),
                           v[kl[0] + 600].view(kvh, 1, d).expand(kvh, heads // kvh, d).reshape(1, heads, d).expand(ql[1], -1, -1)])
         assert torch.equal(got[~hit], want[~hit]), plan.n_joins
+
+
+@gpu
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS)
+@pytest.mark.parametrize("each", [2.0 ** 8, 2.0 ** 12, 2.0 ** 15 - 2.0 ** 7])
+@pytest.mark.parametrize("name", list(SPLIT))
+def test_parts_of_large_scores_weigh_as_they_should(name, each, dt):
+    """Scores are whole numbers 63 each + 0 .. 3, exact in fp32 in any order: only their differences decide.  The keys' values say which score
+    a key has.  Bound: the weights' rounding to the type (u; all are at least
+    e^-3 of the largest, so none is subnormal), exponents (s - m) c with |s - m| <= 3 (2^-20), the fp32 sums (2^-19), as in
+    attention_oracle without its term for the scores' error"""
+    from musev_amd import ops
+    ql, kl, heads, kvh = SPLIT[name]
+    d = 64
+    q = torch.ones(sum(ql), heads * d, dtype=dt, device=DEV)
+    k = torch.full((sum(kl), kvh, d), each, dtype=dt, device=DEV)
+    level = torch.cat([torch.arange(n, device=DEV) // 320 % 4 for n in kl])        # (runs of keys: parts have different maxima)
+    k[:, :, -1] = level[:, None].to(dt)
+    v = torch.zeros(sum(kl), kvh, d, dtype=dt, device=DEV)
+    v[torch.arange(sum(kl), device=DEV), :, level] = 1.0
+    plan = split_plan(name, d, causal=False, scale=1.0)
+    got = ops.attention_packed(plan, q, k.view(-1, kvh * d), v.view(-1, kvh * d)).view(-1, heads, d)
+    torch.cuda.synchronize()
+    want = torch.zeros(sum(ql), heads, d, dtype=torch.float64, device=DEV)
+    for i in range(2):
+        lv = level[sum(kl[:i]):sum(kl[:i + 1])]
+        w = torch.exp(lv.double() - 3)
+        for x in range(4):
+            want[sum(ql[:i]):sum(ql[:i + 1]), :, x] = (w * (lv == x)).sum() / w.sum()
+    u = half_step(dt)
+    within(got, want, (2 * u + 2.0 ** -18) * want + subnormal(dt), what=each)
 
 
 # ---- rotary positions: several tokens per block, results and inputs past the caches ----------------------------------------------
