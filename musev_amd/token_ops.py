@@ -1,7 +1,8 @@
 """Token-transformer operators over the C ABI of include/musev_tokens.h: packed attention, rotary positions with several axes, the gated
 residual norm and the int8 projection.  They are part of :mod:`musev_amd.ops` (``from musev_amd import ops; ops.attention_packed(...)``)
 and follow its manner: 2-D row matrices with unit inner stride, no CPU path, launches on the current stream of the tensors' device.
-fp16 and bf16; forward only, like the rest of the framework: a tensor that requires gradients is refused while gradients are recorded.
+fp16 and bf16; forward only, like the rest of the framework: a tensor that requires gradients is refused while gradients are recorded, and
+so is one that carries a forward-mode tangent.
 
 Each call reads its tensors on the stream it is made on: a tensor made on another stream has to be finished there first.  Nothing is kept
 between calls; what a call needs besides its arguments is allocated for that call (inside a graph capture: from the capture's pool), so
@@ -18,6 +19,7 @@ import struct
 from typing import Callable, List, Optional, Sequence, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import MV_ACT_NONE, MV_ACT_SILU, AttnPackedDesc, GatedNormDesc, GemmI8Desc, LinearI8Desc, RotaryDesc, check
@@ -64,9 +66,16 @@ def _launch(entry: str, desc: bytes, dev: int, held: Sequence["_Held"] = ()) -> 
         check(status, entry)
 
 
-def _no_gradients(name: str) -> None:
-    if torch.is_grad_enabled():
+def _tangents() -> bool:
+    """a forward-mode level is open: tensors may carry tangents"""
+    return forward_ad._current_level >= 0
+
+
+def _no_gradients(name: str, t: torch.Tensor) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name}: requires gradients, and this operator has none to give: call it under torch.no_grad() or detach the tensor")
+    if t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name}: carries a forward-mode tangent, and this operator has no derivative to give: unpack the tensor first")
 
 
 def _matrix(t: torch.Tensor, name: str, dtype: Optional[torch.dtype] = None, dev: Optional[int] = None) -> Tuple[int, int, int]:
@@ -81,8 +90,8 @@ def _matrix(t: torch.Tensor, name: str, dtype: Optional[torch.dtype] = None, dev
         raise ValueError(f"{name}: expected a CUDA {'fp16 | bf16' if dtype is None else dtype} tensor, got {t.dtype} on {t.device}")
     if dev is not None and t.get_device() != dev:
         raise ValueError(f"{name}: on {t.device}, the other tensors are on device {dev}")
-    if t.requires_grad:
-        _no_gradients(name)
+    if t.requires_grad or _tangents():
+        _no_gradients(name, t)
     if rows <= 1:
         return rows, cols, cols
     if ld < cols or ld > _I32_MAX:
@@ -421,8 +430,8 @@ def _affine(t: Optional[torch.Tensor], name: str, c: int, dtype: torch.dtype, de
         return 0
     if t.dtype != dtype or t.get_device() != dev or not t.is_contiguous() or t.numel() != c:
         raise ValueError(f"{name}: expected a contiguous {dtype} tensor of {c} elements on device {dev}")
-    if t.requires_grad:
-        _no_gradients(name)
+    if t.requires_grad or _tangents():
+        _no_gradients(name, t)
     return t.data_ptr()
 
 

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from test_token_ops import DEV, DTYPES, IDS, attention_inputs, attention_oracle, gpu, half_step, norm_oracle, rnd, rotary_oracle, subnormal, within
+from test_token_ops import on_cpu  # noqa: F401  (a fixture)
 
 
 def randn(shape, seed, dt, scale=1.0):
@@ -174,3 +175,26 @@ def test_gated_norm_of_inputs_past_the_last_cache(c, off, dt):
         ws, wh = norm_oracle(x0[a:e], f0[a:e], "layer", 0.75, None, pre, gate, scale, shift, torch.arange(a, e, device=DEV) // per)
         within(s[a:e], *ws, what=("s", c, a))
         within(h[a:e], *wh, what=("h", c, a))
+
+
+# ---- refusals -----------------------------------------------------------------------------------------------------------------------
+def test_tensors_with_a_forward_mode_tangent_are_refused(on_cpu):  # noqa: F811
+    import torch.autograd.forward_ad as fw
+    from musev_amd import ops
+    x, c = torch.zeros(6, 64, dtype=torch.float16), torch.zeros(64, dtype=torch.float16)
+    plan, table = ops.attention_plan([6], heads=1, d=64, device="cpu"), ops.rotary_table([64], device="cpu")
+    w = ops.Int8Rows(torch.zeros(64, 128, dtype=torch.int8), torch.ones(64), 64)
+    pos = torch.zeros(6, 1)
+    calls = (lambda x, c, p: ops.attention_packed(plan, x, x, x), lambda x, c, p: ops.rotary_axes(x, None, p, table, heads=1, d=64),
+             lambda x, c, p: ops.gated_residual_norm(x, x, pre=(c, None, 1e-6)), lambda x, c, p: ops.linear_i8(x, w, bias=c),
+             lambda x, c, p: ops.gemm_i8(w, w, bias=c), lambda x, c, p: ops.linear_i8(x, w, residual=x))
+    with fw.dual_level():
+        tx, tc, tp = (fw.make_dual(t, torch.ones_like(t)) for t in (x, c, pos))
+        for i, call in enumerate(calls):
+            with pytest.raises(on_cpu):
+                call(x, c, pos.int())
+            for args in ([(tx, c, pos)] if i in (0, 5) else [(x, tc, pos)] if i == 4 else [(tx, c, pos), (x, tc, tp)]):
+                with pytest.raises(ValueError, match="tangent"):
+                    call(*args)
+                with torch.no_grad(), pytest.raises(ValueError, match="tangent"):   # (no_grad does not switch forward mode off)
+                    call(*args)
