@@ -547,6 +547,8 @@ def pack_weight_i8(codes: torch.Tensor, scale: torch.Tensor) -> Int8Rows:
         raise ValueError(f"pack_weight_i8: codes must be a CUDA int8 [N, K] tensor, K <= {_I8_MAX_K}")
     if scale.dtype != torch.float32 or scale.shape != (codes.shape[0],) or scale.device != codes.device:
         raise ValueError(f"pack_weight_i8: scale must be fp32 [{codes.shape[0]}] on {codes.device}")
+    if scale.requires_grad or _tangents():
+        _no_gradients("pack_weight_i8: scale", scale)
     n, k = codes.shape
     packed = torch.zeros((n, -(-k // 128) * 128), dtype=torch.int8, device=codes.device)
     packed[:, :k] = codes
@@ -583,6 +585,8 @@ def _i8_result(what: str, m: int, w: Int8Rows, like: torch.Tensor, dtype, bias, 
         raise ValueError(f"{what}: weight on {w.device}, rows on {like.device}")
     if n < 1:
         raise ValueError(f"{what}: a weight without rows")
+    if w.scale.requires_grad or _tangents():
+        _no_gradients(f"{what}: scale", w.scale)
     pb = pr = ldr = 0
     if bias is not None:
         pb = _affine(bias, f"{what}: bias", n, dtype, dev)
@@ -607,6 +611,8 @@ def gemm_i8(a: Int8Rows, w: Int8Rows, *, bias: Optional[torch.Tensor] = None, re
     ``out`` may be ``residual`` itself."""
     if a.k != w.k:
         raise ValueError(f"gemm_i8: rows of {a.k}, weight of {w.k}")
+    if a.scale.requires_grad or _tangents():
+        _no_gradients("gemm_i8: scale", a.scale)
     pb, pr, po, ldr, ldo, out = _i8_result("gemm_i8", a.rows, w, a.codes, dtype, bias, residual, act, out)
     _launch("mv_gemm_i8", _pack_gemm(a._codes, w._codes, a._scale, w._scale, pb, pr, po, a.rows, w.rows, w.kp, a.kp, w.kp, ldr, ldo, act, _DTYPES[dtype]),
             a._dev, (a, w))

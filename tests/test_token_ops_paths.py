@@ -198,3 +198,29 @@ def test_tensors_with_a_forward_mode_tangent_are_refused(on_cpu):  # noqa: F811
                     call(*args)
                 with torch.no_grad(), pytest.raises(ValueError, match="tangent"):   # (no_grad does not switch forward mode off)
                     call(*args)
+
+
+def test_int8_scales_that_require_gradients_are_refused(on_cpu):  # noqa: F811
+    import torch.autograd.forward_ad as fw
+    from musev_amd import ops
+    codes, scale = torch.zeros(64, 128, dtype=torch.int8), torch.ones(64)
+    learnt = torch.ones(64, requires_grad=True)
+    x, plain = torch.zeros(6, 128, dtype=torch.float16), ops.Int8Rows(codes, scale, 128)
+
+    def calls(s):
+        w = ops.Int8Rows(codes, s, 128)
+        return (lambda: ops.linear_i8(x, w), lambda: ops.gemm_i8(plain, w), lambda: ops.gemm_i8(w, plain))
+    for call in calls(learnt):
+        with pytest.raises(ValueError, match="scale: requires gradients"):
+            call()
+        with torch.no_grad(), pytest.raises(on_cpu):
+            call()
+    with pytest.raises(ValueError, match="scale: requires gradients"):
+        ops.pack_weight_i8(codes, learnt)
+    with torch.no_grad():
+        assert not ops.pack_weight_i8(codes, learnt).scale.requires_grad
+    with fw.dual_level():
+        dual = fw.make_dual(scale, torch.ones_like(scale))
+        for call in (*calls(dual), lambda: ops.pack_weight_i8(codes, dual)):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
