@@ -2,7 +2,8 @@
  * musev_tokens.h -- C ABI of the token-transformer operators of libmusev_hip.so (gfx950): packed attention, rotary positions with
  * several axes, the gated residual norm and the int8 projection.  Conventions of musev_hip.h: extern "C", plain device pointers and
  * explicit strides, no hidden allocation, no global mutable state except the thread-local last-error string, every launch on the
- * hipStream_t passed as `stream` of the CURRENT device, 0 = ok / negative = MV_ERR_* with mv_last_error().
+ * hipStream_t passed as `stream` of the CURRENT device, 0 = ok / negative = MV_ERR_* with mv_last_error().  A call whose launch would have 2^32 work
+ * items or more is refused (2^24 blocks of 256: rows of the norm from 2^24, of 2048 columns, to 2^28, of up to 128).
  * Matrices are rows x columns with unit inner stride; row strides (ld*) are in elements.  Element type: MV_F16 or MV_BF16.
  */
 #ifndef MUSEV_TOKENS_H

@@ -410,11 +410,9 @@ extern "C" int64_t mv_attention_packed_workspace_bytes(int64_t ws_rows, int32_t 
     return ws_rows * kv_heads * (d + 2) * 4;
 }
 
-template <typename T, int G>
-static void launch_join(const mv_attn_packed_desc* d, hipStream_t st) {
-    const int blocks = (d->join_rows * (d->d / 4) + 256 / G - 1) / (256 / G);
-    attention_join_kernel<T, G><<<(unsigned)(d->n_joins * d->kv_heads * blocks), 256, 0, st>>>(*d, blocks);
-}
+// threads that share a (row, four columns) of the join, by the parts of a join in the mean; blocks of a join
+static int join_threads(const mv_attn_packed_desc* d) { return d->ws_rows > 16ll * d->n_joins * d->join_rows ? 8 : 1; }
+static int join_blocks(const mv_attn_packed_desc* d) { return (d->join_rows * (d->d / 4) * join_threads(d) + 255) / 256; }
 
 template <typename T, int K16>
 static int launch_packed(const mv_attn_packed_desc* d, hipStream_t st) {
@@ -422,8 +420,10 @@ static int launch_packed(const mv_attn_packed_desc* d, hipStream_t st) {
     attention_packed_kernel<T, K16><<<(unsigned)(d->n_items * d->kv_heads), 256, PackedCfg<K16>::LDS_BYTES, st>>>(*d);
     MV_CHECK_LAUNCH("mv_attention_packed");
     if (d->n_joins > 0) {
-        if (d->ws_rows > 16ll * d->n_joins * d->join_rows) launch_join<T, 8>(d, st);   // (parts of a join, in the mean)
-        else launch_join<T, 1>(d, st);
+        const int blocks = join_blocks(d);
+        const unsigned grid = (unsigned)(d->n_joins * d->kv_heads * blocks);
+        if (join_threads(d) == 8) attention_join_kernel<T, 8><<<grid, 256, 0, st>>>(*d, blocks);
+        else attention_join_kernel<T, 1><<<grid, 256, 0, st>>>(*d, blocks);
         MV_CHECK_LAUNCH("mv_attention_packed (join)");
     }
     return MV_OK;
@@ -453,6 +453,8 @@ extern "C" int mv_attention_packed(const mv_attn_packed_desc* d, void* stream) {
     MV_REQUIRE(d->n_items >= 0 && d->n_joins >= 0 && (int64_t)d->n_items * d->kv_heads < (1ll << 31) && d->join_rows >= 0 && d->join_rows <= 128 &&
                (int64_t)d->n_joins * d->kv_heads * 128 < (1ll << 31), "mv_attention_packed: %d items, %d joins of up to %d rows", d->n_items, d->n_joins,
                d->join_rows);
+    MV_REQUIRE_GRID("mv_attention_packed", (int64_t)d->n_items * d->kv_heads, 256);
+    MV_REQUIRE_GRID("mv_attention_packed (join)", (int64_t)d->n_joins * d->kv_heads * join_blocks(d), 256);
     if (d->n_items == 0) return MV_OK;
     MV_REQUIRE(d->q && d->k && d->v && d->out && d->items, "mv_attention_packed: null pointer");
     MV_REQUIRE((((uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v | (uintptr_t)d->out) & 15) == 0 && ((d->ldq | d->ldk | d->ldv | d->ldo) & 7) == 0,

@@ -93,18 +93,22 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* x, int64_t 
 }
 
 template <typename T, int NV, int WAVES, bool REREAD>
-static void launch_quantize(const void* x, int64_t ldx, int64_t rows, int k, int8_t* codes, int64_t ldc, float* scale, hipStream_t st) {
+static int launch_quantize(const void* x, int64_t ldx, int64_t rows, int k, int8_t* codes, int64_t ldc, float* scale, hipStream_t st) {
     constexpr int R = 4 / WAVES;
-    quantize_rows_kernel<T, NV, WAVES, REREAD><<<(unsigned)((rows + R - 1) / R), 256, 0, st>>>((const T*)x, ldx, rows, k, codes, ldc, scale);
+    const int64_t blocks = (rows + R - 1) / R;
+    MV_REQUIRE_GRID("mv_quantize_rows_i8", blocks, 256);
+    quantize_rows_kernel<T, NV, WAVES, REREAD><<<(unsigned)blocks, 256, 0, st>>>((const T*)x, ldx, rows, k, codes, ldc, scale);
+    MV_CHECK_LAUNCH("mv_quantize_rows_i8");
+    return MV_OK;
 }
 template <typename T>
-static void launch_quantize_width(const void* x, int64_t ldx, int64_t rows, int k, int8_t* codes, int64_t ldc, float* scale, hipStream_t st) {
-    if (ldc <= 512) launch_quantize<T, 1, 1, false>(x, ldx, rows, k, codes, ldc, scale, st);
-    else if (ldc <= 1536) launch_quantize<T, 3, 1, false>(x, ldx, rows, k, codes, ldc, scale, st);
-    else if (ldc <= 2048) launch_quantize<T, 1, 4, false>(x, ldx, rows, k, codes, ldc, scale, st);
-    else if (ldc <= 6144) launch_quantize<T, 3, 4, false>(x, ldx, rows, k, codes, ldc, scale, st);
-    else if (ldc <= 16384) launch_quantize<T, 8, 4, false>(x, ldx, rows, k, codes, ldc, scale, st);
-    else launch_quantize<T, 8, 4, true>(x, ldx, rows, k, codes, ldc, scale, st);
+static int launch_quantize_width(const void* x, int64_t ldx, int64_t rows, int k, int8_t* codes, int64_t ldc, float* scale, hipStream_t st) {
+    if (ldc <= 512) return launch_quantize<T, 1, 1, false>(x, ldx, rows, k, codes, ldc, scale, st);
+    if (ldc <= 1536) return launch_quantize<T, 3, 1, false>(x, ldx, rows, k, codes, ldc, scale, st);
+    if (ldc <= 2048) return launch_quantize<T, 1, 4, false>(x, ldx, rows, k, codes, ldc, scale, st);
+    if (ldc <= 6144) return launch_quantize<T, 3, 4, false>(x, ldx, rows, k, codes, ldc, scale, st);
+    if (ldc <= 16384) return launch_quantize<T, 8, 4, false>(x, ldx, rows, k, codes, ldc, scale, st);
+    return launch_quantize<T, 8, 4, true>(x, ldx, rows, k, codes, ldc, scale, st);
 }
 
 extern "C" int mv_quantize_rows_i8(const void* x, int64_t ldx, int64_t rows, int32_t k, int32_t dtype, int8_t* codes, int64_t ldc, float* scale,
@@ -114,9 +118,7 @@ extern "C" int mv_quantize_rows_i8(const void* x, int64_t ldx, int64_t rows, int
     MV_REQUIRE(ldc % 128 == 0 && ldc >= k && ldc < k + 128, "mv_quantize_rows_i8: code rows of %ld for k = %d (k rounded up to 128)", (long)ldc, k);
     if (rows == 0) return MV_OK;
     MV_REQUIRE(x && codes && scale && ((uintptr_t)codes & 15) == 0, "mv_quantize_rows_i8: null or unaligned pointer");
-    MV_DISPATCH_TYPE(dtype, launch_quantize_width<T>(x, ldx, rows, k, codes, ldc, scale, (hipStream_t)stream));
-    MV_CHECK_LAUNCH("mv_quantize_rows_i8");
-    return MV_OK;
+    MV_DISPATCH_TYPE(dtype, return launch_quantize_width<T>(x, ldx, rows, k, codes, ldc, scale, (hipStream_t)stream));
 }
 
 // ---- the product ---------------------------------------------------------------------------------------------------------------
@@ -457,8 +459,8 @@ template <typename T, int BM, int BN, int WM, int WN, int KS, bool COLD = false>
 static int launch_gemm_i8(const mv_gemm_i8_desc* d, hipStream_t st) {
     using C = GemmI8Cfg<BM, BN, WM, WN, KS>;
     const auto kernel = gemm_i8_kernel<T, BM, BN, WM, WN, KS, COLD>;
-    const int64_t tm = (d->M + BM - 1) / BM, tn = (d->N + BN - 1) / BN;
-    MV_REQUIRE(tm * tn < (1ll << 31), "mv_gemm_i8: %ld x %ld tiles", (long)tm, (long)tn);
+    const int64_t tm = (d->M + BM - 1) / BM, tn = ((int64_t)d->N + BN - 1) / BN;
+    MV_REQUIRE_GRID("mv_gemm_i8", tm * tn, C::THREADS);
     if (C::LDS > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
         if (e != hipSuccess) {
@@ -476,9 +478,10 @@ static int launch_gemm_i8_shape(const mv_gemm_i8_desc* d, hipStream_t st) {
     // Up to 32 rows of a short K: the weight stream (us, stream / 32 x 32 tiles: 16 x 1280 x 5120 4.5 / 4.9; 20 x 640 x 640 3.1 / 4.6; 32 x 2048 x 2048
     // 5.0 / 5.5; beyond, its waves' turns add up: 32 x 5120 x 5120 16.4 / 8.2).
     if (d->M <= 32 && d->kp <= 2048) {
-        const unsigned grid = (d->N + 15) / 16;
-        if (d->M <= 16) gemm_i8_few_kernel<T, 1><<<grid, 512, 0, st>>>(*d);
-        else gemm_i8_few_kernel<T, 2><<<grid, 512, 0, st>>>(*d);
+        const int64_t grid = ((int64_t)d->N + 15) / 16;
+        MV_REQUIRE_GRID("mv_gemm_i8", grid, 512);
+        if (d->M <= 16) gemm_i8_few_kernel<T, 1><<<(unsigned)grid, 512, 0, st>>>(*d);
+        else gemm_i8_few_kernel<T, 2><<<(unsigned)grid, 512, 0, st>>>(*d);
         MV_CHECK_LAUNCH("mv_gemm_i8");
         return MV_OK;
     }
@@ -497,7 +500,7 @@ static int launch_gemm_i8_shape(const mv_gemm_i8_desc* d, hipStream_t st) {
     // 112.6 / 103.1; 400 - / 115.9 / 121.2.  K = 640: 160 16.9 / 18.1 / -; 272 26.4 / 34.1 / 26.8; 384 34.2 / 36.3 / 33.2; 416 37.4 / 36.5 / 37.3.
     if (const int64_t all = tiles(256, 256); all >= 192) {
         constexpr int64_t CUS = 256;
-        const int64_t cols = (d->N + 255) / 256, whole = all / CUS * CUS / cols, left = all - whole * cols;
+        const int64_t cols = ((int64_t)d->N + 255) / 256, whole = all / CUS * CUS / cols, left = all - whole * cols;
         mv_gemm_i8_desc head = *d, tail = *d;
         const bool split = whole > 0 && left > 0 && left <= CUS / 2;
         if (split) {
@@ -549,8 +552,9 @@ extern "C" int mv_linear_i8(const mv_linear_i8_desc* d, void* stream) {
         MV_REQUIRE(d->act == MV_ACT_NONE || d->act == MV_ACT_SILU, "mv_linear_i8: activation %d", d->act);
         MV_REQUIRE(d->N >= 1 && d->ldw % 128 == 0 && d->ldw >= d->kp, "mv_linear_i8: N %d, ldw %ld for kp %ld", d->N, (long)d->ldw, (long)d->kp);
         MV_REQUIRE(d->x && d->w && d->w_scale && d->out && ((uintptr_t)d->w & 15) == 0, "mv_linear_i8: null or unaligned pointer");
-        const unsigned grid = (d->N + 15) / 16;
-        MV_DISPATCH_TYPE(d->dtype, (linear_i8_few_kernel<T><<<grid, 512, 0, (hipStream_t)stream>>>(*d)));
+        const int64_t grid = ((int64_t)d->N + 15) / 16;
+        MV_REQUIRE_GRID("mv_linear_i8", grid, 512);
+        MV_DISPATCH_TYPE(d->dtype, (linear_i8_few_kernel<T><<<(unsigned)grid, 512, 0, (hipStream_t)stream>>>(*d)));
         MV_CHECK_LAUNCH("mv_linear_i8");
         return MV_OK;
     }

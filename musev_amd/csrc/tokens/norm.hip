@@ -143,11 +143,15 @@ __global__ __launch_bounds__(256) void gated_norm_kernel(const mv_gated_norm_des
 }
 
 template <typename T, int NV, int LANES>
-static void launch_norm(const mv_gated_norm_desc* d, hipStream_t st) {
+static int launch_norm(const mv_gated_norm_desc* d, hipStream_t st) {
     constexpr int R = 256 / LANES;
+    const int64_t blocks = (d->rows + R - 1) / R;
+    MV_REQUIRE_GRID("mv_gated_residual_norm", blocks, 256);
     // (53 248 x 1280, 273 MB of inputs: 123 -> 113 us where other work ran in between; 26 624 x 1280, half of that and still in the cache: 57 -> 65)
     const bool cold = d->rows * d->c * 4 > COLD_BYTES;
-    gated_norm_kernel<T, NV, LANES><<<(unsigned)((d->rows + R - 1) / R), 256, 0, st>>>(*d, cold);
+    gated_norm_kernel<T, NV, LANES><<<(unsigned)blocks, 256, 0, st>>>(*d, cold);
+    MV_CHECK_LAUNCH("mv_gated_residual_norm");
+    return MV_OK;
 }
 
 // A wave holds a row of up to 1536 columns where there are rows enough to fill the chip; the block's four waves share it otherwise.  Measured (us,
@@ -156,19 +160,19 @@ static void launch_norm(const mv_gated_norm_desc* d, hipStream_t st) {
 // 11.8; 1 x 128 3.7 / 3.6; 20 000 x 200 16.2 / 9.7; 200 x 256 4.3 / 4.2; with several chunks per lane only where rows are many: 20 000 x 320 17.5 / 13.8,
 // 100 000 x 512 80 / 70, but 2000 x 320 5.2 / 7.7, 4000 x 512 6.5 / 7.3.
 template <typename T>
-static void launch_norm_width(const mv_gated_norm_desc* d, hipStream_t st) {
+static int launch_norm_width(const mv_gated_norm_desc* d, hipStream_t st) {
     const int c = d->c;
-    if (c <= 128) launch_norm<T, 1, 16>(d, st);
-    else if (c <= 256) launch_norm<T, 1, 32>(d, st);
-    else if (c <= 384 && d->rows > 16384) launch_norm<T, 3, 16>(d, st);
-    else if (c <= 512 && d->rows > 16384) launch_norm<T, 2, 32>(d, st);
-    else if (c <= 512) launch_norm<T, 1, 64>(d, st);
-    else if (c > 1536 ? c <= 2048 : d->rows <= 2048) launch_norm<T, 1, 256>(d, st);
-    else if (c <= 1024) launch_norm<T, 2, 64>(d, st);
-    else if (c <= 1536) launch_norm<T, 3, 64>(d, st);
-    else if (c <= 4096) launch_norm<T, 2, 256>(d, st);
-    else if (c <= 8192) launch_norm<T, 4, 256>(d, st);
-    else launch_norm<T, 8, 256>(d, st);
+    if (c <= 128) return launch_norm<T, 1, 16>(d, st);
+    if (c <= 256) return launch_norm<T, 1, 32>(d, st);
+    if (c <= 384 && d->rows > 16384) return launch_norm<T, 3, 16>(d, st);
+    if (c <= 512 && d->rows > 16384) return launch_norm<T, 2, 32>(d, st);
+    if (c <= 512) return launch_norm<T, 1, 64>(d, st);
+    if (c > 1536 ? c <= 2048 : d->rows <= 2048) return launch_norm<T, 1, 256>(d, st);
+    if (c <= 1024) return launch_norm<T, 2, 64>(d, st);
+    if (c <= 1536) return launch_norm<T, 3, 64>(d, st);
+    if (c <= 4096) return launch_norm<T, 2, 256>(d, st);
+    if (c <= 8192) return launch_norm<T, 4, 256>(d, st);
+    return launch_norm<T, 8, 256>(d, st);
 }
 
 extern "C" int mv_gated_residual_norm(const mv_gated_norm_desc* d, void* stream) {
@@ -179,7 +183,5 @@ extern "C" int mv_gated_residual_norm(const mv_gated_norm_desc* d, void* stream)
     MV_REQUIRE(d->rows_per_group >= 0 && d->rows_per_group < (1ll << 31), "mv_gated_residual_norm: groups of %ld rows", (long)d->rows_per_group);
     if (d->rows == 0) return MV_OK;
     MV_REQUIRE(d->x && d->f && d->stream_out, "mv_gated_residual_norm: null pointer");
-    MV_DISPATCH_TYPE(d->dtype, launch_norm_width<T>(d, (hipStream_t)stream));
-    MV_CHECK_LAUNCH("mv_gated_residual_norm");
-    return MV_OK;
+    MV_DISPATCH_TYPE(d->dtype, return launch_norm_width<T>(d, (hipStream_t)stream));
 }

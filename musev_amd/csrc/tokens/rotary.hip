@@ -115,7 +115,7 @@ extern "C" int mv_rotary_axes(const mv_rotary_desc* d, void* stream) {
     a.large = d->tokens * heads * d->d * 2 > (64ll << 20);
     a.cold = d->tokens * heads * d->d * 2 > COLD_BYTES;   // (53 248 x 32 heads x 128: 146 -> 143 us)
     const int64_t grid = (d->tokens + a.tokens_per_block - 1) / a.tokens_per_block;
-    MV_REQUIRE(grid < (1ll << 31), "mv_rotary_axes: %ld tokens", (long)d->tokens);
+    MV_REQUIRE_GRID("mv_rotary_axes", grid, 256);
     const size_t lds = (size_t)a.tokens_per_block * d->pairs * sizeof(float2);
     if (d->halves) MV_DISPATCH_TYPE(d->dtype, (rotary_kernel<T, true><<<(unsigned)grid, 256, lds, (hipStream_t)stream>>>(a)));
     else MV_DISPATCH_TYPE(d->dtype, (rotary_kernel<T, false><<<(unsigned)grid, 256, lds, (hipStream_t)stream>>>(a)));

@@ -90,6 +90,10 @@ __device__ __forceinline__ float wave_sum_fast(float v) {
     return v;
 }
 
+// a launch has fewer than 2^32 work items
+#define MV_REQUIRE_GRID(name, blocks, threads) \
+    MV_REQUIRE((int64_t)(blocks) * (threads) < (1ll << 32), "%s: %ld blocks of %d threads (a launch has fewer than 2^32 work items)", name, (long)(blocks), (int)(threads))
+
 // calls body(T{}) with the element type of a descriptor
 #define MV_DISPATCH_TYPE(dtype, ...)                         \
     do {                                                     \

@@ -224,3 +224,44 @@ def test_int8_scales_that_require_gradients_are_refused(on_cpu):  # noqa: F811
         for call in (*calls(dual), lambda: ops.pack_weight_i8(codes, dual)):
             with pytest.raises(ValueError, match="tangent"):
                 call()
+
+
+def test_calls_of_more_work_than_a_launch_has_are_refused():
+    """a launch has fewer than 2^32 work items: one block more than that is an error of its own, before anything is launched"""
+    import ctypes as C
+    from musev_amd import _lib
+    lib = _lib.load()
+
+    def refused(rc):
+        assert rc == -1 and b"2^32 work items" in lib.mv_last_error(), (rc, lib.mv_last_error())
+    n = _lib.GatedNormDesc()
+    n.x = n.f = n.stream_out = 16
+    n.groups = 1
+    for c, per_block in ((8, 16), (200, 8), (512, 8), (1280, 4), (2048, 1), (16384, 1)):
+        n.c, n.rows = c, ((1 << 24) - 1) * per_block + 1
+        refused(lib.mv_gated_residual_norm(C.byref(n), None))
+    r = _lib.RotaryDesc()
+    r.q = r.out_q = r.positions = r.turns = r.axis = 16
+    r.heads, r.d, r.pairs, r.axes, r.tokens = 1, 8, 4, 1, ((1 << 24) - 1) * 8 + 1
+    refused(lib.mv_rotary_axes(C.byref(r), None))
+    for k, kp, per_block in ((100, 128, 4), (2000, 2048, 1)):
+        refused(lib.mv_quantize_rows_i8(16, k, ((1 << 24) - 1) * per_block + 1, k, 0, 16, kp, 16, None))
+    a = _lib.AttnPackedDesc()
+    a.q = a.k = a.v = a.out = a.items = a.joins = a.workspace = 16
+    a.workspace_bytes, a.heads, a.kv_heads, a.d, a.scale = 1 << 50, 4, 2, 64, 0.125
+    a.ldq = a.ldo = 256
+    a.ldk = a.ldv = 128
+    a.n_items = 1 << 23
+    refused(lib.mv_attention_packed(C.byref(a), None))
+    a.n_items, a.n_joins, a.join_rows = 1, 1 << 20, 128
+    refused(lib.mv_attention_packed(C.byref(a), None))
+    w = _lib.LinearI8Desc()
+    w.x = w.w = w.w_scale = w.out = w.workspace = 16
+    w.M, w.N, w.K, w.kp, w.ldx, w.ldw, w.ldo = 1, 2 ** 31 - 1, 100, 128, 100, 128, 8
+    refused(lib.mv_linear_i8(C.byref(w), None))
+    g = _lib.GemmI8Desc()
+    g.a = g.w = g.a_scale = g.w_scale = g.out = 16
+    g.M, g.N, g.kp, g.lda, g.ldw, g.ldo = 4, 1 << 27, 128, 128, 128, 8
+    refused(lib.mv_gemm_i8(C.byref(g), None))
+    g.M, g.N = 2 ** 31 - 1, 2 ** 31 - 1
+    refused(lib.mv_gemm_i8(C.byref(g), None))
