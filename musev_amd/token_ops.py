@@ -29,6 +29,7 @@ __all__ = ["AttentionPlan", "attention_plan", "attention_packed", "RotaryTable",
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 _I32_MAX = 2 ** 31 - 1
+_F32_MAX = 2.0 ** 128 - 2.0 ** 104
 
 # A small call's time is the host's: checks read each tensor's geometry once, a descriptor is packed in one go, the stream is asked for as a
 # raw handle.
@@ -486,8 +487,10 @@ def gated_residual_norm(x: torch.Tensor, f: torch.Tensor, *, kind: str = "layer"
     elif groups > 1:
         raise ValueError(f"gated_residual_norm: {groups} groups need rows_per_group or group_index")
     for nm, a in (("post", post), ("pre", pre)):
-        if a is not None and not 0.0 <= a[2] < math.inf:
-            raise ValueError(f"gated_residual_norm: {nm} eps {a[2]} (a finite number, not negative)")
+        if a is not None and not 0.0 <= a[2] <= _F32_MAX:
+            raise ValueError(f"gated_residual_norm: {nm} eps {a[2]} (a finite fp32 number, not negative)")
+    if abs(alpha) > _F32_MAX and not math.isinf(alpha):
+        raise ValueError(f"gated_residual_norm: alpha {alpha} is past fp32")
     given = out is not None or norm_out is not None
     if out is None:
         out, lds = torch.empty_like(x), c

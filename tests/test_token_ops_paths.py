@@ -265,3 +265,15 @@ def test_calls_of_more_work_than_a_launch_has_are_refused():
     refused(lib.mv_gemm_i8(C.byref(g), None))
     g.M, g.N = 2 ** 31 - 1, 2 ** 31 - 1
     refused(lib.mv_gemm_i8(C.byref(g), None))
+
+
+def test_the_gated_norm_refuses_factors_past_fp32(on_cpu):  # noqa: F811
+    from musev_amd import ops
+    x = torch.zeros(6, 40, dtype=torch.float16)
+    top = torch.finfo(torch.float32).max
+    for kw, match in ((dict(pre=(None, None, 1e39)), "eps"), (dict(post=(None, None, 1e300)), "eps"), (dict(alpha=1e39), "alpha"), (dict(alpha=-1e39), "alpha")):
+        with pytest.raises(ValueError, match=match):
+            ops.gated_residual_norm(x, x, **kw)
+    for kw in (dict(pre=(None, None, top)), dict(alpha=-top), dict(alpha=float("inf")), dict(alpha=float("nan"))):
+        with pytest.raises(on_cpu):
+            ops.gated_residual_norm(x, x, **kw)
