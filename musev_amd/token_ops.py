@@ -32,9 +32,9 @@ _I32_MAX = 2 ** 31 - 1
 _F32_MAX = 2.0 ** 128 - 2.0 ** 104
 
 # A small call's time is the host's: checks read each tensor's geometry once, a descriptor is packed in one go, the stream is asked for as a
-# raw handle.
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
+# raw handle (a torch built without a GPU has none: the rest of the package is imported beside it all the same).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
 def _packer(desc) -> Callable[..., bytes]:

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_token_ops import DEV, DTYPES, IDS, attention_inputs, attention_oracle, gpu, half_step, norm_oracle, rnd, rotary_oracle, subnormal, within
+from test_token_ops import ROOT, DEV, DTYPES, IDS, attention_inputs, attention_oracle, gpu, half_step, norm_oracle, rnd, rotary_oracle, subnormal, within
 from test_token_ops import on_cpu  # noqa: F401  (a fixture)
 
 
@@ -277,3 +277,13 @@ def test_the_gated_norm_refuses_factors_past_fp32(on_cpu):  # noqa: F811
     for kw in (dict(pre=(None, None, top)), dict(alpha=-top), dict(alpha=float("inf")), dict(alpha=float("nan"))):
         with pytest.raises(on_cpu):
             ops.gated_residual_norm(x, x, **kw)
+
+
+def test_operators_are_importable_beside_a_torch_without_a_gpu_build():
+    """such a build has no stream handles; the operators need them only when they launch"""
+    import subprocess
+    import sys
+    code = ("import torch\n"
+            "for n in ('_cuda_getCurrentRawStream', '_cuda_getDevice'):\n    delattr(torch._C, n)\n"
+            "from musev_amd import ops\nassert ops.attention_plan([4], heads=1, d=64, device='cpu').total_q == 4")
+    assert subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=ROOT).returncode == 0
