@@ -138,17 +138,21 @@ def _no_overlap(out: torch.Tensor, name: str, inputs: Sequence[Tuple[str, Option
 class _Held:
     """device memory that belongs to a plan, table or weight: made on one stream, perhaps used on others"""
 
-    def _hold(self, *tensors: torch.Tensor) -> None:
-        self._tensors = tensors
+    def _hold(self, *tensors: torch.Tensor, ready: Optional[torch.cuda.Event] = None) -> None:
+        self._tensors, self._ready = tensors, ready
         self.device = tensors[0].device
         self._dev = tensors[0].get_device()
         self._streams = {_raw_stream(self._dev)} if tensors[0].is_cuda else set()
 
     def _use(self, stream: int) -> None:
-        # (first use on a stream) the allocator may not hand the memory out again while a launch there still reads it
+        # (first use on a stream) what was filled without a wait for it is waited for there, and the allocator may not hand the memory out again while
+        # a launch there still reads it
         if not torch.cuda.is_current_stream_capturing():
+            here = torch.cuda.current_stream(self.device)
+            if self._ready is not None:
+                here.wait_event(self._ready)
             for t in self._tensors:
-                t.record_stream(torch.cuda.current_stream(self.device))
+                t.record_stream(here)
             self._streams.add(stream)
 
 
@@ -156,12 +160,12 @@ class _Held:
 class AttentionPlan(_Held):
     """the work list of :func:`attention_packed` for one set of sequence lengths (:func:`attention_plan`)"""
 
-    def __init__(self, q_lens, kv_lens, heads, kv_heads, d, causal, scale, items, joins, join_rows, ws_rows):
+    def __init__(self, q_lens, kv_lens, heads, kv_heads, d, causal, scale, items, joins, join_rows, ws_rows, ready=None):
         self.q_lens, self.kv_lens = tuple(q_lens), tuple(kv_lens)
         self.heads, self.kv_heads, self.d, self.causal, self.scale = heads, kv_heads, d, causal, scale
         self.total_q, self.total_kv = sum(q_lens), sum(kv_lens)
         self.n_items, self.n_joins, self.join_rows, self.ws_rows = items.shape[0], joins.shape[0], join_rows, ws_rows
-        self._hold(items, joins)
+        self._hold(items, joins, ready=ready)
         self._tables = items.data_ptr(), joins.data_ptr()
         self._workspace = 4 * ws_rows * kv_heads * (d + 2)   # mv_attention_packed_workspace_bytes
 
@@ -275,7 +279,10 @@ def attention_plan(q_lens: Sequence[int], kv_lens: Optional[Sequence[int]] = Non
                    causal: bool = True, scale: Optional[float] = None, device: Union[str, torch.device] = "cuda") -> AttentionPlan:
     """The plan of :func:`attention_packed` over ``len(q_lens)`` sequences of ``q_lens[i]`` query and ``kv_lens[i]`` key rows (default: as
     many), host integers, zero allowed.  ``causal``: query i of a sequence sees keys j <= i + kv_len - q_len -- the new tokens stand at the
-    end of their keys.  ``scale``: of the scores, default d ** -0.5.  Made once per set of lengths and used for every layer."""
+    end of their keys.  ``scale``: of the scores, default d ** -0.5.  Made once per set of lengths and used for every layer.
+    The list is uploaded on the current stream without a wait for the work queued there; other streams wait for it at the plan's first use.
+    A graph holds the plan that it was captured with: its replays come behind the upload (torch.cuda.graph waits for it), and no plan is
+    made while a graph is captured."""
     kv_heads = heads if kv_heads is None else int(kv_heads)
     heads, d = int(heads), int(d)
     if kv_heads < 1 or heads < 1 or heads % kv_heads:
@@ -292,12 +299,21 @@ def attention_plan(q_lens: Sequence[int], kv_lens: Optional[Sequence[int]] = Non
     if not abs(scale) <= 1e6:
         raise ValueError(f"attention_plan: scale {scale} (at most 1e6 in size)")
     dev = torch.device(device)
-    if dev.type == "cuda" and dev.index is None:
-        dev = torch.device("cuda", torch.cuda.current_device())
+    if dev.type == "cuda":
+        if torch.cuda.is_current_stream_capturing():
+            raise ValueError("attention_plan: a plan's list comes from the host and cannot be part of a graph: make it before the capture")
+        if dev.index is None:
+            dev = torch.device("cuda", torch.cuda.current_device())
     items, joins, ws_rows = _plan_items(ql, kl, heads // kv_heads, kv_heads, bool(causal), d)
-    table = torch.tensor((items + joins) or [(0,) * 8], dtype=torch.int32).to(dev)   # (one upload)
+    # One upload, from pinned memory: from pageable memory the host would wait for all work queued on the stream.  (The allocator keeps the pinned
+    # block until the copy is done.)
+    table, ready = torch.tensor((items + joins) or [(0,) * 8], dtype=torch.int32, pin_memory=dev.type == "cuda").to(dev, non_blocking=True), None
+    if dev.type == "cuda":
+        ready = torch.cuda.Event()
+        ready.record(torch.cuda.current_stream(dev))
     n = len(items)
-    return AttentionPlan(ql, kl, heads, kv_heads, d, bool(causal), scale, table[:n], table[n:n + len(joins)], max((j[6] for j in joins), default=0), ws_rows)
+    return AttentionPlan(ql, kl, heads, kv_heads, d, bool(causal), scale, table[:n], table[n:n + len(joins)], max((j[6] for j in joins), default=0), ws_rows,
+                         ready)
 
 
 def attention_packed(plan: AttentionPlan, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:

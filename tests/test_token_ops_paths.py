@@ -118,6 +118,56 @@ def test_parts_of_large_scores_weigh_as_they_should(name, each, dt):
     u = half_step(dt)
     within(got, want, (2 * u + 2.0 ** -18) * want + subnormal(dt), what=each)
 
+# ---- packed attention: making a plan ------------------------------------------------------------------------------------------------
+@gpu
+def test_a_plan_does_not_wait_for_the_work_queued_on_its_stream():
+    """made behind some 30 ms of work that is still running when the call returns; used at once on its own stream and on another"""
+    from musev_amd import ops
+    heads, kvh, d, ql, kl = 8, 2, 64, [1, 5], [3000, 77]
+    q, k, v = attention_inputs(ql, kl, heads, kvh, d, torch.float16, 1)
+    want, bound = attention_oracle(q, k, v, ql, kl, heads, kvh, d, True)
+    a = randn((8192, 8192), 2, torch.float16)
+    b, side = torch.empty_like(a), torch.cuda.Stream()
+    for on_side in (False, True):
+        ops.attention_packed(ops.attention_plan(ql, kl, heads=heads, kv_heads=kvh, d=d), q, k, v)   # (pinned memory, workspaces: allocated)
+        torch.cuda.synchronize()
+        for _ in range(40):
+            torch.matmul(a, a, out=b)
+        busy = torch.cuda.Event()
+        busy.record()
+        plan = ops.attention_plan(ql, kl, heads=heads, kv_heads=kvh, d=d)
+        assert not busy.query()
+        if on_side:
+            with torch.cuda.stream(side):
+                got = ops.attention_packed(plan, q, k, v)
+        else:
+            got = ops.attention_packed(plan, q, k, v)
+        torch.cuda.synchronize()
+        within(got, want, bound, what=on_side)
+
+
+@gpu
+def test_a_plan_is_not_made_while_a_graph_is_captured():
+    from musev_amd import ops
+    x = torch.zeros(4, device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(ValueError, match="before the capture"):
+            ops.attention_plan([1], [300], heads=1, d=64)
+        x += 1
+    for i in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert bool((x == i + 1).all())
+
+
+def test_a_plan_during_a_capture_is_refused_before_anything_is_uploaded(monkeypatch):
+    from musev_amd import ops
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(ValueError, match="before the capture"):
+        ops.attention_plan([1], [300], heads=1, d=64, device="cuda:0")
+    assert ops.attention_plan([1], [300], heads=1, d=64, device="cpu").total_kv == 300
+
 
 # ---- rotary positions: several tokens per block, results and inputs past the caches ----------------------------------------------
 MANY = {   # tokens, heads, kv_heads, d, sections
