@@ -13,6 +13,7 @@ from __future__ import annotations
 import collections
 import ctypes as C
 import heapq
+import itertools
 import math
 import operator
 import struct
@@ -160,25 +161,34 @@ class _Held:
 class AttentionPlan(_Held):
     """the work list of :func:`attention_packed` for one set of sequence lengths (:func:`attention_plan`)"""
 
-    def __init__(self, q_lens, kv_lens, heads, kv_heads, d, causal, scale, items, joins, join_rows, ws_rows, ready=None):
-        self.q_lens, self.kv_lens = tuple(q_lens), tuple(kv_lens)
+    def __init__(self, q_lens, kv_lens, kv_first, heads, kv_heads, d, causal, scale, items, joins, join_rows, ws_rows, ready=None):
+        self.q_lens, self.kv_lens, self.kv_first = tuple(q_lens), tuple(kv_lens), tuple(kv_first)
         self.heads, self.kv_heads, self.d, self.causal, self.scale = heads, kv_heads, d, causal, scale
-        self.total_q, self.total_kv = sum(q_lens), sum(kv_lens)
+        self.total_q, self.total_kv = sum(q_lens), max((f + n for f, n in zip(kv_first, kv_lens) if n), default=0)   # (rows of q; of k and v)
         self.n_items, self.n_joins, self.join_rows, self.ws_rows = items.shape[0], joins.shape[0], join_rows, ws_rows
         self._hold(items, joins, ready=ready)
         self._tables = items.data_ptr(), joins.data_ptr()
         self._workspace = 4 * ws_rows * kv_heads * (d + 2)   # mv_attention_packed_workspace_bytes
 
 
-def _lens(v, name: str) -> List[int]:
+def _integers(v, name: str) -> List[int]:
     if isinstance(v, torch.Tensor):
         if v.is_cuda:
             raise ValueError(f"{name}: lengths are host integers (reading them from the GPU would wait for it)")
         v = v.tolist()
-    v = [operator.index(x) for x in v]
+    return [operator.index(x) for x in v]
+
+
+def _lens(v, name: str) -> List[int]:
+    v = _integers(v, name)
     if not v or min(v) < 0 or sum(v) > _I32_MAX:
         raise ValueError(f"{name}: expected at least one length, none negative, at most 2^31 - 1 rows in all")
     return v
+
+
+def _behind(lens: Sequence[int]) -> List[int]:
+    """first rows of sequences that stand one behind the other"""
+    return [0, *itertools.accumulate(lens[:-1])]
 
 
 TILE_ROWS = 128   # packed rows per item
@@ -188,16 +198,16 @@ BLOCKS = 512      # two blocks on each of the 256 CUs
 LATE_PART = 1024  # keys of a part of a block that would run late
 
 
-def _plan_items(ql: Sequence[int], kl: Sequence[int], group: int, kv_heads: int, causal: bool, d: int = 128):
+def _plan_items(ql: Sequence[int], kl: Sequence[int], group: int, kv_heads: int, causal: bool, d: int = 128, first: Optional[Sequence[int]] = None):
     """(items, joins, workspace rows): see include/musev_tokens.h.  An item's keys end with what its last query sees.  Where the items alone would
     leave CUs idle, or one item would outlast the others, its keys are split into parts of 1 / BLOCKS of all the work or more (`_cheapest_parts`;
     `_late_parts`: or where a last round would hold few of them); the longest items come first."""
-    tiles, q_row, k_row = [], 0, 0
-    for q, kv in zip(ql, kl):
+    tiles, q_row = [], 0
+    for q, kv, k_row in zip(ql, kl, _behind(kl) if first is None else first):
         for m0 in range(0, q * group, TILE_ROWS):
             last = min(m0 + TILE_ROWS, q * group) - 1
             tiles.append((q_row, q, k_row, kv, m0, max(0, min(kv, last // group + kv - q + 1)) if causal else kv))
-        q_row, k_row = q_row + q, k_row + kv
+        q_row += q
     items, joins, ws = [], [], 0
     part = max(MIN_PART, -(-sum(t[5] for t in tiles) * kv_heads // BLOCKS))
     part = -(-part // 64) * 64
@@ -276,10 +286,14 @@ def _late_parts(ends: Sequence[int], kv_heads: int) -> List[int]:
 
 
 def attention_plan(q_lens: Sequence[int], kv_lens: Optional[Sequence[int]] = None, *, heads: int, kv_heads: Optional[int] = None, d: int,
-                   causal: bool = True, scale: Optional[float] = None, device: Union[str, torch.device] = "cuda") -> AttentionPlan:
+                   causal: bool = True, scale: Optional[float] = None, kv_first: Optional[Sequence[int]] = None,
+                   device: Union[str, torch.device] = "cuda") -> AttentionPlan:
     """The plan of :func:`attention_packed` over ``len(q_lens)`` sequences of ``q_lens[i]`` query and ``kv_lens[i]`` key rows (default: as
     many), host integers, zero allowed.  ``causal``: query i of a sequence sees keys j <= i + kv_len - q_len -- the new tokens stand at the
-    end of their keys.  ``scale``: of the scores, default d ** -0.5.  Made once per set of lengths and used for every layer.
+    end of their keys.  ``scale``: of the scores, default d ** -0.5.  ``kv_first``: the row of ``k`` / ``v`` at which each sequence's keys begin, default one
+    sequence behind the other; with it a cache keeps room behind every sequence, and sequences may share rows.  Made once per set of lengths and
+    used for every layer (lengths that grow need a plan per step: 100 us of host time for 16
+    requests of one token over 86 000 keys, 200 for 128, beside the GPU's work).
     The list is uploaded on the current stream without a wait for the work queued there; other streams wait for it at the plan's first use.
     A graph holds the plan that it was captured with: its replays come behind the upload (torch.cuda.graph waits for it), and no plan is
     made while a graph is captured."""
@@ -293,6 +307,12 @@ def attention_plan(q_lens: Sequence[int], kv_lens: Optional[Sequence[int]] = Non
     kl = ql if kv_lens is None else _lens(kv_lens, "kv_lens")
     if len(ql) != len(kl):
         raise ValueError(f"attention_plan: {len(ql)} query and {len(kl)} key lengths")
+    if kv_first is None:
+        first = _behind(kl)
+    else:
+        first = _integers(kv_first, "kv_first")
+        if len(first) != len(kl) or min(first) < 0 or max(f + n for f, n in zip(first, kl)) > _I32_MAX:
+            raise ValueError("attention_plan: kv_first: expected a row for each sequence, none negative, keys within 2^31 - 1 rows")
     if max(ql) * (heads // kv_heads) > _I32_MAX:
         raise ValueError("attention_plan: more than 2^31 - 1 (query, head) rows per key / value head")
     scale = d ** -0.5 if scale is None else float(scale)
@@ -304,7 +324,7 @@ def attention_plan(q_lens: Sequence[int], kv_lens: Optional[Sequence[int]] = Non
             raise ValueError("attention_plan: a plan's list comes from the host and cannot be part of a graph: make it before the capture")
         if dev.index is None:
             dev = torch.device("cuda", torch.cuda.current_device())
-    items, joins, ws_rows = _plan_items(ql, kl, heads // kv_heads, kv_heads, bool(causal), d)
+    items, joins, ws_rows = _plan_items(ql, kl, heads // kv_heads, kv_heads, bool(causal), d, first)
     # One upload, from pinned memory: from pageable memory the host would wait for all work queued on the stream.  (The allocator keeps the pinned
     # block until the copy is done.)
     table, ready = torch.tensor((items + joins) or [(0,) * 8], dtype=torch.int32, pin_memory=dev.type == "cuda").to(dev, non_blocking=True), None
@@ -312,7 +332,7 @@ def attention_plan(q_lens: Sequence[int], kv_lens: Optional[Sequence[int]] = Non
         ready = torch.cuda.Event()
         ready.record(torch.cuda.current_stream(dev))
     n = len(items)
-    return AttentionPlan(ql, kl, heads, kv_heads, d, bool(causal), scale, table[:n], table[n:n + len(joins)], max((j[6] for j in joins), default=0), ws_rows,
+    return AttentionPlan(ql, kl, first, heads, kv_heads, d, bool(causal), scale, table[:n], table[n:n + len(joins)], max((j[6] for j in joins), default=0), ws_rows,
                          ready)
 
 

@@ -168,6 +168,63 @@ def test_a_plan_during_a_capture_is_refused_before_anything_is_uploaded(monkeypa
         ops.attention_plan([1], [300], heads=1, d=64, device="cuda:0")
     assert ops.attention_plan([1], [300], heads=1, d=64, device="cpu").total_kv == 300
 
+def test_first_key_rows_of_a_plan():
+    from musev_amd import ops, token_ops
+    ok = dict(heads=4, kv_heads=2, d=64, device="cpu")
+    ql, kl, first = [1, 3, 0, 2], [700, 0, 5, 300], [1000, 9000, 3, 0]
+    plan = ops.attention_plan(ql, kl, kv_first=torch.tensor(first), **ok)
+    assert plan.kv_first == (1000, 9000, 3, 0) and plan.total_kv == 1700 and plan.total_q == 6
+    packed, placed = (token_ops._plan_items(ql, kl, 2, 2, True, 64, f) for f in (None, first))
+    assert packed[1:] == placed[1:]          # (joins know no key rows)
+    row = dict(zip([0, 700, 700, 705], first))
+    assert [(*i[:2], row[i[2]] if i[3] else 9000, *i[3:]) for i in packed[0]] == placed[0]
+    assert ops.attention_plan(ql, kl, **ok).kv_first == (0, 700, 700, 705) and ops.attention_plan(ql, kl, **ok).total_kv == 1005
+    assert ops.attention_plan([2], [0], kv_first=[7], **ok).total_kv == 0
+    for bad in ([1], [0, 0, 0, -1], [0, 0, 0, 2 ** 31 - 200]):
+        with pytest.raises(ValueError, match="kv_first"):
+            ops.attention_plan(ql, kl, kv_first=bad, **ok)
+    with pytest.raises(TypeError):
+        ops.attention_plan(ql, kl, kv_first=[0.5, 0, 0, 0], **ok)
+
+
+@gpu
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS)
+def test_attention_over_a_cache_that_grows(dt):
+    """a cache with room for every request: two tokens at once, then one per step, some requests idle; what lies in the room (NaN) is not seen"""
+    from musev_amd import ops
+    heads, kvh, d, room = 8, 2, 80, [1500, 64, 9, 700]
+    first = [sum(room[:i]) + 3 * i for i in range(4)]
+    lens = [1490, 0, 1, 600]
+    cache = [torch.full((sum(room) + 12, kvh * d), float("nan"), dtype=dt, device=DEV) for _ in range(2)]
+    for i, t in enumerate(cache):
+        for f, n in zip(first, lens):
+            t[f:f + n] = rnd((n, kvh * d), 5 + i, dt)
+    for step, new in enumerate(([2, 2, 2, 2], [1, 1, 1, 1], [1, 1, 0, 1], [0, 1, 1, 1], [1, 0, 0, 1])):
+        q, k, v = (rnd((sum(new), h * d), 10 * step + i, dt) for i, h in enumerate((heads, kvh, kvh)))
+        at = torch.tensor([f + n + j for f, n, m in zip(first, lens, new) for j in range(m)], device=DEV)
+        cache[0][at], cache[1][at] = k, v
+        lens = [n + m for n, m in zip(lens, new)]
+        got = ops.attention_packed(ops.attention_plan(new, lens, heads=heads, kv_heads=kvh, d=d, kv_first=first), q, *cache)
+        torch.cuda.synchronize()
+        rows = torch.tensor([f + j for f, n in zip(first, lens) for j in range(n)], device=DEV)
+        within(got, *attention_oracle(q, cache[0][rows], cache[1][rows], new, lens, heads, kvh, d, True), what=step)
+
+
+@gpu
+def test_requests_that_share_a_prefix_of_keys():
+    from musev_amd import ops
+    dt, heads, kvh, d = torch.float16, 4, 2, 64
+    ql, kl, first = [1, 3, 1], [900, 650, 650], [0, 0, 250]
+    q, k, v = rnd((5, heads * d), 1, dt), rnd((900, kvh * d), 2, dt), rnd((900, kvh * d), 3, dt)
+    plan = ops.attention_plan(ql, kl, heads=heads, kv_heads=kvh, d=d, kv_first=first)
+    assert plan.total_kv == 900
+    got = ops.attention_packed(plan, q, k, v)
+    torch.cuda.synchronize()
+    rows = torch.cat([torch.arange(f, f + n) for f, n in zip(first, kl)]).to(DEV)
+    within(got, *attention_oracle(q, k[rows], v[rows], ql, kl, heads, kvh, d, True))
+    with pytest.raises(ValueError, match="k "):
+        ops.attention_packed(plan, q, k[:899], v)
+
 
 # ---- rotary positions: several tokens per block, results and inputs past the caches ----------------------------------------------
 MANY = {   # tokens, heads, kv_heads, d, sections
