@@ -498,7 +498,11 @@ static int launch_gemm_i8_shape(const mv_gemm_i8_desc* d, hipStream_t st) {
     // 256 and the rest apart), K = 1280, N = 4096: 160 tiles 23.6 / 25.3 / -; 208 31.2 / 26.4 / -; 272 38.4 / 48.2 / 37.3; 352 47.3 / 48.9 / 41.4; 384 51.4 /
     // 48.9 / 43.3; 416 56.5 / 50.5 / 51.4; 640 86.3 / 76.6 / 71.5; 672 89.8 / 75.1 / 80.6.  K = 4096: 160 54.7 / 52.4 / -; 272 95.8 / 109.2 / 76.8; 384 130.6 /
     // 112.6 / 103.1; 400 - / 115.9 / 121.2.  K = 640: 160 16.9 / 18.1 / -; 272 26.4 / 34.1 / 26.8; 384 34.2 / 36.3 / 33.2; 416 37.4 / 36.5 / 37.3.
-    if (const int64_t all = tiles(256, 256); all >= 192) {
+    // They are taken where more than three quarters of their area is result: a tile costs the same however few of its columns or rows there are.
+    // Measured (us; 256 / the smaller tiles), 53 248 rows, K = 320 and 1280: N = 64 (a quarter) 12.4 / 6.5, 22.6 / 14.8; 128 13.8 / 9.4, 24.2 / 16.6; 264
+    // 26.5 / 23.0, 45.9 / 38.6; 320 24.6 / 18.9, 44.5 / 37.2; 192 and 384 (three quarters) 13.6 / 12.4, 23.5 / 23.0 and 24.9 / 21.7, 45.1 / 44.3; 416 24.8 / 24.5,
+    // 45.0 / 48.4; 224 13.2 / 15.7, 23.8 / 32.3; few rows, K = 1280, N = 51 200: 64 21.1 / 15.6; 300 43.0 / 41.7; 448 44.6 / 52.6.
+    if (const int64_t all = tiles(256, 256); all >= 192 && d->M * d->N > all * (256 * 256 / 4 * 3)) {
         constexpr int64_t CUS = 256;
         const int64_t cols = ((int64_t)d->N + 255) / 256, whole = all / CUS * CUS / cols, left = all - whole * cols;
         mv_gemm_i8_desc head = *d, tail = *d;

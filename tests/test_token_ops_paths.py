@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_token_ops import ROOT, DEV, DTYPES, IDS, attention_inputs, attention_oracle, gpu, half_step, norm_oracle, rnd, rotary_oracle, subnormal, within
+from test_token_ops import ROOT, DEV, DTYPES, IDS, attention_inputs, attention_oracle, gpu, half_step, linear_oracle, norm_oracle, rnd, rotary_oracle, subnormal, within
 from test_token_ops import on_cpu  # noqa: F401  (a fixture)
 
 
@@ -282,6 +282,23 @@ def test_gated_norm_of_inputs_past_the_last_cache(c, off, dt):
         ws, wh = norm_oracle(x0[a:e], f0[a:e], "layer", 0.75, None, pre, gate, scale, shift, torch.arange(a, e, device=DEV) // per)
         within(s[a:e], *ws, what=("s", c, a))
         within(h[a:e], *wh, what=("h", c, a))
+
+# ---- int8 projection: narrow and flat results --------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS)
+@pytest.mark.parametrize("m,k,n", [(49152, 200, 64), (49300, 130, 130), (26624, 320, 320), (26700, 100, 264), (25000, 150, 385), (60, 140, 49300), (300, 90, 25700)])
+def test_linear_i8_of_few_columns_or_rows(m, k, n, dt):
+    """many tiles of the largest size, mostly empty or just not"""
+    from musev_amd import ops
+    x = randn((m, k), 1, dt)
+    codes = torch.randint(-127, 128, (n, k), generator=torch.Generator().manual_seed(2), dtype=torch.int32).to(torch.int8).to(DEV)
+    ws = ((0.5 + torch.rand(n, generator=torch.Generator().manual_seed(3))) / (73 * math.sqrt(k))).to(DEV)
+    bias, w, res = rnd((n,), 3, dt), ops.pack_weight_i8(codes, ws), randn((m, n + 3), 4, dt)[:, 1:1 + n]
+    for r, act in ((None, ops.MV_ACT_SILU), (res, 0)):
+        got = ops.linear_i8(x, w, bias=bias, residual=r, act=act)
+        torch.cuda.synchronize()
+        for a in range(0, m, 8192):
+            within(got[a:a + 8192], *linear_oracle(x[a:a + 8192], codes, ws, bias, None if r is None else r[a:a + 8192], act == ops.MV_ACT_SILU), what=(m, k, n, a))
 
 
 # ---- refusals -----------------------------------------------------------------------------------------------------------------------
