@@ -124,8 +124,8 @@ def unet_flops(H, W, T, B, model="musev", n_vis=1, n_ip_tokens=4, text_tokens=77
 
 
 def kernel_source_hash() -> str:
-    """sha256 over the kernel sources the library is built from (musev_amd/csrc/*.hip, *.h, include/musev_hip.h): ties a PMC
-    measurement to the code it was taken on"""
+    """sha256 over the kernel sources the library is built from (musev_amd/csrc/*.hip, *.h, include/musev_hip.h) and the flags they are
+    compiled with (the FLAGS of musev_amd/csrc/build.sh): ties a PMC measurement to the code it was taken on"""
     import glob
     import hashlib
     hsh = hashlib.sha256()
@@ -135,6 +135,10 @@ def kernel_source_hash() -> str:
         hsh.update(os.path.basename(f).encode())
         with open(f, "rb") as fh:
             hsh.update(fh.read())
+    with open(os.path.join(ROOT, "musev_amd", "csrc", "build.sh"), "rb") as fh:
+        flags = [line for line in fh if line.startswith(b"FLAGS=")]
+    assert flags, "build.sh names no FLAGS"
+    hsh.update(b"".join(flags))
     return hsh.hexdigest()[:16]
 
 
@@ -142,7 +146,7 @@ def measured_traffic(workload: str):
     """HBM bytes of the GEMM family (gemm2_kernel + split-K reduce) PER DENOISE STEP from the PMC counters: collected offline by tools/gpu_profile.sh (rocprofv3 --pmc
     FETCH_SIZE / WRITE_SIZE in separate passes over this same bench command, gfx950 read correction x2 applied by
     tools/pmc_summary.py) and committed as profiles/hbm_traffic.json -- a counter pass cannot run inside the timed
-    process.  The file records the hash of the kernel sources it was measured on: a measurement of OTHER code is not
+    process.  The file records the hash of the kernel sources and flags it was measured on: a measurement of OTHER code is not
     reported (None), so `traffic` is reproducible from profiles/ or absent."""
     path = os.path.join(ROOT, "profiles", "hbm_traffic.json")
     try:
