@@ -13,6 +13,7 @@ if [ "$LIB" != "libmusev_hip.so" ]; then OBJ=build_${LIB%.so}; fi
 # from ordinary float code (its host pass warns that it does not know the feature)
 FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=fast -Xclang -target-feature -Xclang -packed-fp32-ops ${MV_EXTRA_FLAGS:-}"
 mkdir -p $OBJ
+if [ -n "${MV_REBUILD:-}" ]; then rm -f $OBJ/*.o; fi   # everything anew, whatever its age
 pids=()
 for f in lib gemm norm attention elementwise ffn tsa xab; do
   if [ ! -f $OBJ/$f.o ] || [ build.sh -nt $OBJ/$f.o ] || [ $f.hip -nt $OBJ/$f.o ] || [ common.h -nt $OBJ/$f.o ] || [ gemm_tuned.h -nt $OBJ/$f.o ] || [ ../../include/musev_hip.h -nt $OBJ/$f.o ]; then
