@@ -327,7 +327,8 @@ def attention_plan(q_lens: Sequence[int], kv_lens: Optional[Sequence[int]] = Non
     items, joins, ws_rows = _plan_items(ql, kl, heads // kv_heads, kv_heads, bool(causal), d, first)
     # One upload, from pinned memory: from pageable memory the host would wait for all work queued on the stream.  (The allocator keeps the pinned
     # block until the copy is done.)
-    table, ready = torch.tensor((items + joins) or [(0,) * 8], dtype=torch.int32, pin_memory=dev.type == "cuda").to(dev, non_blocking=True), None
+    table, ready = torch.tensor((items + joins) or [(0,) * 8], dtype=torch.int32, device="cpu", pin_memory=dev.type == "cuda"), None
+    table = table.to(dev, non_blocking=True)
     if dev.type == "cuda":
         ready = torch.cuda.Event()
         ready.record(torch.cuda.current_stream(dev))
@@ -399,7 +400,7 @@ def rotary_table(sections: Sequence[int], theta: float = 10000.0, *, shared: boo
             turns.append(theta ** -e / (2.0 * math.pi))
             axis.append(a)
     dev = torch.device(device)
-    return RotaryTable(torch.tensor(turns, dtype=torch.float64).to(dev), torch.tensor(axis, dtype=torch.int32).to(dev), len(sec))
+    return RotaryTable(torch.tensor(turns, dtype=torch.float64, device="cpu").to(dev), torch.tensor(axis, dtype=torch.int32, device="cpu").to(dev), len(sec))
 
 
 def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, table: RotaryTable, *, heads: int, kv_heads: Optional[int] = None,

@@ -225,6 +225,24 @@ def test_requests_that_share_a_prefix_of_keys():
     with pytest.raises(ValueError, match="k "):
         ops.attention_packed(plan, q, k[:899], v)
 
+def test_plans_and_tables_do_not_go_by_the_default_device():
+    from musev_amd import ops
+    with torch.device("meta"):
+        plan, table = ops.attention_plan([3, 700], heads=1, d=64, device="cpu"), ops.rotary_table([16, 8], device="cpu")
+    assert plan.device.type == table.device.type == "cpu"
+    assert [t.tolist() for t in plan._tensors] == [t.tolist() for t in ops.attention_plan([3, 700], heads=1, d=64, device="cpu")._tensors]
+
+
+@gpu
+def test_a_plan_beside_a_default_device():
+    from musev_amd import ops
+    with torch.device(DEV):
+        plan = ops.attention_plan([3, 700], heads=1, d=64)
+    q, k, v = attention_inputs([3, 700], [3, 700], 1, 1, 64, torch.float16, 1)
+    got = ops.attention_packed(plan, q, k, v)
+    torch.cuda.synchronize()
+    within(got, *attention_oracle(q, k, v, [3, 700], [3, 700], 1, 1, 64, True))
+
 
 # ---- rotary positions: several tokens per block, results and inputs past the caches ----------------------------------------------
 MANY = {   # tokens, heads, kv_heads, d, sections
