@@ -68,11 +68,6 @@ def _launch(entry: str, desc: bytes, dev: int, held: Sequence["_Held"] = ()) -> 
         check(status, entry)
 
 
-def _tangents() -> bool:
-    """a forward-mode level is open: tensors may carry tangents"""
-    return forward_ad._current_level >= 0
-
-
 def _no_gradients(name: str, t: torch.Tensor) -> None:
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name}: requires gradients, and this operator has none to give: call it under torch.no_grad() or detach the tensor")
@@ -92,7 +87,7 @@ def _matrix(t: torch.Tensor, name: str, dtype: Optional[torch.dtype] = None, dev
         raise ValueError(f"{name}: expected a CUDA {'fp16 | bf16' if dtype is None else dtype} tensor, got {t.dtype} on {t.device}")
     if dev is not None and t.get_device() != dev:
         raise ValueError(f"{name}: on {t.device}, the other tensors are on device {dev}")
-    if t.requires_grad or _tangents():
+    if t.requires_grad or forward_ad._current_level >= 0:   # (a level is open: tensors may carry tangents)
         _no_gradients(name, t)
     if rows <= 1:
         return rows, cols, cols
@@ -468,7 +463,7 @@ def _affine(t: Optional[torch.Tensor], name: str, c: int, dtype: torch.dtype, de
         return 0
     if t.dtype != dtype or t.get_device() != dev or not t.is_contiguous() or t.numel() != c:
         raise ValueError(f"{name}: expected a contiguous {dtype} tensor of {c} elements on device {dev}")
-    if t.requires_grad or _tangents():
+    if t.requires_grad or forward_ad._current_level >= 0:
         _no_gradients(name, t)
     return t.data_ptr()
 
@@ -587,7 +582,7 @@ def pack_weight_i8(codes: torch.Tensor, scale: torch.Tensor) -> Int8Rows:
         raise ValueError(f"pack_weight_i8: codes must be a CUDA int8 [N, K] tensor, K <= {_I8_MAX_K}")
     if scale.dtype != torch.float32 or scale.shape != (codes.shape[0],) or scale.device != codes.device:
         raise ValueError(f"pack_weight_i8: scale must be fp32 [{codes.shape[0]}] on {codes.device}")
-    if scale.requires_grad or _tangents():
+    if scale.requires_grad or forward_ad._current_level >= 0:
         _no_gradients("pack_weight_i8: scale", scale)
     n, k = codes.shape
     packed = torch.zeros((n, -(-k // 128) * 128), dtype=torch.int8, device=codes.device)
@@ -625,7 +620,7 @@ def _i8_result(what: str, m: int, w: Int8Rows, like: torch.Tensor, dtype, bias, 
         raise ValueError(f"{what}: weight on {w.device}, rows on {like.device}")
     if n < 1:
         raise ValueError(f"{what}: a weight without rows")
-    if w.scale.requires_grad or _tangents():
+    if w.scale.requires_grad or forward_ad._current_level >= 0:
         _no_gradients(f"{what}: scale", w.scale)
     pb = pr = ldr = 0
     if bias is not None:
@@ -651,7 +646,7 @@ def gemm_i8(a: Int8Rows, w: Int8Rows, *, bias: Optional[torch.Tensor] = None, re
     ``out`` may be ``residual`` itself."""
     if a.k != w.k:
         raise ValueError(f"gemm_i8: rows of {a.k}, weight of {w.k}")
-    if a.scale.requires_grad or _tangents():
+    if a.scale.requires_grad or forward_ad._current_level >= 0:
         _no_gradients("gemm_i8: scale", a.scale)
     pb, pr, po, ldr, ldo, out = _i8_result("gemm_i8", a.rows, w, a.codes, dtype, bias, residual, act, out)
     _launch("mv_gemm_i8", _pack_gemm(a._codes, w._codes, a._scale, w._scale, pb, pr, po, a.rows, w.rows, w.kp, a.kp, w.kp, ldr, ldo, act, _DTYPES[dtype]),
