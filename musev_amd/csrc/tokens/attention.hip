@@ -341,8 +341,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const mv_attn_packe
     // difference is formed first.
     const float c = score_factor(p.scale);
     auto weight = [&](float m, float top) __attribute__((always_inline)) {
-#pragma clang fp contract(off)
-        const float mc = m * c, tc = top * c;
+        float mc = m * c, tc = top * c;
+        MV_KEEP_ONE_REGISTER(mc);   // (rounded products: the compiler would fuse one of them into the difference)
+        MV_KEEP_ONE_REGISTER(tc);
         return __builtin_amdgcn_exp2f(fabsf(tc) > 0x1p12f ? (m - top) * c : mc - tc);
     };
     float mm = -3.0e38f, ll = 0.f;
