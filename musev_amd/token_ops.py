@@ -140,6 +140,15 @@ class _Held:
         self._dev = tensors[0].get_device()
         self._streams = {_raw_stream(self._dev)} if tensors[0].is_cuda else set()
 
+    def _made_of(self) -> tuple:
+        """the constructor's arguments: a copy (copy.deepcopy, pickle) is made anew, with the addresses of its own memory"""
+        raise NotImplementedError
+
+    def __reduce__(self):
+        if self._ready is not None and not torch.cuda.is_current_stream_capturing():   # (whoever copies the memory reads it on the current stream)
+            torch.cuda.current_stream(self.device).wait_event(self._ready)
+        return type(self), self._made_of()
+
     def _use(self, stream: int) -> None:
         # (first use on a stream) what was filled without a wait for it is waited for there, and the allocator may not hand the memory out again while
         # a launch there still reads it
@@ -156,7 +165,8 @@ class _Held:
 class AttentionPlan(_Held):
     """the work list of :func:`attention_packed` for one set of sequence lengths (:func:`attention_plan`)"""
 
-    def __init__(self, q_lens, kv_lens, kv_first, heads, kv_heads, d, causal, scale, items, joins, join_rows, ws_rows, ready=None):
+    def __init__(self, q_lens, kv_lens, heads, kv_heads, d, causal, scale, items, joins, join_rows, ws_rows, kv_first=None, ready=None):
+        kv_first = _behind(kv_lens) if kv_first is None else kv_first
         self.q_lens, self.kv_lens, self.kv_first = tuple(q_lens), tuple(kv_lens), tuple(kv_first)
         self.heads, self.kv_heads, self.d, self.causal, self.scale = heads, kv_heads, d, causal, scale
         self.total_q, self.total_kv = sum(q_lens), max((f + n for f, n in zip(kv_first, kv_lens) if n), default=0)   # (rows of q; of k and v)
@@ -164,6 +174,9 @@ class AttentionPlan(_Held):
         self._hold(items, joins, ready=ready)
         self._tables = items.data_ptr(), joins.data_ptr()
         self._workspace = 4 * ws_rows * kv_heads * (d + 2)   # mv_attention_packed_workspace_bytes
+
+    def _made_of(self) -> tuple:
+        return (self.q_lens, self.kv_lens, self.heads, self.kv_heads, self.d, self.causal, self.scale, *self._tensors, self.join_rows, self.ws_rows, self.kv_first)
 
 
 def _integers(v, name: str) -> List[int]:
@@ -328,8 +341,8 @@ def attention_plan(q_lens: Sequence[int], kv_lens: Optional[Sequence[int]] = Non
         ready = torch.cuda.Event()
         ready.record(torch.cuda.current_stream(dev))
     n = len(items)
-    return AttentionPlan(ql, kl, first, heads, kv_heads, d, bool(causal), scale, table[:n], table[n:n + len(joins)], max((j[6] for j in joins), default=0), ws_rows,
-                         ready)
+    return AttentionPlan(ql, kl, heads, kv_heads, d, bool(causal), scale, table[:n], table[n:n + len(joins)], max((j[6] for j in joins), default=0), ws_rows,
+                         first, ready)
 
 
 def attention_packed(plan: AttentionPlan, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -376,6 +389,9 @@ class RotaryTable(_Held):
         self.pairs, self.axes = turns.numel(), axes
         self._hold(turns, axis)
         self._turns, self._axis = turns.data_ptr(), axis.data_ptr()
+
+    def _made_of(self) -> tuple:
+        return (*self._tensors, self.axes)
 
 
 def rotary_table(sections: Sequence[int], theta: float = 10000.0, *, shared: bool = False, device: Union[str, torch.device] = "cuda") -> RotaryTable:
@@ -573,6 +589,9 @@ class Int8Rows(_Held):
         self.codes, self.scale, self.k, self.rows, self.kp = codes, scale, k, codes.shape[0], codes.shape[1]
         self._hold(codes, scale)
         self._codes, self._scale = codes.data_ptr(), scale.data_ptr()
+
+    def _made_of(self) -> tuple:
+        return self.codes, self.scale, self.k
 
 
 def pack_weight_i8(codes: torch.Tensor, scale: torch.Tensor) -> Int8Rows:

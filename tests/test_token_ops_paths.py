@@ -1,6 +1,8 @@
 """More of the token-transformer operators (musev_amd.token_ops): the forms that only large, split or unusual calls reach, and the refusals
 beside them.  Oracles and bounds are those of test_token_ops; a bound of its own is derived where it stands."""
+import copy
 import math
+import pickle
 
 import pytest
 import torch
@@ -317,6 +319,53 @@ def test_linear_i8_of_few_columns_or_rows(m, k, n, dt):
         torch.cuda.synchronize()
         for a in range(0, m, 8192):
             within(got[a:a + 8192], *linear_oracle(x[a:a + 8192], codes, ws, bias, None if r is None else r[a:a + 8192], act == ops.MV_ACT_SILU), what=(m, k, n, a))
+
+# ---- copies of plans, tables and weights --------------------------------------------------------------------------------------------
+COPIES = {"deepcopy": copy.deepcopy, "pickle": lambda x: pickle.loads(pickle.dumps(x)), "copy": copy.copy}
+
+
+@pytest.mark.parametrize("how", list(COPIES))
+def test_copies_hold_addresses_of_their_own_memory(how):
+    from musev_amd import ops
+    w = ops.Int8Rows(torch.arange(256, dtype=torch.int8).view(2, 128), torch.tensor([1.0, 2.0]), 100)
+    table = ops.rotary_table([16, 8], device="cpu")
+    plan = ops.attention_plan([1, 3], [5000, 7], kv_first=[9, 0], heads=4, kv_heads=2, d=64, device="cpu", scale=0.5, causal=False)
+    w2, table2, plan2 = (COPIES[how](x) for x in (w, table, plan))
+    assert (w2._codes, w2._scale) == (w2.codes.data_ptr(), w2.scale.data_ptr()) and torch.equal(w2.codes, w.codes) and torch.equal(w2.scale, w.scale) and w2.k == 100
+    assert (table2._turns, table2._axis) == tuple(t.data_ptr() for t in table2._tensors) and (table2.pairs, table2.axes) == (12, 2)
+    assert plan2._tables == tuple(t.data_ptr() for t in plan2._tensors)
+    skip = {"_tensors", "_tables", "_streams", "_ready"}
+    assert {k: v for k, v in vars(plan2).items() if k not in skip} == {k: v for k, v in vars(plan).items() if k not in skip}
+    for a, b in ((w, w2), (table, table2), (plan, plan2)):
+        assert all(torch.equal(x, y) for x, y in zip(a._tensors, b._tensors))
+        if how != "copy":
+            assert all(x.data_ptr() != y.data_ptr() for x, y in zip(a._tensors, b._tensors))
+
+
+@gpu
+def test_a_copy_outlives_what_it_was_copied_from():
+    from musev_amd import ops
+    dt, ql, kl, heads, kvh, d = torch.float16, [1, 3], [5000, 70], 4, 2, 64
+    q, k, v = attention_inputs(ql, kl, heads, kvh, d, dt, 1)
+    x = rnd((20, 200), 2, dt)
+    codes = torch.randint(-127, 128, (64, 200), generator=torch.Generator().manual_seed(3), dtype=torch.int32).to(torch.int8).to(DEV)
+    pos = torch.arange(20, dtype=torch.int32, device=DEV).view(20, 1)
+    first = [ops.attention_plan(ql, kl, heads=heads, kv_heads=kvh, d=d), ops.pack_weight_i8(codes, torch.full((64,), 0.01, device=DEV)), ops.rotary_table([200])]
+
+    def run(plan, w, table):
+        return ops.attention_packed(plan, q, k, v), ops.linear_i8(x, w), ops.rotary_axes(x, None, pos, table, heads=1, d=200)[0]
+    want = [t.clone() for t in run(*first)]
+    for how in ("deepcopy", "pickle"):
+        second = [COPIES[how](t) for t in first]
+        torch.cuda.synchronize()
+        for t in first[1:]:
+            for m in t._tensors:
+                m.fill_(0)        # (as another tensor in the freed memory would: no code, no turn)
+        assert second[0]._tables == tuple(t.data_ptr() for t in second[0]._tensors)
+        got = run(*second)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), how
+        first = second
 
 
 # ---- refusals -----------------------------------------------------------------------------------------------------------------------
